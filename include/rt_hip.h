@@ -322,6 +322,75 @@ int32_t rt_matmul(rt_ctx* ctx, int32_t dtype,
                   const int64_t* rhs_strides, int32_t rhs_contiguity,
                   void* dst, uint64_t dst_len, uint64_t b, uint64_t m, uint64_t k, uint64_t n);
 
+/* ---- gated linear recurrence -----------------------------------------------------------------------------------------
+ * No counterpart in the reference: the operator along a sequence next to the axis reductions.  Operands are row-major contiguous runs
+ * from element 0 of their buffers, viewed as (outer, steps, inner) like a reduction along a dim; the state runs along `steps`:
+ *     p[t] = 0 where reset[t], else h[t - 1];   h[-1] = state (0 when state is null)
+ *     RT_SCAN_LINEAR    h[t] = gate[t] * p[t] + x[t]                          (h[t] = x[t], the gate unused, where nothing precedes:
+ *                                                                              reset[t], or t = 0 without a state)
+ *     RT_SCAN_SIGMOID   h[t] = s * p[t] + (1 - s) * x[t],  s = 1 / (1 + exp(-gate[t]))
+ * `state` and `last` are (outer, inner); `reset` (RT_BOOL, non-zero = a new document starts at this step) is (outer, steps); each of
+ * the three may be null.  last = h[steps - 1]; for steps = 0 the state (zeros when null).  steps = 1 with state and last is the
+ * single-token form of serving; last may be the state buffer itself.  h may be x itself or gate itself; any other overlap of an
+ * output is RT_E_INVALID.  The state is held and summed in the tensor's own dtype (f32 / f64); how the steps are grouped for the
+ * sum depends on the sizes alone, so equal calls give equal bits.
+ *
+ * rt_gated_scan_backward: from dh (gradient of h) and dlast (gradient of last, null = 0), with a[t] the factor of p[t]:
+ *     D[t] = dh[t] + (reset[t + 1] ? 0 : a[t + 1] * D[t + 1]),   D[steps - 1] = dh[steps - 1] + dlast
+ *     RT_SCAN_LINEAR    dx = D,            dgate = D * p   (0 where nothing precedes)
+ *     RT_SCAN_SIGMOID   dx = (1 - s) * D,  dgate = D * (p - x) * s * (1 - s)
+ *     dstate = a[0] * D[0] (0 where reset[0]); dstate may be null
+ * h is what the forward pass wrote.  x is read by RT_SCAN_SIGMOID alone and may be null for RT_SCAN_LINEAR.  dx may be dh itself or
+ * x itself, dstate may be dlast itself.
+ * rt_gated_scan_backward_packed8: the same with x and h in the 8-bit form below (codes and exponents of the whole (outer, steps,
+ * inner) runs).  They enter d(gate) element by element and never the recurrence, so their rounding does not grow along the steps. */
+typedef enum rt_scan_form { RT_SCAN_LINEAR = 0, RT_SCAN_SIGMOID = 1 } rt_scan_form;
+int32_t rt_gated_scan(rt_ctx* ctx, int32_t dtype, int32_t form, const void* gate, uint64_t gate_len, const void* x, uint64_t x_len,
+                      const void* state, uint64_t state_len, const void* reset, uint64_t reset_len, void* h, uint64_t h_len,
+                      void* last, uint64_t last_len, uint64_t outer, uint64_t steps, uint64_t inner);
+int32_t rt_gated_scan_backward(rt_ctx* ctx, int32_t dtype, int32_t form, const void* gate, uint64_t gate_len, const void* x, uint64_t x_len,
+                               const void* h, uint64_t h_len, const void* state, uint64_t state_len, const void* reset, uint64_t reset_len,
+                               const void* dh, uint64_t dh_len, const void* dlast, uint64_t dlast_len, void* dgate, uint64_t dgate_len,
+                               void* dx, uint64_t dx_len, void* dstate, uint64_t dstate_len, uint64_t outer, uint64_t steps, uint64_t inner);
+int32_t rt_gated_scan_backward_packed8(rt_ctx* ctx, int32_t dtype, int32_t form, const void* gate, uint64_t gate_len,
+                                       const void* x_codes, uint64_t x_codes_len, const void* x_exps, uint64_t x_exps_len,
+                                       const void* h_codes, uint64_t h_codes_len, const void* h_exps, uint64_t h_exps_len,
+                                       const void* state, uint64_t state_len, const void* reset, uint64_t reset_len,
+                                       const void* dh, uint64_t dh_len, const void* dlast, uint64_t dlast_len, void* dgate, uint64_t dgate_len,
+                                       void* dx, uint64_t dx_len, void* dstate, uint64_t dstate_len, uint64_t outer, uint64_t steps, uint64_t inner);
+
+/* ---- activations held in 8 bits for the backward pass ------------------------------------------------------------------
+ * No counterpart in the reference, whose tape keeps whole copies.  A run of len f32 / f64 elements is held as len codes (RT_I8) and
+ * ceil(len / 32) exponent bytes (RT_U8), one for each 32 consecutive elements (the last group may be shorter):
+ *     M = max |x| of the group;  e = the least integer >= -119 with rint(M * 2^-e) <= 127;  byte = e + 127
+ *     code = rint(x * 2^-e), ties to even;     restored = code * 2^e
+ * so an element is off by at most half a step, 2^(e-1) <= M / 126.  A restored value has at most 7 significant bits: it is exact in
+ * f32 and f64.  Magnitudes below 2^-120 become 0.  A group that holds NaN or an infinity (f64: or a magnitude of 127.5 * 2^127 or
+ * more) has byte 255 and restores as NaN throughout, so a diverged run stays visible.
+ *   rt_pack8                  codes, exps = src[start .. start + len)
+ *   rt_unpack8                dst = restored
+ *   rt_pack8_unary            dst = op(src[start .. start + len)) and the 8-bit form of the source, in one pass; op is RT_U_SIGMOID,
+ *                             RT_U_SILU or RT_U_TANH and dst is bit for bit that of rt_unary_to (the gradients of relu and abs need
+ *                             signs only, which rounding to 8 bits would lose near 0)
+ *   rt_pack8_unary_backward   dst = upstream * op'(restored)
+ *   rt_pack8_matmul_backward  the weight gradient of y = x w:  dst[b] (k x n) = restored[b]^T (m x k, transposed) * upstream[b] (m x n)
+ *                             for every batch; codes and exps are those of the whole (b, m, k) run; dst is zero for m = 0
+ * Buffers are row-major runs from element 0.  dst of rt_pack8_unary may be src (start = 0), that of rt_pack8_unary_backward may be
+ * upstream; any other overlap of an output is RT_E_INVALID.  f32 products are summed in f32, f64 ones in f64, in an order that
+ * depends on the sizes alone. */
+#define RT_PACK8_GROUP 32
+int32_t rt_pack8(rt_ctx* ctx, int32_t dtype, const void* src, uint64_t src_len, uint64_t start, uint64_t len,
+                 void* codes, uint64_t codes_len, void* exps, uint64_t exps_len);
+int32_t rt_unpack8(rt_ctx* ctx, int32_t dtype, const void* codes, uint64_t codes_len, const void* exps, uint64_t exps_len, uint64_t len,
+                   void* dst, uint64_t dst_len);
+int32_t rt_pack8_unary(rt_ctx* ctx, int32_t dtype, int32_t op, const void* src, uint64_t src_len, uint64_t start, uint64_t len,
+                       void* dst, uint64_t dst_len, void* codes, uint64_t codes_len, void* exps, uint64_t exps_len);
+int32_t rt_pack8_unary_backward(rt_ctx* ctx, int32_t dtype, int32_t op, const void* codes, uint64_t codes_len, const void* exps,
+                                uint64_t exps_len, const void* upstream, uint64_t upstream_len, uint64_t len, void* dst, uint64_t dst_len);
+int32_t rt_pack8_matmul_backward(rt_ctx* ctx, int32_t dtype, const void* codes, uint64_t codes_len, const void* exps, uint64_t exps_len,
+                                 const void* upstream, uint64_t upstream_len, void* dst, uint64_t dst_len,
+                                 uint64_t b, uint64_t m, uint64_t k, uint64_t n);
+
 /* ---- strided gather (what TensorView::owned / contiguous need, core/tensor.rs:299-325: the reference issues one
  * copy_range_within per forward-contiguous run; this is the same result in one launch) ------------------------- */
 int32_t rt_gather(rt_ctx* ctx, int32_t dtype, const void* src, uint64_t src_len, uint64_t offset, int32_t rank,

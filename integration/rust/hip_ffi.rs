@@ -186,6 +186,34 @@ extern "C" {
                      lhs_shape: *const u64, lhs_strides: *const i64, lhs_contiguity: i32, rhs: *const c_void, rhs_len: u64,
                      rhs_offset: u64, rhs_rank: i32, rhs_shape: *const u64, rhs_strides: *const i64, rhs_contiguity: i32,
                      dst: *mut c_void, dst_len: u64, b: u64, m: u64, k: u64, n: u64) -> i32;
+    pub fn rt_gated_scan(ctx: *mut rt_ctx, dtype: i32, form: i32, gate: *const c_void, gate_len: u64, x: *const c_void,
+                         x_len: u64, state: *const c_void, state_len: u64, reset: *const c_void, reset_len: u64, h: *mut c_void,
+                         h_len: u64, last: *mut c_void, last_len: u64, outer: u64, steps: u64, inner: u64) -> i32;
+    pub fn rt_gated_scan_backward(ctx: *mut rt_ctx, dtype: i32, form: i32, gate: *const c_void, gate_len: u64, x: *const c_void,
+                                  x_len: u64, h: *const c_void, h_len: u64, state: *const c_void, state_len: u64,
+                                  reset: *const c_void, reset_len: u64, dh: *const c_void, dh_len: u64, dlast: *const c_void,
+                                  dlast_len: u64, dgate: *mut c_void, dgate_len: u64, dx: *mut c_void, dx_len: u64,
+                                  dstate: *mut c_void, dstate_len: u64, outer: u64, steps: u64, inner: u64) -> i32;
+    pub fn rt_gated_scan_backward_packed8(ctx: *mut rt_ctx, dtype: i32, form: i32, gate: *const c_void, gate_len: u64,
+                                          x_codes: *const c_void, x_codes_len: u64, x_exps: *const c_void, x_exps_len: u64,
+                                          h_codes: *const c_void, h_codes_len: u64, h_exps: *const c_void, h_exps_len: u64,
+                                          state: *const c_void, state_len: u64, reset: *const c_void, reset_len: u64,
+                                          dh: *const c_void, dh_len: u64, dlast: *const c_void, dlast_len: u64,
+                                          dgate: *mut c_void, dgate_len: u64, dx: *mut c_void, dx_len: u64, dstate: *mut c_void,
+                                          dstate_len: u64, outer: u64, steps: u64, inner: u64) -> i32;
+    pub fn rt_pack8(ctx: *mut rt_ctx, dtype: i32, src: *const c_void, src_len: u64, start: u64, len: u64, codes: *mut c_void,
+                    codes_len: u64, exps: *mut c_void, exps_len: u64) -> i32;
+    pub fn rt_unpack8(ctx: *mut rt_ctx, dtype: i32, codes: *const c_void, codes_len: u64, exps: *const c_void, exps_len: u64,
+                      len: u64, dst: *mut c_void, dst_len: u64) -> i32;
+    pub fn rt_pack8_unary(ctx: *mut rt_ctx, dtype: i32, op: i32, src: *const c_void, src_len: u64, start: u64, len: u64,
+                          dst: *mut c_void, dst_len: u64, codes: *mut c_void, codes_len: u64, exps: *mut c_void,
+                          exps_len: u64) -> i32;
+    pub fn rt_pack8_unary_backward(ctx: *mut rt_ctx, dtype: i32, op: i32, codes: *const c_void, codes_len: u64,
+                                   exps: *const c_void, exps_len: u64, upstream: *const c_void, upstream_len: u64, len: u64,
+                                   dst: *mut c_void, dst_len: u64) -> i32;
+    pub fn rt_pack8_matmul_backward(ctx: *mut rt_ctx, dtype: i32, codes: *const c_void, codes_len: u64, exps: *const c_void,
+                                    exps_len: u64, upstream: *const c_void, upstream_len: u64, dst: *mut c_void, dst_len: u64,
+                                    b: u64, m: u64, k: u64, n: u64) -> i32;
     pub fn rt_gather(ctx: *mut rt_ctx, dtype: i32, src: *const c_void, src_len: u64, offset: u64, rank: i32,
                      shape: *const u64, strides: *const i64, dst: *mut c_void, dst_len: u64) -> i32;
     pub fn rt_debug_check_view(offset: u64, rank: i32, shape: *const u64, strides: *const i64, len: u64, out_count: *mut u64,

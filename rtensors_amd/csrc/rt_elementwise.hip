@@ -9,6 +9,7 @@
 #include "rt_common.h"
 #include "rt_div128.h"
 #include "rt_math64.h"
+#include "rt_unary_math.h"
 
 #include <type_traits>
 
@@ -86,8 +87,6 @@ template <class T> __device__ __forceinline__ T one_of() {
 }
 
 // libm spellings per precision
-__device__ __forceinline__ float m_exp(float x) { return expf(x); }
-__device__ __forceinline__ double m_exp(double x) { return exp(x); }
 __device__ __forceinline__ float m_expm1(float x) { return expm1f(x); }
 __device__ __forceinline__ double m_expm1(double x) { return expm1(x); }
 __device__ __forceinline__ float m_log(float x) { return logf(x); }
@@ -162,33 +161,6 @@ __device__ __forceinline__ double atanh_ratio(double x) {
     return __builtin_fabs(x) < 1.0 ? q : a * rt_rcp_seed_f64(d);
 }
 
-// 1 / (1 + e) of sigmoid and silu, e = exp(-x) >= 0, and (a - b) / (a + b) of tanh, a = exp(x), b = exp(-x).  f64: the divisor is at
-// least 1, so the refined reciprocal (within an ulp) replaces the general division sequence, which is a third of these kernels'
-// arithmetic.  The ends of the range are patched by selects, with what the reference's formulas give there: 1 / (1 + inf) = 0;
-// (a - b) / (a + b) = +-1 exactly from |x| = 690 on (the smaller exponential is lost in the sum) and inf / inf = NaN once exp overflows.
-__device__ __forceinline__ float recip_1p(float e) { return 1.0f / (1.0f + e); }
-__device__ __forceinline__ double recip_1p(double e) {
-    const double d = 1.0 + e;
-    const double r = rt_rcp_f64(d);                              // NaN for d = inf (and for NaN)
-    return d == __builtin_inf() ? 0.0 : r;
-}
-__device__ __forceinline__ float tanh_ratio(float x, float a, float b) { return (a - b) / (a + b); }
-__device__ __forceinline__ double tanh_ratio(double x, double a, double b) {
-    const double t = a + b;
-    const double q = rt_quot_f64(a - b, t);
-    const double far = __builtin_copysign(1.0, x) + (t - t);     // t - t: 0 for a finite sum, NaN for inf and NaN
-    return __builtin_fabs(x) < 690.0 ? q : far;
-}
-// exp(-x) next to a = exp(x), for tanh, sinh and cosh.  f64: 1 / a from the refined reciprocal (within an ulp, as the library's
-// exponential is) at a quarter of a second exponential's instructions.  Where the refinement has no answer -- a = 0 and a = inf, the
-// exponential under- or overflowed -- the raw estimate has the right one (inf, 0).
-__device__ __forceinline__ float exp_neg(float x, float a) { return m_exp(-x); }
-__device__ __forceinline__ double exp_neg(double x, double a) {
-    const double seed = rt_rcp_seed_f64(a);
-    double r = __builtin_fma(__builtin_fma(-a, seed, 1.0), seed, seed);
-    r = __builtin_fma(__builtin_fma(-a, r, 1.0), r, r);
-    return r != r ? seed : r;
-}
 // sqrt(x^2 + 1) of asinh: the argument is at least 1, so the scaling and the zero / denormal handling of the general square root fall
 // away (within an ulp).
 __device__ __forceinline__ float sqrt_ge1(float a) { return sqrtf(a); }

@@ -26,6 +26,8 @@ UNARY = {n: i for i, n in enumerate(
     "neg relu sigmoid silu tanh abs sqrt ln expm1 ln1p floor ceil round trunc sin cos tan asin acos atan sinh cosh "
     "asinh acosh atanh rsqrt reciprocal square cube exp sign step abs_grad".split())}
 SCALAR = {n: i for i, n in enumerate("add sub mul div log log1p leaky_relu elu leaky_grad".split())}
+SCAN_FORM = {"linear": 0, "sigmoid": 1}                         # rt_scan_form
+PACK8_GROUP = 32                                                # elements that share an exponent byte
 CONTIGUITY = {"row_major": 0, "column_major": 1, "none": 2}     # core/meta.rs:744-750
 BINARY = {"add": 0, "sub": 1, "mul": 2, "div": 3}
 # ReductionOpTypes::get_code (ops/reduction/mod.rs:161-175) in the low byte; the payload of Variance / Stdev / Norm in the flag bits
@@ -62,6 +64,11 @@ def _value(dtype: int, value) -> np.ndarray:
     if dtype in (U128, I128):
         return np.frombuffer((int(value) & ((1 << 128) - 1)).to_bytes(16, "little"), dtype=V16).copy()
     return np.array([value], dtype=NP_DTYPE[dtype])
+
+
+def _pl(buf):
+    """(pointer, length) of an operand, (null, 0) for one that is left out."""
+    return (None, 0) if buf is None else (buf.ptr, buf.len)
 
 
 class HipBuf:
@@ -121,6 +128,12 @@ class Hip:
         p = C.c_void_p()
         _check(lib.rt_alloc_from_slice(self._ctx, dtype, src.ctypes.data_as(C.c_void_p), src.size, C.byref(p)))
         return HipBuf(self, p.value, src.size, dtype)
+
+    def borrow(self, ptr: int, length: int, dtype: int) -> HipBuf:
+        """`length` elements of device memory that something else owns (a buffer of another library, a part of a larger one): usable in
+        every call, never freed from here.  The owner keeps it alive, and orders its own work on it against this context's stream
+        (`sync()`, or its own wait, where another stream wrote it)."""
+        return HipBuf(None, ptr, length, dtype)
 
     def copy_from_slice(self, dst: HipBuf, src: np.ndarray):
         src = np.ascontiguousarray(src, dtype=NP_DTYPE[dst.dtype]).reshape(-1)
@@ -300,6 +313,83 @@ class Hip:
             elif kind >= 2:
                 arr[i].operand = st[2]
         _check(lib.rt_fused_chain(self._ctx, dtype, n, ptrs, lens, starts, length, len(steps), arr, dst.ptr, dst.len, dst_start))
+
+    # ---- gated linear recurrence (no counterpart in the trait) ---------------------------------------------------------------------------
+    def gated_scan(self, form: str, gate: HipBuf, x: HipBuf, h: HipBuf, outer: int, steps: int, inner: int, state: HipBuf = None,
+                   reset: HipBuf = None, last: HipBuf = None):
+        """rt_gated_scan: h[t] = a[t] * h[t - 1] + b[t] along `steps` of (outer, steps, inner); form "linear" (a = gate, b = x) or "sigmoid"
+        (a = sigmoid(gate), b = (1 - a) * x).  state / last: (outer, inner); reset: bool (outer, steps)."""
+        self._same("gated scan", gate.dtype, x, h, state, last)
+        self._code("gated scan", BOOL, reset)
+        _check(lib.rt_gated_scan(self._ctx, gate.dtype, SCAN_FORM[form], *_pl(gate), *_pl(x), *_pl(state), *_pl(reset), *_pl(h), *_pl(last),
+                                 outer, steps, inner))
+
+    def gated_scan_backward(self, form: str, gate: HipBuf, x: HipBuf, h: HipBuf, dh: HipBuf, dgate: HipBuf, dx: HipBuf, outer: int, steps: int,
+                            inner: int, state: HipBuf = None, reset: HipBuf = None, dlast: HipBuf = None, dstate: HipBuf = None):
+        """rt_gated_scan_backward: the gradients of gate, x and state; x may be None for form "linear"."""
+        self._same("gated scan backward", gate.dtype, x, h, dh, dgate, dx, state, dlast, dstate)
+        self._code("gated scan backward", BOOL, reset)
+        _check(lib.rt_gated_scan_backward(self._ctx, gate.dtype, SCAN_FORM[form], *_pl(gate), *_pl(x), *_pl(h), *_pl(state), *_pl(reset), *_pl(dh),
+                                          *_pl(dlast), *_pl(dgate), *_pl(dx), *_pl(dstate), outer, steps, inner))
+
+    def gated_scan_backward_packed8(self, form: str, gate: HipBuf, x8, h8, dh: HipBuf, dgate: HipBuf, dx: HipBuf, outer: int, steps: int, inner: int,
+                                    state: HipBuf = None, reset: HipBuf = None, dlast: HipBuf = None, dstate: HipBuf = None):
+        """The same with x and h as (codes, exps) pairs of their 8-bit form; x8 may be None for form "linear"."""
+        xc, xe = x8 if x8 is not None else (None, None)
+        hc, he = h8
+        self._same("gated scan backward", gate.dtype, dh, dgate, dx, state, dlast, dstate)
+        self._code("gated scan backward", BOOL, reset)
+        self._code("gated scan backward", I8, xc, hc)
+        self._code("gated scan backward", U8, xe, he)
+        _check(lib.rt_gated_scan_backward_packed8(self._ctx, gate.dtype, SCAN_FORM[form], *_pl(gate), *_pl(xc), *_pl(xe), *_pl(hc), *_pl(he), *_pl(state),
+                                                  *_pl(reset), *_pl(dh), *_pl(dlast), *_pl(dgate), *_pl(dx), *_pl(dstate), outer, steps, inner))
+
+    # ---- activations held in 8 bits (no counterpart in the trait): codes i8, exps u8 with one byte for each 32 elements ----------------------
+    def alloc_pack8(self, length: int) -> Tuple[HipBuf, HipBuf]:
+        return self.alloc_uninit(I8, length), self.alloc_uninit(U8, -(-length // PACK8_GROUP))
+
+    def pack8(self, src: HipBuf, start: int, length: int, codes: HipBuf, exps: HipBuf):
+        self._code("pack8", I8, codes)
+        self._code("pack8", U8, exps)
+        _check(lib.rt_pack8(self._ctx, src.dtype, *_pl(src), start, length, *_pl(codes), *_pl(exps)))
+
+    def unpack8(self, codes: HipBuf, exps: HipBuf, length: int, dst: HipBuf):
+        self._code("unpack8", I8, codes)
+        self._code("unpack8", U8, exps)
+        _check(lib.rt_unpack8(self._ctx, dst.dtype, *_pl(codes), *_pl(exps), length, *_pl(dst)))
+
+    def pack8_unary(self, op: str, src: HipBuf, start: int, length: int, dst: HipBuf, codes: HipBuf, exps: HipBuf):
+        """dst = op(src run) and the 8-bit form of the run in one pass; op is sigmoid, silu or tanh."""
+        self._same("pack8 unary", src.dtype, dst)
+        self._code("pack8 unary", I8, codes)
+        self._code("pack8 unary", U8, exps)
+        _check(lib.rt_pack8_unary(self._ctx, src.dtype, UNARY[op], *_pl(src), start, length, *_pl(dst), *_pl(codes), *_pl(exps)))
+
+    def pack8_unary_backward(self, op: str, codes: HipBuf, exps: HipBuf, upstream: HipBuf, length: int, dst: HipBuf):
+        """dst = upstream * op'(restored)."""
+        self._same("pack8 unary backward", dst.dtype, upstream)
+        self._code("pack8 unary backward", I8, codes)
+        self._code("pack8 unary backward", U8, exps)
+        _check(lib.rt_pack8_unary_backward(self._ctx, dst.dtype, UNARY[op], *_pl(codes), *_pl(exps), *_pl(upstream), length, *_pl(dst)))
+
+    def pack8_matmul_backward(self, codes: HipBuf, exps: HipBuf, upstream: HipBuf, dst: HipBuf, b: int, m: int, k: int, n: int):
+        """dst[b] (k x n) = restored[b]^T * upstream[b]: the weight gradient of a projection whose input (b, m, k) is held in 8 bits."""
+        self._same("pack8 matmul backward", dst.dtype, upstream)
+        self._code("pack8 matmul backward", I8, codes)
+        self._code("pack8 matmul backward", U8, exps)
+        _check(lib.rt_pack8_matmul_backward(self._ctx, dst.dtype, *_pl(codes), *_pl(exps), *_pl(upstream), *_pl(dst), b, m, k, n))
+
+    @staticmethod
+    def _same(what: str, dtype: int, *bufs):
+        for b in bufs:
+            if b is not None and b.dtype != dtype:
+                raise TensorError(2, f"{what}: operands of different dtypes")
+
+    @staticmethod
+    def _code(what: str, dtype: int, *bufs):
+        for b in bufs:
+            if b is not None and b.dtype != dtype:
+                raise TensorError(2, f"{what}: an operand has dtype code {b.dtype}, expected {dtype}")
 
     # ---- timing -----------------------------------------------------------------------------------------------------------
     def event(self):
