@@ -102,6 +102,7 @@ extern "C" int32_t rt_ctx_destroy(rt_ctx* ctx) {
         for (auto& kv : ctx->free_blocks) (void)hipFree(kv.second);
         for (auto& kv : ctx->live) (void)hipFree(kv.first);
         if (ctx->scratch) (void)hipFree(ctx->scratch);
+        if (ctx->chain) (void)hipFree(ctx->chain);
         if (ctx->blas && ctx->blas_destroy) (void)ctx->blas_destroy(ctx->blas);
         for (int i = 0; i < 4; ++i) {
             if (ctx->stage[i]) (void)hipHostFree(ctx->stage[i]);
@@ -226,6 +227,37 @@ __global__ __launch_bounds__(512) void rt_zero_tiled_kernel(rt_u32x4* p, size_t 
     if (!rt_tile_index(m, blockIdx.x, 512, threadIdx.x, nvec, &i)) return;
     const rt_u32x4 z = {0u, 0u, 0u, 0u};
     __builtin_nontemporal_store(z, p + i);
+}
+
+int32_t rt_chain_clear(rt_ctx* ctx) {
+    const size_t nvec = ctx->chain_bytes / sizeof(uint4), blocks = (nvec + 255) / 256;
+    hipLaunchKernelGGL(rt_zero_kernel, dim3((uint32_t)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, ctx->stream, (uint4*)ctx->chain, nvec);
+    RT_HIP(hipGetLastError());
+    return RT_OK;
+}
+
+int32_t rt_chain_room(rt_ctx* ctx, size_t bytes, void** out) {
+    if (bytes > ctx->chain_bytes) {
+        if (ctx->chain) {
+            RT_HIP(hipStreamSynchronize(ctx->stream));
+            RT_HIP(hipFree(ctx->chain));
+            ctx->chain = nullptr;
+            ctx->chain_bytes = 0;
+        }
+        const size_t cap = size_class(bytes < (1u << 20) ? (1u << 20) : bytes);
+        const hipError_t e = hipMalloc(&ctx->chain, cap);
+        if (e != hipSuccess) {
+            (void)hipGetLastError();
+            ctx->chain = nullptr;
+            return e == hipErrorOutOfMemory ? rt_fail(RT_E_OOM, "the workspace of %zu bytes for a split scan could not be allocated", cap) : rt_hip_fail(e, "hipMalloc(chain)");
+        }
+        ctx->chain_bytes = cap;
+        ctx->device_allocs += 1;
+        ctx->chain_launches = 0;
+        RT_TRY(rt_chain_clear(ctx));
+    }
+    *out = ctx->chain;
+    return RT_OK;
 }
 
 // ---- host <-> device transfers ----------------------------------------------------------------------------------------

@@ -9,12 +9,16 @@ constexpr int kSBlock = 256;
 // x and h of the backward pass: whole values or the 8-bit form
 template <class T> struct Whole {
     const T* p;
-    __device__ __forceinline__ T at(uint64_t i) const { return p[i]; }
+    // element i of the run that starts at `base` (wave-uniform; base + i does not leave the run, base alone may)
+    __device__ __forceinline__ T at(uint64_t base, uint32_t i) const { return __builtin_nontemporal_load(p + base + i); }
 };
 template <class T> struct Held {
     const int8_t* codes;
     const uint8_t* exps;
-    __device__ __forceinline__ T at(uint64_t i) const { return p8_value<T>(codes[i], exps[i / kP8Group]); }
+    __device__ __forceinline__ T at(uint64_t base, uint32_t i) const {
+        const uint64_t e = base + i;
+        return p8_value<T>(codes[e], exps[e / kP8Group]);
+    }
 };
 
 template <class T> struct ScanArgs {
@@ -69,20 +73,384 @@ __global__ __launch_bounds__(kSBlock) void scan_backward_columns_kernel(BackArgs
         const bool none = cut || (t == 0 && !a.state);
         const T d = a.dh[at] + carry;
         const T g = a.gate[at];
-        const T p = none ? (T)0 : (t == 0 ? a.state[col] : a.h.at(at - a.inner));
+        const T p = none ? (T)0 : (t == 0 ? a.state[col] : a.h.at(at - a.inner, 0));
         if constexpr (FORM == RT_SCAN_LINEAR) {
             a.dgate[at] = none ? (T)0 : d * p;
             a.dx[at] = d;
             carry = none ? (T)0 : g * d;
         } else {
             const RtGate<T> q = rt_gate_of(g);
-            const T x = a.x.at(at);
+            const T x = a.x.at(at, 0);
             a.dgate[at] = d * (p - x) * (q.s * q.r);
             a.dx[at] = q.r * d;
             carry = cut ? (T)0 : q.s * d;
         }
     }
     if (a.dstate) a.dstate[col] = carry;
+}
+
+// ---- tiles along the steps ---------------------------------------------------------------------------------------------------------
+// Two stretches of the recurrence join as (A1, H1), (A2, H2) -> (A1 A2, A2 H1 + H2): A is the product of a stretch's factors, H what
+// it ends at from a state of zero.  A block takes a tile of the steps for 64 columns, holds it in registers, and needs one thing from
+// the tiles before: the state it starts from.  So that the data are read once, the tiles of a column run in the same launch and hand
+// states on through words in memory: a tile publishes (A, H) as soon as it has them, and its end state once it knows its start; a
+// tile that starts looks at the kWindow tiles before it, takes the nearest end state that is there, and goes through the (A, H) from
+// there on.  An end state is always A * start + H of its own tile, however many tiles it was found over, so the bits do not depend on
+// which block ran when.
+//
+// Every wait ends: tiles are numbered by a counter as blocks start, all tiles a block waits for have lower numbers, so they have
+// started, and the lowest unfinished one waits for nobody.
+//
+// A word is 32 bits of a value and a tag, written and read as one 64-bit access at device scope: a word with the right tag is valid by
+// itself, with no order between words.  Tags hold the launch's number (counted on the device, so a replayed launch has one of its own)
+// and are never cleared between launches.
+struct ChainControl {
+    uint32_t ticket, done, epoch, pad[13];
+};
+struct Chain {
+    ChainControl* ctl;
+    uint64_t* words;
+    uint32_t tiles;          // along the steps
+    uint32_t lines;          // sets of columns that are chained on their own
+};
+constexpr uint32_t kAgg = 1, kEnd = 2;                           // what a slot holds: (A, H), or the end state in place of H
+constexpr int kWindow = 4;
+
+__device__ __forceinline__ void put_word(uint64_t* p, uint32_t bits, uint32_t tag) {
+    __hip_atomic_store(p, (uint64_t)tag << 32 | bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t get_word(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+template <class T> struct Slot {
+    static constexpr int kHalves = sizeof(T) / 4;
+    static constexpr uint32_t kWords = 2 * kHalves * 64;         // per tile: H and A of 64 lanes
+    uint64_t w[2 * kHalves];
+    static __device__ __forceinline__ uint64_t* at(const Chain& c, uint32_t item) { return c.words + (uint64_t)item * kWords; }
+    static __device__ __forceinline__ void put(uint64_t* base, int which, T v, uint32_t tag) {
+        if constexpr (kHalves == 1) {
+            put_word(base + which * 64, __builtin_bit_cast(uint32_t, v), tag);
+        } else {
+            const uint64_t b = __builtin_bit_cast(uint64_t, v);
+            put_word(base + (which * 2) * 64, (uint32_t)b, tag);
+            put_word(base + (which * 2 + 1) * 64, (uint32_t)(b >> 32), tag);
+        }
+    }
+    __device__ __forceinline__ void get(const uint64_t* base) {
+#pragma unroll
+        for (int k = 0; k < 2 * kHalves; ++k) w[k] = get_word(base + k * 64);
+    }
+    // 0: not there (yet); the halves of a value may come from two writes, then it is read again
+    __device__ __forceinline__ uint32_t kind(uint32_t epoch) const {
+        const uint32_t t = (uint32_t)(w[0] >> 32);
+        bool ok = (t >> 2) == epoch;
+        if constexpr (kHalves == 2) ok = ok && (uint32_t)(w[1] >> 32) == t;
+        const uint32_t k = t & 3u;
+        if (k == kAgg) {
+#pragma unroll
+            for (int j = kHalves; j < 2 * kHalves; ++j) ok = ok && (uint32_t)(w[j] >> 32) == (epoch << 2 | kAgg);
+        }
+        return ok ? k : 0u;
+    }
+    __device__ __forceinline__ T value(int which) const {
+        if constexpr (kHalves == 1) return __builtin_bit_cast(float, (uint32_t)w[which]);
+        else return __builtin_bit_cast(double, (uint64_t)(uint32_t)w[which * 2 + 1] << 32 | (uint32_t)w[which * 2]);
+    }
+};
+
+__device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
+__device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
+__device__ __forceinline__ bool finite(double v) { return __builtin_fabs(v) < __builtin_inf(); }
+
+// The end state of tile k - 1 for this lane's column: one wave, all lanes together.
+template <class T> __device__ T chain_start(const Chain& ch, uint32_t item, uint32_t k, uint32_t epoch, int lane) {
+    const int n = k < (uint32_t)kWindow ? (int)k : kWindow;      // tiles before this one that are looked at
+    for (;;) {
+        Slot<T> s[kWindow];
+#pragma unroll
+        for (int q = 0; q < kWindow; ++q)
+            if (q < n) s[q].get(Slot<T>::at(ch, item - (uint32_t)(q + 1) * ch.lines) + lane);
+        int found = -1;                                          // nearest tile with an end state, all nearer ones having (A, H)
+        bool open = true;
+#pragma unroll
+        for (int q = 0; q < kWindow; ++q) {
+            if (q < n) {
+                const uint32_t kind = s[q].kind(epoch);
+                if (open && kind == kEnd) found = q;
+                open = open && kind == kAgg;
+            }
+        }
+        if (__all(found >= 0)) {
+            T c = (T)0;
+#pragma unroll
+            for (int q = kWindow - 1; q >= 0; --q) {
+                if (q < n) {
+                    if (q == found) c = s[q].value(0);
+                    else if (q < found) c = fused(s[q].value(1), c, s[q].value(0));
+                }
+            }
+            return c;
+        }
+        __builtin_amdgcn_s_sleep(1);
+    }
+}
+
+template <class T, int W> struct JoinRoom {
+    T A[W][64], H[W][64], start[64];
+    uint32_t cut[W];
+    uint32_t item, epoch;
+};
+
+// Takes a number for the block (the block's index where nothing is chained) and the launch's number.
+template <class T, int W> __device__ __forceinline__ uint32_t take_item(const Chain& ch, JoinRoom<T, W>& room) {
+    if (ch.tiles == 1) return blockIdx.x;
+    if (threadIdx.x == 0) {
+        room.item = __hip_atomic_fetch_add(&ch.ctl->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        room.epoch = __hip_atomic_load(&ch.ctl->epoch, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & 0x3fffffffu;
+    }
+    __syncthreads();
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)room.item);
+}
+// The last block to end leaves the counters as the next launch needs them.  A block is past its own use of the counters here.
+__device__ __forceinline__ void leave_item(const Chain& ch) {
+    if (ch.tiles == 1 || threadIdx.x != 0) return;
+    const uint32_t items = ch.tiles * ch.lines;
+    if (__hip_atomic_fetch_add(&ch.ctl->done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == items - 1) {
+        __hip_atomic_store(&ch.ctl->ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&ch.ctl->done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_fetch_add(&ch.ctl->epoch, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+
+// Joins the W stretches of a tile (one a wave, in the order of the waves) with the tiles before it.  (A, H) of the wave's own stretch;
+// cut: nothing crosses the stretch (wave-uniform; A has no meaning then); first: the state before tile 0.  `run(start)` goes through
+// the stretch from its start state and returns the state it ends at; so does this function.
+//
+// A product of factors above 1 can leave the range while the states stay inside it (a start of zero, say).  Where one does, the tile's
+// stretches run one after the other and only its end state is published: the plain loop's result, at the plain loop's pace.
+template <class T, int W, class Run>
+__device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W>& room, uint32_t item, uint32_t k, T A, T H, bool cut, T first, Run run) {
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const bool last = k == ch.tiles - 1;
+    room.A[w][lane] = A;
+    room.H[w][lane] = H;
+    if (lane == 0) room.cut[w] = cut ? 1u : 0u;
+    __syncthreads();
+    const uint32_t epoch = ch.tiles == 1 ? 0u : (uint32_t)__builtin_amdgcn_readfirstlane((int)room.epoch);
+    T ta = (T)1, th = (T)0;
+    bool tcut = false, bad = false;
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+        const T av = room.A[v][lane], hv = room.H[v][lane];
+        if (room.cut[v]) {
+            th = hv;
+            tcut = true;
+        } else {
+            th = v == 0 ? hv : fused(av, th, hv);
+            bad = bad || !finite(av);
+            if (!tcut) {
+                ta = v == 0 ? av : ta * av;
+                bad = bad || !finite(ta);
+            }
+        }
+    }
+    const bool serial = __any(bad);                              // the same in all waves: they look at the same numbers
+    if (w == 0) {
+        uint64_t* slot = last ? nullptr : Slot<T>::at(ch, item) + lane;
+        T start = first;
+        if (!last && !serial) {
+            if (tcut) Slot<T>::put(slot, 0, th, epoch << 2 | kEnd);
+            else if (k == 0) Slot<T>::put(slot, 0, fused(ta, first, th), epoch << 2 | kEnd);
+            else {
+                Slot<T>::put(slot, 1, ta, epoch << 2 | kAgg);
+                Slot<T>::put(slot, 0, th, epoch << 2 | kAgg);
+            }
+        }
+        if (k > 0) {
+            start = chain_start<T>(ch, item, k, epoch, lane);
+            if (!last && !serial && !tcut) Slot<T>::put(slot, 0, fused(ta, start, th), epoch << 2 | kEnd);
+        }
+        room.start[lane] = start;
+    }
+    __syncthreads();
+    T end = (T)0;
+    for (int turn = 0; turn < (serial ? W : 1); ++turn) {
+        if (!serial || turn == w) {
+            T start = room.start[lane];
+            if (!serial) {
+                for (int v = 0; v < w; ++v) start = room.cut[v] ? room.H[v][lane] : fused(room.A[v][lane], start, room.H[v][lane]);
+            }
+            end = run(start);
+            if (serial) room.start[lane] = end;
+        }
+        if (serial) __syncthreads();
+    }
+    if (serial && w == 0 && !last) Slot<T>::put(Slot<T>::at(ch, item) + lane, 0, room.start[lane], epoch << 2 | kEnd);
+    return end;
+}
+
+// Bits 0 .. n - 1: whether the steps at flags[0], flags[stride], ... are reset.  n <= 64, all lanes of the wave.
+__device__ __forceinline__ uint64_t reset_bits(const uint8_t* flags, int64_t stride, int n, int lane) {
+    return __ballot(lane < n && flags[(int64_t)lane * stride] != 0);
+}
+
+// Copies of what a wave's second run through its steps takes from the first, which the compiler does not know to be the same: it would
+// keep every address and every condition of the first run in a register until the second.
+#define RT_APART                        \
+    int rn = n;                         \
+    uint64_t rcuts = cuts;              \
+    uint32_t rrow = row;                \
+    RT_PIN(rn);                         \
+    RT_PIN(rcuts);                      \
+    RT_PIN(rrow)
+
+// W waves of 64 columns, L steps each, in registers.  A wave that ends before its L steps, and lanes behind the last column, load what
+// the last step and the last column hold, and neither use nor store it.
+template <class T, int FORM, int W, int L>
+__global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain ch, uint32_t col_blocks) {
+    __shared__ JoinRoom<T, W> room;
+    const uint32_t item = take_item<T, W>(ch, room);
+    const uint32_t k = item / ch.lines, line = item - k * ch.lines, o = line / col_blocks;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t row = (uint32_t)a.inner, col0 = (line - o * col_blocks) * 64, col = col0 + lane;
+    const bool in = col < row;
+    const uint32_t lc = in ? lane : row - 1 - col0;
+    const uint64_t t0 = ((uint64_t)k * W + w) * L;
+    const int n = t0 >= a.steps ? 0 : (a.steps - t0 < (uint64_t)L ? (int)(a.steps - t0) : L);   // steps of this wave
+    const uint64_t base = ((uint64_t)o * a.steps + t0) * row + col0;                            // wave-uniform
+    const uint64_t sc = (uint64_t)o * row + col0 + lc;                                          // the column in (outer, inner)
+    T f[L], b[L], A = (T)1, H = (T)0;
+    uint64_t cuts = t0 == 0 && !a.state ? 1 : 0;
+    if (n) {
+        const T *gate = a.gate + base, *x = a.x + base;
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+            const uint32_t at = lc + (uint32_t)(j < n ? j : n - 1) * row;
+            f[j] = __builtin_nontemporal_load(gate + at);
+            b[j] = __builtin_nontemporal_load(x + at);
+        }
+        if (a.reset) cuts |= reset_bits(a.reset + (uint64_t)o * a.steps + t0, 1, n, lane);
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+            if constexpr (FORM == RT_SCAN_SIGMOID) {
+                const RtGate<T> q = rt_gate_of(f[j]);
+                f[j] = q.s;
+                b[j] = q.r * b[j];
+            }
+            if (j < n) {
+                H = j == 0 || (cuts >> j & 1) ? b[j] : fused(f[j], H, b[j]);
+                A = j == 0 ? f[j] : A * f[j];
+            }
+        }
+    }
+    const T first = k == 0 && a.state ? a.state[sc] : (T)0;
+    T* h = a.h + base;
+    const T end = join_tile<T, W>(ch, room, item, k, A, H, cuts != 0, first, [&](T p) {
+        RT_APART;
+        if (in) {
+#pragma unroll
+            for (int j = 0; j < L; ++j) {
+                if (j < rn) {
+                    p = rcuts >> j & 1 ? b[j] : fused(f[j], p, b[j]);
+                    __builtin_nontemporal_store(p, h + (uint32_t)(lane + j * rrow));
+                }
+            }
+        }
+        return p;
+    });
+    if (a.last && in && n && t0 + n == a.steps) a.last[sc] = end;
+    leave_item(ch);
+}
+
+// The same backward: position r counts from the last step.  A state's gradient D comes to a step from the one behind it (r - 1) times
+// that one's gate.
+template <class T, int FORM, class S, int W, int L>
+__global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, S> a, Chain ch, uint32_t col_blocks) {
+    __shared__ JoinRoom<T, W> room;
+    const uint32_t item = take_item<T, W>(ch, room);
+    const uint32_t k = item / ch.lines, line = item - k * ch.lines, o = line / col_blocks;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t row = (uint32_t)a.inner, col0 = (line - o * col_blocks) * 64, col = col0 + lane;
+    const bool in = col < row;
+    const uint32_t lc = in ? lane : row - 1 - col0;
+    const uint64_t r0 = ((uint64_t)k * W + w) * L;
+    const int n = r0 >= a.steps ? 0 : (a.steps - r0 < (uint64_t)L ? (int)(a.steps - r0) : L);
+    const uint64_t tl = n ? a.steps - 1 - r0 : 0, te = n ? tl + 1 - n : 0;                      // the wave's last and earliest step
+    const bool top = te == 0;
+    const uint64_t base = ((uint64_t)o * a.steps + te) * row + col0;                            // of the earliest step: j is n - 1 - j rows on
+    const uint64_t sc = (uint64_t)o * row + col0 + lc;
+    T g[L], up[L], hp[L], xv[L], s[L], f0 = (T)1, A = (T)1, H = (T)0;
+    uint64_t resets = 0, cuts = 0;                               // bit j: step j is reset; the step behind j is
+    if (n) {
+        const T *gate = a.gate + base, *dh = a.dh + base;
+        const T st = top && a.state ? a.state[sc] : (T)0;
+        if (r0 > 0) f0 = gate[lc + (uint32_t)n * row];           // the gate of the step behind j = 0
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+            const int q = j < n ? n - 1 - j : 0;
+            const uint32_t at = lc + (uint32_t)q * row;
+            g[j] = __builtin_nontemporal_load(gate + at);
+            up[j] = __builtin_nontemporal_load(dh + at);
+            if constexpr (FORM == RT_SCAN_SIGMOID) xv[j] = a.x.at(base, at);
+            hp[j] = top && q == 0 ? st : a.h.at(base - row, at);
+        }
+        if (a.reset) {
+            resets = reset_bits(a.reset + (uint64_t)o * a.steps + tl, -1, n, lane);
+            cuts = resets << 1;
+            if (r0 > 0 && a.reset[(uint64_t)o * a.steps + tl + 1]) cuts |= 1;
+            cuts &= (2ull << (n - 1)) - 1;
+        }
+        if constexpr (FORM == RT_SCAN_SIGMOID)
+            if (r0 > 0) f0 = rt_gate_of(f0).s;
+        T f = f0;
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+            s[j] = g[j];
+            if constexpr (FORM == RT_SCAN_SIGMOID) {
+                const RtGate<T> q = rt_gate_of(g[j]);
+                s[j] = q.s;
+                g[j] = q.r;
+            }
+            if (j < n) {
+                H = j == 0 || (cuts >> j & 1) ? up[j] : fused(f, H, up[j]);
+                A = j == 0 ? f : A * f;
+            }
+            f = s[j];
+        }
+    }
+    const T first = k == 0 && a.dlast ? a.dlast[sc] : (T)0;
+    T *dg = a.dgate + base, *dx = a.dx + base;
+    const T end = join_tile<T, W>(ch, room, item, k, A, H, cuts != 0, first, [&](T d) {
+        RT_APART;
+        uint64_t rresets = resets;
+        RT_PIN(rresets);
+        if (in) {
+#pragma unroll
+            for (int j = 0; j < L; ++j) {
+                if (j < rn) {
+                    d = rcuts >> j & 1 ? up[j] : fused(j == 0 ? f0 : s[j ? j - 1 : 0], d, up[j]);
+                    const bool none = rresets >> j & 1;
+                    const T p = none ? (T)0 : hp[j];
+                    const uint32_t at = lane + (uint32_t)(rn - 1 - j) * rrow;
+                    if constexpr (FORM == RT_SCAN_LINEAR) {
+                        const bool unused = none || (top && j == rn - 1 && !a.state);
+                        __builtin_nontemporal_store(unused ? (T)0 : d * p, dg + at);
+                        __builtin_nontemporal_store(d, dx + at);
+                    } else {
+                        __builtin_nontemporal_store(d * (p - xv[j]) * (s[j] * g[j]), dg + at);
+                        __builtin_nontemporal_store(g[j] * d, dx + at);
+                    }
+                }
+            }
+        }
+        return d;
+    });
+    if (a.dstate && in && n && top) {
+        const T g0 = a.gate[(uint64_t)o * a.steps * row + col];
+        const bool none = (a.reset && a.reset[(uint64_t)o * a.steps]) || (FORM == RT_SCAN_LINEAR && !a.state);
+        a.dstate[sc] = none ? (T)0 : (FORM == RT_SCAN_SIGMOID ? rt_gate_of(g0).s : g0) * end;
+    }
+    leave_item(ch);
 }
 
 // dst = src, or zeros: the states of a run of no steps
@@ -100,18 +468,60 @@ template <class T> int32_t no_steps(rt_ctx* ctx, const void* src, void* dst, uin
     return RT_OK;
 }
 
+// The chain of a launch: `tiles` along the steps for each of `lines` sets of columns; a workspace only where there is more than one tile.
+template <class T> int32_t make_chain(rt_ctx* ctx, uint64_t tiles, uint64_t lines, Chain* out) {
+    if (tiles >= (1ull << 31) / lines) return rt_fail(RT_E_INVALID, "gated scan: too long for one launch");
+    out->tiles = (uint32_t)tiles;
+    out->lines = (uint32_t)lines;
+    out->ctl = nullptr;
+    out->words = nullptr;
+    if (tiles == 1) return RT_OK;
+    void* p = nullptr;
+    RT_TRY(rt_chain_room(ctx, sizeof(ChainControl) + tiles * lines * Slot<T>::kWords * sizeof(uint64_t), &p));
+    out->ctl = (ChainControl*)p;
+    out->words = (uint64_t*)(out->ctl + 1);
+    // the 30 bits of the launch's number are cleared, and old tags with them, long before they come round
+    if (++ctx->chain_launches == 1u << 29) {
+        RT_TRY(rt_chain_clear(ctx));
+        ctx->chain_launches = 0;
+    }
+    return RT_OK;
+}
+
+constexpr int kWaves = 8;
+constexpr uint64_t kWideMost = 1ull << 22;      // inner: a wave's rows are addressed with 32-bit offsets; beyond it columns alone fill the card
 template <class T> int32_t forward_typed(rt_ctx* ctx, int form, const ScanArgs<T>& a) {
+    constexpr int L = sizeof(T) == 4 ? 32 : 16;
     const uint64_t cols = a.outer * a.inner;
-    if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_columns_kernel<T, RT_SCAN_LINEAR>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
-    else hipLaunchKernelGGL((scan_columns_kernel<T, RT_SCAN_SIGMOID>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
+    if (a.inner >= 32 && a.inner < kWideMost && a.steps > 8) {
+        const uint64_t cb = (a.inner + 63) / 64;
+        Chain ch;
+        RT_TRY(make_chain<T>(ctx, (a.steps + kWaves * L - 1) / (kWaves * L), a.outer * cb, &ch));
+        const dim3 grid(ch.tiles * ch.lines);
+        if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_wide_kernel<T, RT_SCAN_LINEAR, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
+        else hipLaunchKernelGGL((scan_wide_kernel<T, RT_SCAN_SIGMOID, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
+    } else {
+        if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_columns_kernel<T, RT_SCAN_LINEAR>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
+        else hipLaunchKernelGGL((scan_columns_kernel<T, RT_SCAN_SIGMOID>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
+    }
     RT_HIP(hipGetLastError());
     return RT_OK;
 }
 
 template <class T, class S> int32_t backward_typed(rt_ctx* ctx, int form, const BackArgs<T, S>& a) {
+    constexpr int L = sizeof(T) == 4 ? 16 : 8;
     const uint64_t cols = a.outer * a.inner;
-    if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_backward_columns_kernel<T, RT_SCAN_LINEAR, S>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
-    else hipLaunchKernelGGL((scan_backward_columns_kernel<T, RT_SCAN_SIGMOID, S>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
+    if (a.inner >= 32 && a.inner < kWideMost && a.steps > 8) {
+        const uint64_t cb = (a.inner + 63) / 64;
+        Chain ch;
+        RT_TRY(make_chain<T>(ctx, (a.steps + kWaves * L - 1) / (kWaves * L), a.outer * cb, &ch));
+        const dim3 grid(ch.tiles * ch.lines);
+        if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_backward_wide_kernel<T, RT_SCAN_LINEAR, S, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
+        else hipLaunchKernelGGL((scan_backward_wide_kernel<T, RT_SCAN_SIGMOID, S, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
+    } else {
+        if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_backward_columns_kernel<T, RT_SCAN_LINEAR, S>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
+        else hipLaunchKernelGGL((scan_backward_columns_kernel<T, RT_SCAN_SIGMOID, S>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
+    }
     RT_HIP(hipGetLastError());
     return RT_OK;
 }
