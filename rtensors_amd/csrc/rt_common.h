@@ -63,10 +63,9 @@ struct rt_ctx {
     // the next call that waits for the stream, and only when such a kernel was launched since the last look
     int32_t* fault_dev = nullptr;
     bool fault_pending = false;
-    // words through which the tiles of a split scan hand their states on (rt_scan.hip): a control block and the tiles' slots, zeroed
-    // when they are allocated and kept between calls
-    void* chain = nullptr;
-    size_t chain_bytes = 0;
+    // what the tiles of a split scan hand their states on through (rt_scan.hip): the lines' counters and the tiles' slots, zeroed when they
+    // are allocated and kept between calls
+    struct { void* p = nullptr; size_t bytes = 0; } chain[2];
     uint32_t chain_launches = 0;
     int num_cus = 256;
 };
@@ -81,8 +80,8 @@ int32_t rt_ctx_enter(rt_ctx* ctx);                                   // validate
 int32_t rt_alloc_bytes(rt_ctx* ctx, size_t bytes, void** out);       // caller holds ctx->mu
 int32_t rt_free_locked(rt_ctx* ctx, void* p);
 int32_t rt_scratch(rt_ctx* ctx, size_t bytes, void** out);           // caller holds ctx->mu; growth counts as a device allocation
-int32_t rt_chain_room(rt_ctx* ctx, size_t bytes, void** out);        // likewise; zeroes what it allocates and nothing else
-int32_t rt_chain_clear(rt_ctx* ctx);                                 // zeroes all of it
+int32_t rt_chain_room(rt_ctx* ctx, int which, size_t bytes, void** out);   // likewise; zeroes what it allocates and nothing else
+int32_t rt_chain_clear(rt_ctx* ctx, int which);                      // zeroes all of it
 // Device address of the built-in workspace of rt_reduce_nd_static on `device`, which must be current (looked up once per device).
 int32_t rt_static_scratch_init(int device, void** out);
 // After the stream has been waited for: RT_E_ARITH if an integer division launched since the last look met a fault, and the fault

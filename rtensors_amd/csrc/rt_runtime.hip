@@ -102,7 +102,8 @@ extern "C" int32_t rt_ctx_destroy(rt_ctx* ctx) {
         for (auto& kv : ctx->free_blocks) (void)hipFree(kv.second);
         for (auto& kv : ctx->live) (void)hipFree(kv.first);
         if (ctx->scratch) (void)hipFree(ctx->scratch);
-        if (ctx->chain) (void)hipFree(ctx->chain);
+        for (auto& c : ctx->chain)
+            if (c.p) (void)hipFree(c.p);
         if (ctx->blas && ctx->blas_destroy) (void)ctx->blas_destroy(ctx->blas);
         for (int i = 0; i < 4; ++i) {
             if (ctx->stage[i]) (void)hipHostFree(ctx->stage[i]);
@@ -229,34 +230,34 @@ __global__ __launch_bounds__(512) void rt_zero_tiled_kernel(rt_u32x4* p, size_t 
     __builtin_nontemporal_store(z, p + i);
 }
 
-int32_t rt_chain_clear(rt_ctx* ctx) {
-    const size_t nvec = ctx->chain_bytes / sizeof(uint4), blocks = (nvec + 255) / 256;
-    hipLaunchKernelGGL(rt_zero_kernel, dim3((uint32_t)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, ctx->stream, (uint4*)ctx->chain, nvec);
+int32_t rt_chain_clear(rt_ctx* ctx, int which) {
+    const size_t nvec = ctx->chain[which].bytes / sizeof(uint4), blocks = (nvec + 255) / 256;
+    hipLaunchKernelGGL(rt_zero_kernel, dim3((uint32_t)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, ctx->stream, (uint4*)ctx->chain[which].p, nvec);
     RT_HIP(hipGetLastError());
     return RT_OK;
 }
 
-int32_t rt_chain_room(rt_ctx* ctx, size_t bytes, void** out) {
-    if (bytes > ctx->chain_bytes) {
-        if (ctx->chain) {
+int32_t rt_chain_room(rt_ctx* ctx, int which, size_t bytes, void** out) {
+    auto& c = ctx->chain[which];
+    if (bytes > c.bytes) {
+        if (c.p) {
             RT_HIP(hipStreamSynchronize(ctx->stream));
-            RT_HIP(hipFree(ctx->chain));
-            ctx->chain = nullptr;
-            ctx->chain_bytes = 0;
+            RT_HIP(hipFree(c.p));
+            c.p = nullptr;
+            c.bytes = 0;
         }
         const size_t cap = size_class(bytes < (1u << 20) ? (1u << 20) : bytes);
-        const hipError_t e = hipMalloc(&ctx->chain, cap);
+        const hipError_t e = hipMalloc(&c.p, cap);
         if (e != hipSuccess) {
             (void)hipGetLastError();
-            ctx->chain = nullptr;
+            c.p = nullptr;
             return e == hipErrorOutOfMemory ? rt_fail(RT_E_OOM, "the workspace of %zu bytes for a split scan could not be allocated", cap) : rt_hip_fail(e, "hipMalloc(chain)");
         }
-        ctx->chain_bytes = cap;
+        c.bytes = cap;
         ctx->device_allocs += 1;
-        ctx->chain_launches = 0;
-        RT_TRY(rt_chain_clear(ctx));
+        RT_TRY(rt_chain_clear(ctx, which));
     }
-    *out = ctx->chain;
+    *out = c.p;
     return RT_OK;
 }
 

@@ -98,23 +98,25 @@ __global__ __launch_bounds__(kSBlock) void scan_backward_columns_kernel(BackArgs
 // there on.  An end state is always A * start + H of its own tile, however many tiles it was found over, so the bits do not depend on
 // which block ran when.
 //
-// Every wait ends: tiles are numbered by a counter as blocks start, all tiles a block waits for have lower numbers, so they have
-// started, and the lowest unfinished one waits for nobody.
+// Every wait ends: the tiles of a line of columns are numbered by the line's counter as blocks start, all tiles a block waits for have
+// lower numbers, so they have started, and the lowest unfinished one waits for nobody.  (One counter for the whole launch costs 45 ns a
+// block, an atomic operation on one address from eight XCDs: 16384 tiles took 1441 us.)
 //
 // A word is 32 bits of a value and a tag, written and read as one 64-bit access at device scope: a word with the right tag is valid by
-// itself, with no order between words.  Tags hold the launch's number (counted on the device, so a replayed launch has one of its own)
-// and are never cleared between launches.
-struct ChainControl {
-    uint32_t ticket, done, epoch, pad[13];
-};
+// itself, with no order between words.  Tags hold the launch's number and are not cleared between launches.  The number comes from the
+// host, so a launch must not be replayed from a graph; the context's stream is never under capture, and make_chain refuses it.
 struct Chain {
-    ChainControl* ctl;
+    uint32_t* tickets;       // one counter a line, 64 bytes apart, 0 between launches
     uint64_t* words;
     uint32_t tiles;          // along the steps
     uint32_t lines;          // sets of columns that are chained on their own
+    uint32_t epoch;          // the launch's number, 30 bits
 };
+constexpr uint32_t kTicketPitch = 16;
 constexpr uint32_t kAgg = 1, kEnd = 2;                           // what a slot holds: (A, H), or the end state in place of H
-constexpr int kWindow = 4;
+#ifndef RT_WIN
+#define RT_WIN 16
+#endif
 
 __device__ __forceinline__ void put_word(uint64_t* p, uint32_t bits, uint32_t tag) {
     __hip_atomic_store(p, (uint64_t)tag << 32 | bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -162,64 +164,80 @@ __device__ __forceinline__ double fused(double a, double b, double c) { return _
 __device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
 __device__ __forceinline__ bool finite(double v) { return __builtin_fabs(v) < __builtin_inf(); }
 
-// The end state of tile k - 1 for this lane's column: one wave, all lanes together.
-template <class T> __device__ T chain_start(const Chain& ch, uint32_t item, uint32_t k, uint32_t epoch, int lane) {
-    const int n = k < (uint32_t)kWindow ? (int)k : kWindow;      // tiles before this one that are looked at
-    for (;;) {
-        Slot<T> s[kWindow];
-#pragma unroll
-        for (int q = 0; q < kWindow; ++q)
-            if (q < n) s[q].get(Slot<T>::at(ch, item - (uint32_t)(q + 1) * ch.lines) + lane);
-        int found = -1;                                          // nearest tile with an end state, all nearer ones having (A, H)
-        bool open = true;
-#pragma unroll
-        for (int q = 0; q < kWindow; ++q) {
-            if (q < n) {
-                const uint32_t kind = s[q].kind(epoch);
-                if (open && kind == kEnd) found = q;
-                open = open && kind == kAgg;
-            }
-        }
-        if (__all(found >= 0)) {
-            T c = (T)0;
-#pragma unroll
-            for (int q = kWindow - 1; q >= 0; --q) {
-                if (q < n) {
-                    if (q == found) c = s[q].value(0);
-                    else if (q < found) c = fused(s[q].value(1), c, s[q].value(0));
-                }
-            }
-            return c;
-        }
-        __builtin_amdgcn_s_sleep(1);
-    }
-}
-
 template <class T, int W> struct JoinRoom {
+    static constexpr int kWindow = sizeof(T) == 4 ? RT_WIN : RT_WIN / 2;      // tiles before its own that a tile looks at
     T A[W][64], H[W][64], start[64];
+    T winA[kWindow][64], winH[kWindow][64];
+    uint64_t ends[kWindow];
     uint32_t cut[W];
-    uint32_t item, epoch;
+    uint32_t tile;
+    int found;
 };
 
-// Takes a number for the block (the block's index where nothing is chained) and the launch's number.
-template <class T, int W> __device__ __forceinline__ uint32_t take_item(const Chain& ch, JoinRoom<T, W>& room) {
-    if (ch.tiles == 1) return blockIdx.x;
-    if (threadIdx.x == 0) {
-        room.item = __hip_atomic_fetch_add(&ch.ctl->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        room.epoch = __hip_atomic_load(&ch.ctl->epoch, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & 0x3fffffffu;
+// The end state of tile k - 1 for this lane's column, for all waves of the block.  Waiting is done by one wave on one word of each of the
+// tiles in the window, read by one lane each: polling whole slots takes the bandwidth that the tiles being waited for need.  Then the
+// waves read the slots between them, again where not all of their words are there yet, and go through them from the farthest.
+template <class T, int W> __device__ __forceinline__ T chain_start(const Chain& ch, JoinRoom<T, W>& room, uint32_t item, uint32_t k, int w, int lane) {
+    constexpr int kWindow = JoinRoom<T, W>::kWindow, kEach = (kWindow + W - 1) / W;
+    if (w == 0) {
+        const int n = k < (uint32_t)kWindow ? (int)k : kWindow;
+        int found;                                               // nearest tile with an end state, all nearer ones having (A, H)
+        for (;;) {
+            uint32_t tag = 0;
+            if (lane < n) tag = (uint32_t)(get_word(Slot<T>::at(ch, item - (uint32_t)(lane + 1) * ch.lines)) >> 32);
+            const bool mine = lane < n && (tag >> 2) == ch.epoch;
+            const uint64_t ends = __ballot(mine && (tag & 3u) == kEnd), aggs = __ballot(mine && (tag & 3u) == kAgg);
+            found = ends ? (int)__builtin_ctzll(ends) : -1;
+            if (found >= 0 && (~aggs & ((1ull << found) - 1)) == 0) break;
+            __builtin_amdgcn_s_sleep(2);
+        }
+        if (lane == 0) room.found = found;
     }
     __syncthreads();
-    return (uint32_t)__builtin_amdgcn_readfirstlane((int)room.item);
-}
-// The last block to end leaves the counters as the next launch needs them.  A block is past its own use of the counters here.
-__device__ __forceinline__ void leave_item(const Chain& ch) {
-    if (ch.tiles == 1 || threadIdx.x != 0) return;
-    const uint32_t items = ch.tiles * ch.lines;
-    if (__hip_atomic_fetch_add(&ch.ctl->done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == items - 1) {
-        __hip_atomic_store(&ch.ctl->ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(&ch.ctl->done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_fetch_add(&ch.ctl->epoch, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int found = __builtin_amdgcn_readfirstlane(room.found);
+    Slot<T> s[kEach];
+    for (;;) {
+        bool ok = true;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (w + i * W <= found) s[i].get(Slot<T>::at(ch, item - (uint32_t)(w + i * W + 1) * ch.lines) + lane);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (w + i * W <= found) {
+                const uint32_t kind = s[i].kind(ch.epoch);
+                ok = ok && (kind == kEnd || (kind == kAgg && w + i * W < found));
+            }
+        if (__all(ok)) break;
+        __builtin_amdgcn_s_sleep(1);
     }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int q = w + i * W;
+        if (q <= found) {
+            // an end state may have taken the place of a nearer tile's (A, H) meanwhile
+            const uint64_t ends = __ballot(s[i].kind(ch.epoch) == kEnd);
+            room.winH[q][lane] = s[i].value(0);
+            room.winA[q][lane] = s[i].value(1);
+            if (lane == 0) room.ends[q] = ends;
+        }
+    }
+    __syncthreads();
+    T c = (T)0;
+    for (int q = found; q >= 0; --q) c = room.ends[q] >> lane & 1 ? room.winH[q][lane] : fused(room.winA[q][lane], c, room.winH[q][lane]);
+    return c;
+}
+
+// The block's tile among those of its line; whoever takes the last one leaves the counter as the next launch needs it.
+template <class T, int W> __device__ __forceinline__ uint32_t take_tile(const Chain& ch, uint32_t line, JoinRoom<T, W>& room) {
+    if (ch.tiles == 1) return 0;
+    if (threadIdx.x == 0) {
+        uint32_t* c = ch.tickets + (uint64_t)line * kTicketPitch;
+        const uint32_t t = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (t == ch.tiles - 1) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        room.tile = t;
+    }
+    __syncthreads();
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)room.tile);
 }
 
 // Joins the W stretches of a tile (one a wave, in the order of the waves) with the tiles before it.  (A, H) of the wave's own stretch;
@@ -236,7 +254,7 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W>& room, ui
     room.H[w][lane] = H;
     if (lane == 0) room.cut[w] = cut ? 1u : 0u;
     __syncthreads();
-    const uint32_t epoch = ch.tiles == 1 ? 0u : (uint32_t)__builtin_amdgcn_readfirstlane((int)room.epoch);
+    const uint32_t epoch = ch.epoch;
     T ta = (T)1, th = (T)0;
     bool tcut = false, bad = false;
 #pragma unroll
@@ -255,29 +273,29 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W>& room, ui
         }
     }
     const bool serial = __any(bad);                              // the same in all waves: they look at the same numbers
-    if (w == 0) {
-        uint64_t* slot = last ? nullptr : Slot<T>::at(ch, item) + lane;
-        T start = first;
-        if (!last && !serial) {
-            if (tcut) Slot<T>::put(slot, 0, th, epoch << 2 | kEnd);
-            else if (k == 0) Slot<T>::put(slot, 0, fused(ta, first, th), epoch << 2 | kEnd);
-            else {
-                Slot<T>::put(slot, 1, ta, epoch << 2 | kAgg);
-                Slot<T>::put(slot, 0, th, epoch << 2 | kAgg);
-            }
+    uint64_t* slot = last ? nullptr : Slot<T>::at(ch, item) + lane;
+    T start = first;
+    if (w == 0 && !last && !serial) {
+        if (tcut) Slot<T>::put(slot, 0, th, epoch << 2 | kEnd);
+        else if (k == 0) Slot<T>::put(slot, 0, fused(ta, first, th), epoch << 2 | kEnd);
+        else {
+            Slot<T>::put(slot, 1, ta, epoch << 2 | kAgg);
+            Slot<T>::put(slot, 0, th, epoch << 2 | kAgg);
         }
-        if (k > 0) {
-            start = chain_start<T>(ch, item, k, epoch, lane);
-            if (!last && !serial && !tcut) Slot<T>::put(slot, 0, fused(ta, start, th), epoch << 2 | kEnd);
-        }
-        room.start[lane] = start;
     }
-    __syncthreads();
+    if (k > 0) {
+        start = chain_start<T, W>(ch, room, item, k, w, lane);
+        if (w == 0 && !last && !serial && !tcut) Slot<T>::put(slot, 0, fused(ta, start, th), epoch << 2 | kEnd);
+    }
+    if (serial) {
+        if (w == 0) room.start[lane] = start;
+        __syncthreads();
+    }
     T end = (T)0;
     for (int turn = 0; turn < (serial ? W : 1); ++turn) {
         if (!serial || turn == w) {
-            T start = room.start[lane];
-            if (!serial) {
+            if (serial) start = room.start[lane];
+            else {
                 for (int v = 0; v < w; ++v) start = room.cut[v] ? room.H[v][lane] : fused(room.A[v][lane], start, room.H[v][lane]);
             }
             end = run(start);
@@ -285,7 +303,7 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W>& room, ui
         }
         if (serial) __syncthreads();
     }
-    if (serial && w == 0 && !last) Slot<T>::put(Slot<T>::at(ch, item) + lane, 0, room.start[lane], epoch << 2 | kEnd);
+    if (serial && w == 0 && !last) Slot<T>::put(slot, 0, room.start[lane], epoch << 2 | kEnd);
     return end;
 }
 
@@ -309,8 +327,7 @@ __device__ __forceinline__ uint64_t reset_bits(const uint8_t* flags, int64_t str
 template <class T, int FORM, int W, int L>
 __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain ch, uint32_t col_blocks) {
     __shared__ JoinRoom<T, W> room;
-    const uint32_t item = take_item<T, W>(ch, room);
-    const uint32_t k = item / ch.lines, line = item - k * ch.lines, o = line / col_blocks;
+    const uint32_t line = blockIdx.x % ch.lines, k = take_tile<T, W>(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t row = (uint32_t)a.inner, col0 = (line - o * col_blocks) * 64, col = col0 + lane;
     const bool in = col < row;
@@ -359,7 +376,6 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
         return p;
     });
     if (a.last && in && n && t0 + n == a.steps) a.last[sc] = end;
-    leave_item(ch);
 }
 
 // The same backward: position r counts from the last step.  A state's gradient D comes to a step from the one behind it (r - 1) times
@@ -367,8 +383,7 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
 template <class T, int FORM, class S, int W, int L>
 __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, S> a, Chain ch, uint32_t col_blocks) {
     __shared__ JoinRoom<T, W> room;
-    const uint32_t item = take_item<T, W>(ch, room);
-    const uint32_t k = item / ch.lines, line = item - k * ch.lines, o = line / col_blocks;
+    const uint32_t line = blockIdx.x % ch.lines, k = take_tile<T, W>(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t row = (uint32_t)a.inner, col0 = (line - o * col_blocks) * 64, col = col0 + lane;
     const bool in = col < row;
@@ -450,7 +465,6 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
         const bool none = (a.reset && a.reset[(uint64_t)o * a.steps]) || (FORM == RT_SCAN_LINEAR && !a.state);
         a.dstate[sc] = none ? (T)0 : (FORM == RT_SCAN_SIGMOID ? rt_gate_of(g0).s : g0) * end;
     }
-    leave_item(ch);
 }
 
 // dst = src, or zeros: the states of a run of no steps
@@ -473,22 +487,28 @@ template <class T> int32_t make_chain(rt_ctx* ctx, uint64_t tiles, uint64_t line
     if (tiles >= (1ull << 31) / lines) return rt_fail(RT_E_INVALID, "gated scan: too long for one launch");
     out->tiles = (uint32_t)tiles;
     out->lines = (uint32_t)lines;
-    out->ctl = nullptr;
+    out->tickets = nullptr;
     out->words = nullptr;
+    out->epoch = 0;
     if (tiles == 1) return RT_OK;
-    void* p = nullptr;
-    RT_TRY(rt_chain_room(ctx, sizeof(ChainControl) + tiles * lines * Slot<T>::kWords * sizeof(uint64_t), &p));
-    out->ctl = (ChainControl*)p;
-    out->words = (uint64_t*)(out->ctl + 1);
-    // the 30 bits of the launch's number are cleared, and old tags with them, long before they come round
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    RT_HIP(hipStreamIsCapturing(ctx->stream, &capture));
+    if (capture != hipStreamCaptureStatusNone) return rt_fail(RT_E_INVALID, "gated scan: a launch that hands states from tile to tile cannot be captured");
+    void *tickets = nullptr, *words = nullptr;
+    RT_TRY(rt_chain_room(ctx, 0, lines * kTicketPitch * sizeof(uint32_t), &tickets));
+    RT_TRY(rt_chain_room(ctx, 1, tiles * lines * Slot<T>::kWords * sizeof(uint64_t), &words));
+    // the slots are cleared, and old tags with them, before numbers come round
     if (++ctx->chain_launches == 1u << 29) {
-        RT_TRY(rt_chain_clear(ctx));
-        ctx->chain_launches = 0;
+        RT_TRY(rt_chain_clear(ctx, 1));
+        ctx->chain_launches = 1;
     }
+    out->tickets = (uint32_t*)tickets;
+    out->words = (uint64_t*)words;
+    out->epoch = ctx->chain_launches;
     return RT_OK;
 }
 
-constexpr int kWaves = 8;
+constexpr int kWaves = 8, kBackWaves = 4;         // of a tile
 constexpr uint64_t kWideMost = 1ull << 22;      // inner: a wave's rows are addressed with 32-bit offsets; beyond it columns alone fill the card
 template <class T> int32_t forward_typed(rt_ctx* ctx, int form, const ScanArgs<T>& a) {
     constexpr int L = sizeof(T) == 4 ? 32 : 16;
@@ -514,10 +534,10 @@ template <class T, class S> int32_t backward_typed(rt_ctx* ctx, int form, const 
     if (a.inner >= 32 && a.inner < kWideMost && a.steps > 8) {
         const uint64_t cb = (a.inner + 63) / 64;
         Chain ch;
-        RT_TRY(make_chain<T>(ctx, (a.steps + kWaves * L - 1) / (kWaves * L), a.outer * cb, &ch));
+        RT_TRY(make_chain<T>(ctx, (a.steps + kBackWaves * L - 1) / (kBackWaves * L), a.outer * cb, &ch));
         const dim3 grid(ch.tiles * ch.lines);
-        if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_backward_wide_kernel<T, RT_SCAN_LINEAR, S, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
-        else hipLaunchKernelGGL((scan_backward_wide_kernel<T, RT_SCAN_SIGMOID, S, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
+        if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_backward_wide_kernel<T, RT_SCAN_LINEAR, S, kBackWaves, L>), grid, dim3(kBackWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
+        else hipLaunchKernelGGL((scan_backward_wide_kernel<T, RT_SCAN_SIGMOID, S, kBackWaves, L>), grid, dim3(kBackWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
     } else {
         if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_backward_columns_kernel<T, RT_SCAN_LINEAR, S>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
         else hipLaunchKernelGGL((scan_backward_columns_kernel<T, RT_SCAN_SIGMOID, S>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
