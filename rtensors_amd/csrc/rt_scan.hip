@@ -111,12 +111,11 @@ struct Chain {
     uint32_t tiles;          // along the steps
     uint32_t lines;          // sets of columns that are chained on their own
     uint32_t epoch;          // the launch's number, 30 bits
+    uint32_t rounds;         // blocks a line gets: `tiles`, or the next multiple of 8
 };
 constexpr uint32_t kTicketPitch = 16;
 constexpr uint32_t kAgg = 1, kEnd = 2;                           // what a slot holds: (A, H), or the end state in place of H
-#ifndef RT_WIN
-#define RT_WIN 16
-#endif
+constexpr int kWindowF32 = 16, kWindowF64 = 8;                  // tiles before its own that a tile looks at
 
 __device__ __forceinline__ void put_word(uint64_t* p, uint32_t bits, uint32_t tag) {
     __hip_atomic_store(p, (uint64_t)tag << 32 | bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -159,13 +158,30 @@ template <class T> struct Slot {
     }
 };
 
+// rt_gate_of for f32 in about half the instructions: the hardware's 2^x with the rounding of x log2 e put right (1.5 ulp; results below
+// the normal range are 0), and its reciprocal refined once.
+__device__ __forceinline__ RtGate<double> gate_of(double g) { return rt_gate_of(g); }
+__device__ __forceinline__ RtGate<float> gate_of(float g) {
+    float t = g < 0.0f ? g : -g;
+    t = t < -200.0f ? -200.0f : t;                               // -inf would make the correction below inf - inf; NaN stays
+    const float p = t * 0x1.715476p+0f;                          // log2 e = this + 0x1.4ae0c0p-26
+    const float q = __builtin_fmaf(t, 0x1.4ae0c0p-26f, __builtin_fmaf(t, 0x1.715476p+0f, -p));
+    const float e0 = __builtin_amdgcn_exp2f(p);
+    const float e = __builtin_fmaf(e0, q * 0x1.62e430p-1f, e0);
+    const float d = 1.0f + e;
+    const float i0 = __builtin_amdgcn_rcpf(d);
+    const float inv = __builtin_fmaf(__builtin_fmaf(-d, i0, 1.0f), i0, i0);
+    const float low = e * inv;
+    return g < 0.0f ? RtGate<float>{low, inv} : RtGate<float>{inv, low};
+}
+
 __device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
 __device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
 __device__ __forceinline__ bool finite(double v) { return __builtin_fabs(v) < __builtin_inf(); }
 
 template <class T, int W> struct JoinRoom {
-    static constexpr int kWindow = sizeof(T) == 4 ? RT_WIN : RT_WIN / 2;      // tiles before its own that a tile looks at
+    static constexpr int kWindow = sizeof(T) == 4 ? kWindowF32 : kWindowF64;
     T A[W][64], H[W][64], start[64];
     T winA[kWindow][64], winH[kWindow][64];
     uint64_t ends[kWindow];
@@ -227,13 +243,22 @@ template <class T, int W> __device__ __forceinline__ T chain_start(const Chain& 
     return c;
 }
 
-// The block's tile among those of its line; whoever takes the last one leaves the counter as the next launch needs it.
+// The line a block works on.  Blocks go to the eight XCDs in turn, each with an L2 of its own, and lines that are neighbours in memory
+// share the cache lines at their borders (all of them where rows are no multiple of 128 bytes): every XCD goes through all lines in
+// order, the XCDs an eighth of the lines apart, so that neighbouring lines mostly get the same tile in the same L2.
+__device__ __forceinline__ uint32_t line_of_block(const Chain& ch) {
+    const uint32_t b = blockIdx.x;
+    if (ch.rounds % 8 != 0 || ch.tiles == 1) return b % ch.lines;
+    const uint32_t x = b % 8;
+    return (b / 8 + (uint32_t)((uint64_t)x * ch.lines / 8)) % ch.lines;
+}
+// The block's tile among those of its line (one that is not there for the blocks too many); whoever takes the last one leaves the counter as the next launch needs it.
 template <class T, int W> __device__ __forceinline__ uint32_t take_tile(const Chain& ch, uint32_t line, JoinRoom<T, W>& room) {
     if (ch.tiles == 1) return 0;
     if (threadIdx.x == 0) {
         uint32_t* c = ch.tickets + (uint64_t)line * kTicketPitch;
         const uint32_t t = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (t == ch.tiles - 1) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (t == ch.rounds - 1) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         room.tile = t;
     }
     __syncthreads();
@@ -327,7 +352,8 @@ __device__ __forceinline__ uint64_t reset_bits(const uint8_t* flags, int64_t str
 template <class T, int FORM, int W, int L>
 __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain ch, uint32_t col_blocks) {
     __shared__ JoinRoom<T, W> room;
-    const uint32_t line = blockIdx.x % ch.lines, k = take_tile<T, W>(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
+    const uint32_t line = line_of_block(ch), k = take_tile<T, W>(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
+    if (k >= ch.tiles) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t row = (uint32_t)a.inner, col0 = (line - o * col_blocks) * 64, col = col0 + lane;
     const bool in = col < row;
@@ -350,7 +376,7 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
 #pragma unroll
         for (int j = 0; j < L; ++j) {
             if constexpr (FORM == RT_SCAN_SIGMOID) {
-                const RtGate<T> q = rt_gate_of(f[j]);
+                const RtGate<T> q = gate_of(f[j]);
                 f[j] = q.s;
                 b[j] = q.r * b[j];
             }
@@ -383,7 +409,8 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
 template <class T, int FORM, class S, int W, int L>
 __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, S> a, Chain ch, uint32_t col_blocks) {
     __shared__ JoinRoom<T, W> room;
-    const uint32_t line = blockIdx.x % ch.lines, k = take_tile<T, W>(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
+    const uint32_t line = line_of_block(ch), k = take_tile<T, W>(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
+    if (k >= ch.tiles) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t row = (uint32_t)a.inner, col0 = (line - o * col_blocks) * 64, col = col0 + lane;
     const bool in = col < row;
@@ -416,13 +443,13 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
             cuts &= (2ull << (n - 1)) - 1;
         }
         if constexpr (FORM == RT_SCAN_SIGMOID)
-            if (r0 > 0) f0 = rt_gate_of(f0).s;
+            if (r0 > 0) f0 = gate_of(f0).s;
         T f = f0;
 #pragma unroll
         for (int j = 0; j < L; ++j) {
             s[j] = g[j];
             if constexpr (FORM == RT_SCAN_SIGMOID) {
-                const RtGate<T> q = rt_gate_of(g[j]);
+                const RtGate<T> q = gate_of(g[j]);
                 s[j] = q.s;
                 g[j] = q.r;
             }
@@ -463,7 +490,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
     if (a.dstate && in && n && top) {
         const T g0 = a.gate[(uint64_t)o * a.steps * row + col];
         const bool none = (a.reset && a.reset[(uint64_t)o * a.steps]) || (FORM == RT_SCAN_LINEAR && !a.state);
-        a.dstate[sc] = none ? (T)0 : (FORM == RT_SCAN_SIGMOID ? rt_gate_of(g0).s : g0) * end;
+        a.dstate[sc] = none ? (T)0 : (FORM == RT_SCAN_SIGMOID ? gate_of(g0).s : g0) * end;
     }
 }
 
@@ -484,12 +511,13 @@ template <class T> int32_t no_steps(rt_ctx* ctx, const void* src, void* dst, uin
 
 // The chain of a launch: `tiles` along the steps for each of `lines` sets of columns; a workspace only where there is more than one tile.
 template <class T> int32_t make_chain(rt_ctx* ctx, uint64_t tiles, uint64_t lines, Chain* out) {
-    if (tiles >= (1ull << 31) / lines) return rt_fail(RT_E_INVALID, "gated scan: too long for one launch");
+    if (tiles + 7 >= (1ull << 31) / lines) return rt_fail(RT_E_INVALID, "gated scan: too long for one launch");
     out->tiles = (uint32_t)tiles;
     out->lines = (uint32_t)lines;
     out->tickets = nullptr;
     out->words = nullptr;
     out->epoch = 0;
+    out->rounds = (uint32_t)(tiles >= 16 ? (tiles + 7) / 8 * 8 : tiles);
     if (tiles == 1) return RT_OK;
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
     RT_HIP(hipStreamIsCapturing(ctx->stream, &capture));
@@ -517,7 +545,7 @@ template <class T> int32_t forward_typed(rt_ctx* ctx, int form, const ScanArgs<T
         const uint64_t cb = (a.inner + 63) / 64;
         Chain ch;
         RT_TRY(make_chain<T>(ctx, (a.steps + kWaves * L - 1) / (kWaves * L), a.outer * cb, &ch));
-        const dim3 grid(ch.tiles * ch.lines);
+        const dim3 grid(ch.rounds * ch.lines);
         if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_wide_kernel<T, RT_SCAN_LINEAR, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
         else hipLaunchKernelGGL((scan_wide_kernel<T, RT_SCAN_SIGMOID, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
     } else {
@@ -535,7 +563,7 @@ template <class T, class S> int32_t backward_typed(rt_ctx* ctx, int form, const 
         const uint64_t cb = (a.inner + 63) / 64;
         Chain ch;
         RT_TRY(make_chain<T>(ctx, (a.steps + kBackWaves * L - 1) / (kBackWaves * L), a.outer * cb, &ch));
-        const dim3 grid(ch.tiles * ch.lines);
+        const dim3 grid(ch.rounds * ch.lines);
         if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_backward_wide_kernel<T, RT_SCAN_LINEAR, S, kBackWaves, L>), grid, dim3(kBackWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
         else hipLaunchKernelGGL((scan_backward_wide_kernel<T, RT_SCAN_SIGMOID, S, kBackWaves, L>), grid, dim3(kBackWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
     } else {
