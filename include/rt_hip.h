@@ -374,7 +374,8 @@ int32_t rt_gated_scan_backward_packed8(rt_ctx* ctx, int32_t dtype, int32_t form,
  *                             signs only, which rounding to 8 bits would lose near 0)
  *   rt_pack8_unary_backward   dst = upstream * op'(restored)
  *   rt_pack8_matmul_backward  the weight gradient of y = x w:  dst[b] (k x n) = restored[b]^T (m x k, transposed) * upstream[b] (m x n)
- *                             for every batch; codes and exps are those of the whole (b, m, k) run; dst is zero for m = 0
+ *                             for every batch; codes and exps are those of the whole (b, m, k) run; dst is zero for m = 0;
+ *                             k and n below 2^25
  * Buffers are row-major runs from element 0.  dst of rt_pack8_unary may be src (start = 0), that of rt_pack8_unary_backward may be
  * upstream; any other overlap of an output is RT_E_INVALID.  f32 products are summed in f32, f64 ones in f64, in an order that
  * depends on the sizes alone. */

@@ -1,42 +1,371 @@
 // Weight gradient of a projection whose input is held in 8 bits: dst[b] (k x n) = restored[b]^T * upstream[b] (m x n).
 #include "rt_pack8.h"
 
+#include <atomic>
+
 namespace {
 
-constexpr int kTile = 16;
+// ---- f32 -----------------------------------------------------------------------------------------------------------------------------
+// A restored value has 7 significant bits and is a bf16 number exactly.  An f32 number v is the exact sum of three bf16 numbers: v cut to
+// its upper 16 bits, what is left cut again, and the last 8 bits.  A product of two bf16 numbers is exact in f32, so three bf16 matrix
+// products accumulated in f32 give the f32 product, at a sixteenth of the f32 matrix instructions' time each.  (Of an element below
+// 2^-110 the last parts may fall below the normal range, where the matrix unit may take them as 0: at most 2^-126 of it.)
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16_a1 __attribute__((aligned(1)));
 
-// One element of dst per lane, 16 x 16 a block, 16 rows of both operands staged at a time.
-template <class T>
-__global__ __launch_bounds__(kTile * kTile) void pack8_matmul_plain_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
-                                                                           const T* __restrict__ up, T* __restrict__ dst, uint64_t m, uint64_t k, uint64_t n,
-                                                                           uint64_t tiles_k, uint64_t tiles_n) {
-    __shared__ T xs[kTile][kTile + 1], ys[kTile][kTile + 1];
-    const uint64_t tile = blockIdx.x, batch = tile / (tiles_k * tiles_n), kn = tile - batch * tiles_k * tiles_n;
-    const uint64_t k0 = kn / tiles_n * kTile, n0 = kn % tiles_n * kTile;
-    const int c = threadIdx.x % kTile, r = threadIdx.x / kTile;
-    T acc = (T)0;
-    for (uint64_t m0 = 0; m0 < m; m0 += kTile) {
-        const uint64_t row = batch * m + m0 + r;
-        const bool in = m0 + r < m;
-        const uint64_t at = row * k + k0 + c;
-        xs[r][c] = in && k0 + c < k ? p8_value<T>(codes[at], exps[at / kP8Group]) : (T)0;
-        ys[r][c] = in && n0 + c < n ? up[row * n + n0 + c] : (T)0;
-        __syncthreads();
-        const int rows = m - m0 < (uint64_t)kTile ? (int)(m - m0) : kTile;
-        for (int j = 0; j < rows; ++j) acc += xs[j][r] * ys[j][c];
-        __syncthreads();
+// Upper halves of two words, the first one's in the lower half of the result.
+__device__ __forceinline__ uint32_t uppers(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+__device__ __forceinline__ uint32_t bits(float v) { return __builtin_bit_cast(uint32_t, v); }
+__device__ __forceinline__ float number(uint32_t b) { return __builtin_bit_cast(float, b); }
+
+// The three parts of eight numbers, one below the other in the summed dim, as the matrix instructions take them.
+struct Parts { u32x4 p[3]; };
+__device__ __forceinline__ Parts parts_of(const uint32_t (&v)[8]) {
+    Parts out;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t h[2], m[2], l[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            h[e] = v[2 * j + e];
+            const float x = number(h[e]);
+            // inf - inf: an infinity has no further parts (a NaN is one in all of them)
+            const float r = __builtin_fabsf(x) == __builtin_inff() ? 0.0f : x - number(h[e] & 0xffff0000u);
+            m[e] = bits(r);
+            l[e] = bits(r - number(m[e] & 0xffff0000u));
+        }
+        out.p[0][j] = uppers(h[0], h[1]);
+        out.p[1][j] = uppers(m[0], m[1]);
+        out.p[2][j] = uppers(l[0], l[1]);
     }
-    if (k0 + r < k && n0 + c < n) dst[(batch * k + k0 + r) * n + n0 + c] = acc;
+    return out;
 }
 
-template <class T>
-int32_t matmul_typed(rt_ctx* ctx, const void* codes, const void* exps, const void* up, void* dst, uint64_t b, uint64_t m, uint64_t k, uint64_t n) {
-    const uint64_t tk = (k + kTile - 1) / kTile, tn = (n + kTile - 1) / kTile;
-    if (b * tk * tn >= (1ull << 31)) return rt_fail(RT_E_INVALID, "pack8 matmul backward: the result is too large for one launch");
-    hipLaunchKernelGGL(pack8_matmul_plain_kernel<T>, dim3((uint32_t)(b * tk * tn)), dim3(kTile * kTile), 0, ctx->stream, (const int8_t*)codes,
-                       (const uint8_t*)exps, (const T*)up, (T*)dst, m, k, n, tk, tn);
+// dst tile of BI x BJ by WI x WJ waves, kStep rows of both operands staged in LDS at a time, two buffers.  LDS holds 16-byte pieces of
+// eight rows of one column, [part][row group][column]: what a lane of the 32x32x16 matrix instruction takes is one piece, and neither
+// the writes nor the reads of a wave meet in a bank.
+constexpr int kStep = 32, kGroups = kStep / 8;
+template <int BI, int BJ> struct Stage {
+    u32x4 x[kGroups][BI];
+    u32x4 y[3][kGroups][BJ];
+};
+
+// Which rows a block sums: split `s` of `splits` takes whole steps.
+struct Share { uint64_t from, to; };
+__device__ __forceinline__ Share share_of(uint64_t m, uint32_t splits, uint32_t s) {
+    const uint64_t steps = (m + kStep - 1) / kStep, per = steps / splits, more = steps % splits;
+    const uint64_t a = s * per + (s < more ? s : more), n = per + (s < more ? 1 : 0);
+    const uint64_t to = (a + n) * kStep;
+    return Share{a * kStep, to < m ? to : m};
+}
+
+struct Product {
+    const int8_t* codes;
+    const uint8_t* exps;
+    const void* up;
+    void* out;                        // dst, or the splits' partial results, each as large as dst
+    uint64_t b, m, k, n;
+    uint32_t ti, tj, splits;          // tiles of dst, shares of the rows
+};
+// Tile of a block: batch-major, then the splits; within one (batch, split) the tiles in bands of eight along i, so that blocks that run
+// at the same time on one XCD (every eighth block) share columns of both operands in its L2.
+struct Where { uint64_t batch; uint32_t split, i, j; };
+__device__ __forceinline__ Where where(const Product& p) {
+    const uint32_t tiles = p.ti * p.tj, total = gridDim.x;
+    uint32_t t = blockIdx.x;
+    if (total % 8 == 0) t = t % 8 * (total / 8) + t / 8;
+    Where w;
+    const uint32_t bs = t / tiles;
+    t -= bs * tiles;
+    w.batch = bs / p.splits;
+    w.split = bs % p.splits;
+    const uint32_t band = t / (8 * p.tj), rows = p.ti - band * 8 < 8 ? p.ti - band * 8 : 8;
+    t -= band * 8 * p.tj;
+    w.i = band * 8 + t % rows;
+    w.j = t / rows;
+    return w;
+}
+
+template <int BI, int BJ, int WI, int WJ>
+__global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product p) {
+    constexpr int kThreads = WI * WJ * 64, FI = BI / WI / 32, FJ = BJ / WJ / 32;             // 32 x 32 pieces of a wave
+    constexpr int kYEach = kGroups * BJ / kThreads;                                          // columns x row groups of y a lane stages
+    static_assert(kGroups * BI / 2 == kThreads && kYEach * kThreads == kGroups * BJ, "staging covers the tile once");
+    extern __shared__ __align__(16) char lds[];
+    Stage<BI, BJ>* stage = reinterpret_cast<Stage<BI, BJ>*>(lds);
+    const Where at = where(p);
+    const Share share = share_of(p.m, p.splits, at.split);
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wi = w / WJ, wj = w % WJ;
+    const uint64_t i0 = (uint64_t)at.i * BI, j0 = (uint64_t)at.j * BJ;
+    // staging: the lane's two columns of x and one row group; kYEach row groups of one column of y
+    const int xc = tid % (BI / 2) * 2, xg = tid / (BI / 2);
+    const int yc = tid % BJ, yg = tid / BJ * kYEach;
+    // addresses: a wave-uniform start of the step's rows and 32-bit offsets (k and n are below 2^25)
+    const uint32_t k = (uint32_t)p.k, n = (uint32_t)p.n;
+    const bool even = (k & 1) == 0;                              // the lane's two codes lie in one group, at an even place
+    const uint32_t xcol = i0 + xc < k ? (uint32_t)i0 + xc : (even ? k - 2 : k - 1), xnext = xcol + 1 < k ? 1u : 0u;
+    const uint32_t ycol = j0 + yc < n ? (uint32_t)j0 + yc : n - 1;
+    const uint64_t xrow = at.batch * p.m;
+    const float* up = static_cast<const float*>(p.up) + at.batch * p.m * p.n;
+
+    uint32_t cx[8], ex[8], yv[kYEach][8];                        // two codes, two exponent bytes, bits of y
+    auto load = [&](uint64_t m0) {
+        const int rows = share.to - m0 < (uint64_t)kStep ? (int)(share.to - m0) : kStep;
+        const uint64_t xe = (xrow + m0) * k;
+        const int8_t* codes = p.codes + xe;
+        const uint8_t* exps = p.exps + xe / kP8Group;
+        const float* y = up + m0 * n;
+        const uint32_t rem = (uint32_t)xe % kP8Group;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int row = xg * 8 + r < rows ? xg * 8 + r : rows - 1;
+            const uint32_t e = (uint32_t)row * k + xcol;
+            if (even) {
+                cx[r] = *reinterpret_cast<const u16_a1*>(codes + e);
+                ex[r] = exps[(rem + e) / kP8Group] * 0x101u;
+            } else {
+                cx[r] = (uint32_t)(uint8_t)codes[e] | (uint32_t)(uint8_t)codes[e + xnext] << 8;
+                ex[r] = (uint32_t)exps[(rem + e) / kP8Group] | (uint32_t)exps[(rem + e + xnext) / kP8Group] << 8;
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < kYEach; ++g)
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const int row = (yg + g) * 8 + r < rows ? (yg + g) * 8 + r : rows - 1;
+                yv[g][r] = bits(y[(uint32_t)row * n + ycol]);
+            }
+    };
+    auto store = [&](Stage<BI, BJ>& st, uint64_t m0) {
+        const bool whole = m0 + kStep <= share.to;
+        u32x4 a, b;
+#pragma unroll
+        for (int r = 0; r < 8; r += 2) {
+            uint32_t v[2][2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const bool in = whole || m0 + xg * 8 + r + q < share.to;
+                const uint32_t c = in ? cx[r + q] : 0u, e = in ? ex[r + q] : 0u;
+                v[q][0] = bits(p8_value<float>((int8_t)c, e & 255u));
+                v[q][1] = bits(p8_value<float>((int8_t)(c >> 8), e >> 8));
+            }
+            a[r / 2] = uppers(v[0][0], v[1][0]);
+            b[r / 2] = uppers(v[0][1], v[1][1]);
+        }
+        st.x[xg][xc] = a;
+        st.x[xg][xc + 1] = b;
+#pragma unroll
+        for (int g = 0; g < kYEach; ++g) {
+            if (!whole) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (m0 + (yg + g) * 8 + r >= share.to) yv[g][r] = 0u;
+            }
+            const Parts q = parts_of(yv[g]);
+#pragma unroll
+            for (int s = 0; s < 3; ++s) st.y[s][yg + g][yc] = q.p[s];
+        }
+    };
+
+    f32x16 acc[FI][FJ];
+#pragma unroll
+    for (int a = 0; a < FI; ++a)
+#pragma unroll
+        for (int b = 0; b < FJ; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.0f;
+
+    if (share.from < share.to) {
+        load(share.from);
+        store(stage[0], share.from);
+        __syncthreads();
+        int cur = 0;
+        for (uint64_t m0 = share.from; m0 < share.to; m0 += kStep) {
+            const bool more = m0 + kStep < share.to;
+            if (more) load(m0 + kStep);
+            const Stage<BI, BJ>& st = stage[cur];
+#pragma unroll
+            for (int half = 0; half < kStep / 16; ++half) {
+                const int g = half * 2 + (lane >> 5), c = lane & 31;
+                bf16x8 xa[FI];
+#pragma unroll
+                for (int a = 0; a < FI; ++a) xa[a] = __builtin_bit_cast(bf16x8, st.x[g][(wi * FI + a) * 32 + c]);
+#pragma unroll
+                for (int s = 2; s >= 0; --s) {                   // the smallest parts first
+                    bf16x8 yb[FJ];
+#pragma unroll
+                    for (int b = 0; b < FJ; ++b) yb[b] = __builtin_bit_cast(bf16x8, st.y[s][g][(wj * FJ + b) * 32 + c]);
+#pragma unroll
+                    for (int a = 0; a < FI; ++a)
+#pragma unroll
+                        for (int b = 0; b < FJ; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa[a], yb[b], acc[a][b], 0, 0, 0);
+                }
+            }
+            if (more) store(stage[cur ^ 1], m0 + kStep);
+            __syncthreads();
+            cur ^= 1;
+        }
+    }
+    float* out = static_cast<float*>(p.out) + ((uint64_t)at.split * p.b + at.batch) * p.k * p.n;
+#pragma unroll
+    for (int a = 0; a < FI; ++a)
+#pragma unroll
+        for (int b = 0; b < FJ; ++b) {
+            const uint64_t j = j0 + (wj * FJ + b) * 32 + (lane & 31);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const uint64_t i = i0 + (wi * FI + a) * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
+                if (i < p.k && j < p.n) out[i * p.n + j] = acc[a][b][r];
+            }
+        }
+}
+
+// ---- f64 -----------------------------------------------------------------------------------------------------------------------------
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+constexpr int kStep64 = 16, kSide64 = 64;
+constexpr int kPitch64 = kSide64 + 2;                            // in doubles: rows 4 apart, which one instruction reads, start 8 banks apart
+
+// 64 x 64 of dst by 2 x 2 waves, the 16x16x4 matrix instruction, kStep64 rows staged at a time.
+__global__ __launch_bounds__(256) void pack8_matmul_f64_kernel(Product p) {
+    __shared__ double xs[2][kStep64][kPitch64], ys[2][kStep64][kPitch64];
+    const Where at = where(p);
+    const Share share = share_of(p.m, p.splits, at.split);
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wi = w >> 1, wj = w & 1;
+    const uint64_t i0 = (uint64_t)at.i * kSide64, j0 = (uint64_t)at.j * kSide64;
+    const int c = tid % kSide64, r0 = tid / kSide64 * 4;         // the lane's column and four rows of both operands
+    const uint32_t k = (uint32_t)p.k, n = (uint32_t)p.n;
+    const uint32_t xcol = i0 + c < k ? (uint32_t)i0 + c : k - 1, ycol = j0 + c < n ? (uint32_t)j0 + c : n - 1;
+    const double* up = static_cast<const double*>(p.up) + at.batch * p.m * p.n;
+    int32_t cx[4];
+    uint32_t ex[4];
+    double yv[4];
+    auto load = [&](uint64_t m0) {
+        const int rows = share.to - m0 < (uint64_t)kStep64 ? (int)(share.to - m0) : kStep64;
+        const uint64_t xe = (at.batch * p.m + m0) * k;
+        const int8_t* codes = p.codes + xe;
+        const uint8_t* exps = p.exps + xe / kP8Group;
+        const double* y = up + m0 * n;
+        const uint32_t rem = (uint32_t)xe % kP8Group;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = r0 + r < rows ? r0 + r : rows - 1;
+            const uint32_t e = (uint32_t)row * k + xcol;
+            cx[r] = codes[e];
+            ex[r] = exps[(rem + e) / kP8Group];
+            yv[r] = y[(uint32_t)row * n + ycol];
+        }
+    };
+    auto store = [&](int b, uint64_t m0) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool in = m0 + r0 + r < share.to;
+            xs[b][r0 + r][c] = in ? p8_value<double>(cx[r], ex[r]) : 0.0;
+            ys[b][r0 + r][c] = in ? yv[r] : 0.0;
+        }
+    };
+    f64x4 acc[2][2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) acc[a][b] = f64x4{0.0, 0.0, 0.0, 0.0};
+    if (share.from < share.to) {
+        load(share.from);
+        store(0, share.from);
+        __syncthreads();
+        int cur = 0;
+        for (uint64_t m0 = share.from; m0 < share.to; m0 += kStep64) {
+            const bool more = m0 + kStep64 < share.to;
+            if (more) load(m0 + kStep64);
+#pragma unroll
+            for (int q = 0; q < kStep64 / 4; ++q) {
+                const int row = q * 4 + (lane >> 4), cc = lane & 15;
+                double xa[2], yb[2];
+#pragma unroll
+                for (int a = 0; a < 2; ++a) xa[a] = xs[cur][row][wi * 32 + a * 16 + cc];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) yb[b] = ys[cur][row][wj * 32 + b * 16 + cc];
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) acc[a][b] = __builtin_amdgcn_mfma_f64_16x16x4f64(xa[a], yb[b], acc[a][b], 0, 0, 0);
+            }
+            if (more) store(cur ^ 1, m0 + kStep64);
+            __syncthreads();
+            cur ^= 1;
+        }
+    }
+    double* out = static_cast<double*>(p.out) + ((uint64_t)at.split * p.b + at.batch) * p.k * p.n;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint64_t i = i0 + wi * 32 + a * 16 + r * 4 + (lane >> 4), j = j0 + wj * 32 + b * 16 + (lane & 15);
+                if (i < p.k && j < p.n) out[i * p.n + j] = acc[a][b][r];
+            }
+}
+
+// ---- the splits' partial results, added in order -----------------------------------------------------------------------------------------
+template <class T> __global__ __launch_bounds__(256) void pack8_matmul_join_kernel(const T* __restrict__ part, T* __restrict__ dst, uint64_t n, uint32_t splits) {
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    T s = part[i];
+    for (uint32_t k = 1; k < splits; ++k) s += part[k * n + i];
+    dst[i] = s;
+}
+
+// Shares of the rows: enough blocks to fill the card, each share long enough to pay for its partial result.
+uint32_t splits_for(rt_ctx* ctx, uint64_t tiles, uint64_t m, uint64_t least_rows, uint64_t blocks_per_cu) {
+    const uint64_t want = (uint64_t)ctx->num_cus * blocks_per_cu, most = m / least_rows;
+    uint64_t s = tiles >= want ? 1 : want / tiles;
+    s = s < most ? s : most;
+    return (uint32_t)(s < 1 ? 1 : s);
+}
+
+template <class T> int32_t join(rt_ctx* ctx, const void* part, void* dst, uint64_t n, uint32_t splits) {
+    hipLaunchKernelGGL(pack8_matmul_join_kernel<T>, dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, ctx->stream, (const T*)part, (T*)dst, n, splits);
     RT_HIP(hipGetLastError());
     return RT_OK;
+}
+
+template <int BI, int BJ, int WI, int WJ> int32_t f32_launch(rt_ctx* ctx, const Product& p) {
+    constexpr size_t bytes = 2 * sizeof(Stage<BI, BJ>);
+    auto kernel = pack8_matmul_f32_kernel<BI, BJ, WI, WJ>;
+    static std::atomic<uint64_t> allowed{0};                     // more than 64 KiB of LDS has to be asked for, once a device
+    const uint64_t bit = 1ull << (ctx->device & 63);
+    if (!(allowed.load() & bit) || ctx->device > 63) {
+        RT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        allowed.fetch_or(bit);
+    }
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(p.b * p.splits * p.ti * p.tj)), dim3(WI * WJ * 64), bytes, ctx->stream, p);
+    RT_HIP(hipGetLastError());
+    return RT_OK;
+}
+
+int32_t run_product(rt_ctx* ctx, int dtype, Product p, void* dst) {
+    auto tiles_of = [&](uint64_t bi, uint64_t bj) { return p.b * ((p.k + bi - 1) / bi) * ((p.n + bj - 1) / bj); };
+    const bool big = dtype == RT_F32 && tiles_of(256, 256) * (p.m / 1024 ? p.m / 1024 : 1) >= (uint64_t)ctx->num_cus && p.k > 128 && p.n > 128;
+    const uint64_t bi = dtype == RT_F64 ? kSide64 : big ? 256 : 128, bj = bi, tiles = tiles_of(bi, bj);
+    if (tiles >= (1ull << 24)) return rt_fail(RT_E_INVALID, "pack8 matmul backward: the result is too large for one launch");
+    p.ti = (uint32_t)((p.k + bi - 1) / bi);
+    p.tj = (uint32_t)((p.n + bj - 1) / bj);
+    p.splits = splits_for(ctx, tiles, p.m, big ? 1024 : 256, dtype == RT_F64 ? 4 : big ? 1 : 2);
+    const uint64_t n = p.b * p.k * p.n;
+    p.out = dst;
+    if (p.splits > 1) RT_TRY(rt_scratch(ctx, n * p.splits * rt_elem_size(dtype), &p.out));
+    if (dtype == RT_F64) {
+        hipLaunchKernelGGL(pack8_matmul_f64_kernel, dim3((uint32_t)(tiles * p.splits)), dim3(256), 0, ctx->stream, p);
+        RT_HIP(hipGetLastError());
+    } else if (big) {
+        RT_TRY((f32_launch<256, 256, 2, 4>(ctx, p)));
+    } else {
+        RT_TRY((f32_launch<128, 128, 2, 2>(ctx, p)));
+    }
+    if (p.splits == 1) return RT_OK;
+    return dtype == RT_F32 ? join<float>(ctx, p.out, dst, n, p.splits) : join<double>(ctx, p.out, dst, n, p.splits);
 }
 
 bool product(uint64_t a, uint64_t b, uint64_t c, uint64_t* out) {
@@ -57,6 +386,7 @@ extern "C" int32_t rt_pack8_matmul_backward(rt_ctx* ctx, int32_t dtype, const vo
     if (dtype != RT_F32 && dtype != RT_F64) return rt_fail(RT_E_DTYPE, "%s: f32 / f64 only", what);
     uint64_t nx, ny, nd;
     if (!product(b, m, k, &nx) || !product(b, m, n, &ny) || !product(b, k, n, &nd)) return rt_fail(RT_E_INVALID, "%s: sizes are too large", what);
+    if (k >= (1ull << 25) || n >= (1ull << 25)) return rt_fail(RT_E_INVALID, "%s: k and n have to be below 2^25", what);
     const uint64_t groups = (nx + kP8Group - 1) / kP8Group;
     const int es = rt_elem_size(dtype);
     if (codes_len < nx || exps_len < groups) return rt_fail(RT_E_OUT_OF_BOUNDS, "%s: codes or exps are shorter than b * m * k elements need", what);
@@ -72,5 +402,5 @@ extern "C" int32_t rt_pack8_matmul_backward(rt_ctx* ctx, int32_t dtype, const vo
         return rt_fail(RT_E_INVALID, "%s: dst overlaps an input", what);
     RT_TRY(rt_ctx_enter(ctx));
     CtxGuard g(ctx);
-    return dtype == RT_F32 ? matmul_typed<float>(ctx, codes, exps, upstream, dst, b, m, k, n) : matmul_typed<double>(ctx, codes, exps, upstream, dst, b, m, k, n);
+    return run_product(ctx, dtype, Product{(const int8_t*)codes, (const uint8_t*)exps, upstream, nullptr, b, m, k, n, 0, 0, 1}, dst);
 }
