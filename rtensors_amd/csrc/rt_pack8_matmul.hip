@@ -88,10 +88,13 @@ __device__ __forceinline__ Where where(const Product& p) {
     return w;
 }
 
-template <int BI, int BJ, int WI, int WJ>
+// One step of the loop works on three steps of the rows at once: the matrix instructions take the one in the current buffer, the next one
+// is turned into parts and written to the other buffer, and the one after that is on its way from memory into registers.  EVEN: k is
+// even, so a lane's two codes lie in one group.
+template <int BI, int BJ, int WI, int WJ, bool EVEN>
 __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product p) {
     constexpr int kThreads = WI * WJ * 64, FI = BI / WI / 32, FJ = BJ / WJ / 32;             // 32 x 32 pieces of a wave
-    constexpr int kYEach = kGroups * BJ / kThreads;                                          // columns x row groups of y a lane stages
+    constexpr int kYEach = kGroups * BJ / kThreads;                                          // row groups of y a lane stages
     static_assert(kGroups * BI / 2 == kThreads && kYEach * kThreads == kGroups * BJ, "staging covers the tile once");
     extern __shared__ __align__(16) char lds[];
     Stage<BI, BJ>* stage = reinterpret_cast<Stage<BI, BJ>*>(lds);
@@ -102,54 +105,63 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product 
     // staging: the lane's two columns of x and one row group; kYEach row groups of one column of y
     const int xc = tid % (BI / 2) * 2, xg = tid / (BI / 2);
     const int yc = tid % BJ, yg = tid / BJ * kYEach;
-    // addresses: a wave-uniform start of the step's rows and 32-bit offsets (k and n are below 2^25)
+    // addresses: a wave-uniform start of each row and one 32-bit offset (k and n are below 2^25); columns behind the last one load it
     const uint32_t k = (uint32_t)p.k, n = (uint32_t)p.n;
-    const bool even = (k & 1) == 0;                              // the lane's two codes lie in one group, at an even place
-    const uint32_t xcol = i0 + xc < k ? (uint32_t)i0 + xc : (even ? k - 2 : k - 1), xnext = xcol + 1 < k ? 1u : 0u;
+    const uint32_t xcol = i0 + xc < k ? (uint32_t)i0 + xc : (EVEN ? k - 2 : k - 1), xnext = xcol + 1 < k ? 1u : 0u;
     const uint32_t ycol = j0 + yc < n ? (uint32_t)j0 + yc : n - 1;
     const uint64_t xrow = at.batch * p.m;
     const float* up = static_cast<const float*>(p.up) + at.batch * p.m * p.n;
 
-    uint32_t cx[8], ex[8], yv[kYEach][8];                        // two codes, two exponent bytes, bits of y
-    auto load = [&](uint64_t m0) {
-        const int rows = share.to - m0 < (uint64_t)kStep ? (int)(share.to - m0) : kStep;
-        const uint64_t xe = (xrow + m0) * k;
-        const int8_t* codes = p.codes + xe;
-        const uint8_t* exps = p.exps + xe / kP8Group;
-        const float* y = up + m0 * n;
-        const uint32_t rem = (uint32_t)xe % kP8Group;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const int row = xg * 8 + r < rows ? xg * 8 + r : rows - 1;
-            const uint32_t e = (uint32_t)row * k + xcol;
-            if (even) {
-                cx[r] = *reinterpret_cast<const u16_a1*>(codes + e);
-                ex[r] = exps[(rem + e) / kP8Group] * 0x101u;
-            } else {
-                cx[r] = (uint32_t)(uint8_t)codes[e] | (uint32_t)(uint8_t)codes[e + xnext] << 8;
-                ex[r] = (uint32_t)exps[(rem + e) / kP8Group] | (uint32_t)exps[(rem + e + xnext) / kP8Group] << 8;
-            }
+    uint32_t cx[8], ex[8], yv[kYEach][8];                        // two codes, one or two exponent bytes, bits of y
+    auto load_row_of_x = [&](int r, uint64_t from, uint32_t off) {       // from: a wave-uniform row; off: the lane's place from its start
+        const uint64_t e = (xrow + from) * k;
+        const int8_t* codes = p.codes + e;
+        const uint8_t* exps = p.exps + e / kP8Group;
+        const uint32_t rem = (uint32_t)e % kP8Group;
+        if constexpr (EVEN) {
+            cx[r] = *reinterpret_cast<const u16_a1*>(codes + off);
+            ex[r] = exps[(rem + off) / kP8Group];
+        } else {
+            cx[r] = (uint32_t)(uint8_t)codes[off] | (uint32_t)(uint8_t)codes[off + xnext] << 8;
+            ex[r] = (uint32_t)exps[(rem + off) / kP8Group] | (uint32_t)exps[(rem + off + xnext) / kP8Group] << 8;
         }
+    };
+    const uint32_t xoff = (uint32_t)(xg * 8) * k + xcol, yoff = (uint32_t)(yg * 8) * n + ycol;
+    auto load = [&](uint64_t m0) {
+        if (m0 + kStep <= share.to) {
 #pragma unroll
-        for (int g = 0; g < kYEach; ++g)
+            for (int r = 0; r < 8; ++r) load_row_of_x(r, m0 + r, xoff);
+#pragma unroll
+            for (int g = 0; g < kYEach; ++g)
+#pragma unroll
+                for (int r = 0; r < 8; ++r) yv[g][r] = bits((up + (m0 + g * 8 + r) * n)[yoff]);
+        } else {                                                 // rows behind the last one load it
+            const int rows = (int)(share.to - m0);
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                const int row = (yg + g) * 8 + r < rows ? (yg + g) * 8 + r : rows - 1;
-                yv[g][r] = bits(y[(uint32_t)row * n + ycol]);
+                const int row = xg * 8 + r < rows ? xg * 8 + r : rows - 1;
+                load_row_of_x(r, m0, (uint32_t)row * k + xcol);
             }
+#pragma unroll
+            for (int g = 0; g < kYEach; ++g)
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const int row = (yg + g) * 8 + r < rows ? (yg + g) * 8 + r : rows - 1;
+                    yv[g][r] = bits((up + m0 * n)[(uint32_t)row * n + ycol]);
+                }
+        }
     };
-    auto store = [&](Stage<BI, BJ>& st, uint64_t m0) {
-        const bool whole = m0 + kStep <= share.to;
+    auto store = [&](Stage<BI, BJ>& st) {
         u32x4 a, b;
 #pragma unroll
         for (int r = 0; r < 8; r += 2) {
             uint32_t v[2][2];
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const bool in = whole || m0 + xg * 8 + r + q < share.to;
-                const uint32_t c = in ? cx[r + q] : 0u, e = in ? ex[r + q] : 0u;
-                v[q][0] = bits(p8_value<float>((int8_t)c, e & 255u));
-                v[q][1] = bits(p8_value<float>((int8_t)(c >> 8), e >> 8));
+                const uint32_t c = cx[r + q], e = ex[r + q];
+                const float s0 = p8_step<float>(EVEN ? e : e & 255u), s1 = EVEN ? s0 : p8_step<float>(e >> 8);
+                v[q][0] = bits((float)(int8_t)c * s0);
+                v[q][1] = bits((float)(int8_t)(c >> 8) * s1);
             }
             a[r / 2] = uppers(v[0][0], v[1][0]);
             b[r / 2] = uppers(v[0][1], v[1][1]);
@@ -158,14 +170,19 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product 
         st.x[xg][xc + 1] = b;
 #pragma unroll
         for (int g = 0; g < kYEach; ++g) {
-            if (!whole) {
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    if (m0 + (yg + g) * 8 + r >= share.to) yv[g][r] = 0u;
-            }
             const Parts q = parts_of(yv[g]);
 #pragma unroll
             for (int s = 0; s < 3; ++s) st.y[s][yg + g][yc] = q.p[s];
+        }
+    };
+    auto mask = [&](uint64_t m0) {                               // rows behind the last one are zeros
+        const int rows = share.to - m0 < (uint64_t)kStep ? (int)(share.to - m0) : kStep;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            if (xg * 8 + r >= rows) cx[r] = ex[r] = 0u;
+#pragma unroll
+            for (int g = 0; g < kYEach; ++g)
+                if ((yg + g) * 8 + r >= rows) yv[g][r] = 0u;
         }
     };
 
@@ -176,37 +193,49 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product 
         for (int b = 0; b < FJ; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.0f;
+    auto multiply = [&](const Stage<BI, BJ>& st) {
+#pragma unroll
+        for (int half = 0; half < kStep / 16; ++half) {
+            const int g = half * 2 + (lane >> 5), c = lane & 31;
+            bf16x8 xa[FI];
+#pragma unroll
+            for (int a = 0; a < FI; ++a) xa[a] = __builtin_bit_cast(bf16x8, st.x[g][(wi * FI + a) * 32 + c]);
+#pragma unroll
+            for (int s = 2; s >= 0; --s) {                       // the smallest parts first
+                bf16x8 yb[FJ];
+#pragma unroll
+                for (int b = 0; b < FJ; ++b) yb[b] = __builtin_bit_cast(bf16x8, st.y[s][g][(wj * FJ + b) * 32 + c]);
+#pragma unroll
+                for (int a = 0; a < FI; ++a)
+#pragma unroll
+                    for (int b = 0; b < FJ; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa[a], yb[b], acc[a][b], 0, 0, 0);
+            }
+        }
+    };
 
     if (share.from < share.to) {
+        const uint32_t steps = (uint32_t)((share.to - share.from + kStep - 1) / kStep);
         load(share.from);
-        store(stage[0], share.from);
+        if (steps == 1) mask(share.from);
+        store(stage[0]);
+        if (steps > 1) load(share.from + kStep);
         __syncthreads();
         int cur = 0;
-        for (uint64_t m0 = share.from; m0 < share.to; m0 += kStep) {
-            const bool more = m0 + kStep < share.to;
-            if (more) load(m0 + kStep);
-            const Stage<BI, BJ>& st = stage[cur];
-#pragma unroll
-            for (int half = 0; half < kStep / 16; ++half) {
-                const int g = half * 2 + (lane >> 5), c = lane & 31;
-                bf16x8 xa[FI];
-#pragma unroll
-                for (int a = 0; a < FI; ++a) xa[a] = __builtin_bit_cast(bf16x8, st.x[g][(wi * FI + a) * 32 + c]);
-#pragma unroll
-                for (int s = 2; s >= 0; --s) {                   // the smallest parts first
-                    bf16x8 yb[FJ];
-#pragma unroll
-                    for (int b = 0; b < FJ; ++b) yb[b] = __builtin_bit_cast(bf16x8, st.y[s][g][(wj * FJ + b) * 32 + c]);
-#pragma unroll
-                    for (int a = 0; a < FI; ++a)
-#pragma unroll
-                        for (int b = 0; b < FJ; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa[a], yb[b], acc[a][b], 0, 0, 0);
-                }
-            }
-            if (more) store(stage[cur ^ 1], m0 + kStep);
+        for (uint32_t t = 0; t + 2 < steps; ++t) {
+            store(stage[cur ^ 1]);
+            load(share.from + (uint64_t)(t + 2) * kStep);
+            multiply(stage[cur]);
             __syncthreads();
             cur ^= 1;
         }
+        if (steps > 1) {
+            mask(share.from + (uint64_t)(steps - 1) * kStep);
+            store(stage[cur ^ 1]);
+            multiply(stage[cur]);
+            __syncthreads();
+            cur ^= 1;
+        }
+        multiply(stage[cur]);
     }
     float* out = static_cast<float*>(p.out) + ((uint64_t)at.split * p.b + at.batch) * p.k * p.n;
 #pragma unroll
@@ -331,9 +360,9 @@ template <class T> int32_t join(rt_ctx* ctx, const void* part, void* dst, uint64
     return RT_OK;
 }
 
-template <int BI, int BJ, int WI, int WJ> int32_t f32_launch(rt_ctx* ctx, const Product& p) {
+template <int BI, int BJ, int WI, int WJ, bool EVEN> int32_t f32_launch(rt_ctx* ctx, const Product& p) {
     constexpr size_t bytes = 2 * sizeof(Stage<BI, BJ>);
-    auto kernel = pack8_matmul_f32_kernel<BI, BJ, WI, WJ>;
+    auto kernel = pack8_matmul_f32_kernel<BI, BJ, WI, WJ, EVEN>;
     static std::atomic<uint64_t> allowed{0};                     // more than 64 KiB of LDS has to be asked for, once a device
     const uint64_t bit = 1ull << (ctx->device & 63);
     if (!(allowed.load() & bit) || ctx->device > 63) {
@@ -360,9 +389,9 @@ int32_t run_product(rt_ctx* ctx, int dtype, Product p, void* dst) {
         hipLaunchKernelGGL(pack8_matmul_f64_kernel, dim3((uint32_t)(tiles * p.splits)), dim3(256), 0, ctx->stream, p);
         RT_HIP(hipGetLastError());
     } else if (big) {
-        RT_TRY((f32_launch<256, 256, 2, 4>(ctx, p)));
+        RT_TRY((p.k % 2 == 0 ? f32_launch<256, 256, 2, 4, true>(ctx, p) : f32_launch<256, 256, 2, 4, false>(ctx, p)));
     } else {
-        RT_TRY((f32_launch<128, 128, 2, 2>(ctx, p)));
+        RT_TRY((p.k % 2 == 0 ? f32_launch<128, 128, 2, 2, true>(ctx, p) : f32_launch<128, 128, 2, 2, false>(ctx, p)));
     }
     if (p.splits == 1) return RT_OK;
     return dtype == RT_F32 ? join<float>(ctx, p.out, dst, n, p.splits) : join<double>(ctx, p.out, dst, n, p.splits);
