@@ -91,7 +91,7 @@ __device__ __forceinline__ Where where(const Product& p) {
 // One step of the loop works on three steps of the rows at once: the matrix instructions take the one in the current buffer, the next one
 // is turned into parts and written to the other buffer, and the one after that is on its way from memory into registers.  EVEN: k is
 // even, so a lane's two codes lie in one group.
-template <int BI, int BJ, int WI, int WJ, bool EVEN>
+template <int BI, int BJ, int WI, int WJ, int DEPTH, bool EVEN>
 __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product p) {
     constexpr int kThreads = WI * WJ * 64, FI = BI / WI / 32, FJ = BJ / WJ / 32;             // 32 x 32 pieces of a wave
     constexpr int kYEach = kGroups * BJ / kThreads;                                          // row groups of y a lane stages
@@ -112,56 +112,64 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product 
     const uint64_t xrow = at.batch * p.m;
     const float* up = static_cast<const float*>(p.up) + at.batch * p.m * p.n;
 
-    uint32_t cx[8], ex[8], yv[kYEach][8];                        // two codes, one or two exponent bytes, bits of y
-    auto load_row_of_x = [&](int r, uint64_t from, uint32_t off) {       // from: a wave-uniform row; off: the lane's place from its start
+    // EVEN: two codes in cx, their exponent byte in ex; else one each in [0] and [1].  Bits of y.
+    struct Held { uint32_t cx[EVEN ? 1 : 2][8], ex[EVEN ? 1 : 2][8], yv[kYEach][8]; };
+    Held held[DEPTH];
+    auto load_row_of_x = [&](Held& d, int r, uint64_t from, uint32_t off) {       // from: a wave-uniform row; off: the lane's place from its start
         const uint64_t e = (xrow + from) * k;
         const int8_t* codes = p.codes + e;
         const uint8_t* exps = p.exps + e / kP8Group;
         const uint32_t rem = (uint32_t)e % kP8Group;
         if constexpr (EVEN) {
-            cx[r] = *reinterpret_cast<const u16_a1*>(codes + off);
-            ex[r] = exps[(rem + off) / kP8Group];
+            d.cx[0][r] = *reinterpret_cast<const u16_a1*>(codes + off);
+            d.ex[0][r] = exps[(rem + off) / kP8Group];
         } else {
-            cx[r] = (uint32_t)(uint8_t)codes[off] | (uint32_t)(uint8_t)codes[off + xnext] << 8;
-            ex[r] = (uint32_t)exps[(rem + off) / kP8Group] | (uint32_t)exps[(rem + off + xnext) / kP8Group] << 8;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                d.cx[q][r] = (uint8_t)codes[off + q * xnext];
+                d.ex[q][r] = exps[(rem + off + q * xnext) / kP8Group];
+            }
         }
     };
     const uint32_t xoff = (uint32_t)(xg * 8) * k + xcol, yoff = (uint32_t)(yg * 8) * n + ycol;
-    auto load = [&](uint64_t m0) {
+    auto load_whole = [&](Held& d, uint64_t m0) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) load_row_of_x(d, r, m0 + r, xoff);
+#pragma unroll
+        for (int g = 0; g < kYEach; ++g)
+#pragma unroll
+            for (int r = 0; r < 8; ++r) d.yv[g][r] = bits((up + (m0 + g * 8 + r) * n)[yoff]);
+    };
+    auto load = [&](Held& d, uint64_t m0) {
+        if (m0 >= share.to) return;
         if (m0 + kStep <= share.to) {
-#pragma unroll
-            for (int r = 0; r < 8; ++r) load_row_of_x(r, m0 + r, xoff);
-#pragma unroll
-            for (int g = 0; g < kYEach; ++g)
-#pragma unroll
-                for (int r = 0; r < 8; ++r) yv[g][r] = bits((up + (m0 + g * 8 + r) * n)[yoff]);
+            load_whole(d, m0);
         } else {                                                 // rows behind the last one load it
             const int rows = (int)(share.to - m0);
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
                 const int row = xg * 8 + r < rows ? xg * 8 + r : rows - 1;
-                load_row_of_x(r, m0, (uint32_t)row * k + xcol);
+                load_row_of_x(d, r, m0, (uint32_t)row * k + xcol);
             }
 #pragma unroll
             for (int g = 0; g < kYEach; ++g)
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
                     const int row = (yg + g) * 8 + r < rows ? (yg + g) * 8 + r : rows - 1;
-                    yv[g][r] = bits((up + m0 * n)[(uint32_t)row * n + ycol]);
+                    d.yv[g][r] = bits((up + m0 * n)[(uint32_t)row * n + ycol]);
                 }
         }
     };
-    auto store = [&](Stage<BI, BJ>& st) {
+    auto store = [&](Held& d, Stage<BI, BJ>& st) {
         u32x4 a, b;
 #pragma unroll
         for (int r = 0; r < 8; r += 2) {
             uint32_t v[2][2];
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const uint32_t c = cx[r + q], e = ex[r + q];
-                const float s0 = p8_step<float>(EVEN ? e : e & 255u), s1 = EVEN ? s0 : p8_step<float>(e >> 8);
-                v[q][0] = bits((float)(int8_t)c * s0);
-                v[q][1] = bits((float)(int8_t)(c >> 8) * s1);
+                constexpr int kSecond = EVEN ? 0 : 1, kShift = EVEN ? 8 : 0;
+                v[q][0] = bits(p8_value<float>((int8_t)d.cx[0][r + q], d.ex[0][r + q]));
+                v[q][1] = bits(p8_value<float>((int8_t)(d.cx[kSecond][r + q] >> kShift), d.ex[kSecond][r + q]));
             }
             a[r / 2] = uppers(v[0][0], v[1][0]);
             b[r / 2] = uppers(v[0][1], v[1][1]);
@@ -170,19 +178,21 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product 
         st.x[xg][xc + 1] = b;
 #pragma unroll
         for (int g = 0; g < kYEach; ++g) {
-            const Parts q = parts_of(yv[g]);
+            const Parts q = parts_of(d.yv[g]);
 #pragma unroll
             for (int s = 0; s < 3; ++s) st.y[s][yg + g][yc] = q.p[s];
         }
     };
-    auto mask = [&](uint64_t m0) {                               // rows behind the last one are zeros
+    auto mask = [&](Held& d, uint64_t m0) {                               // rows behind the last one are zeros
         const int rows = share.to - m0 < (uint64_t)kStep ? (int)(share.to - m0) : kStep;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-            if (xg * 8 + r >= rows) cx[r] = ex[r] = 0u;
+#pragma unroll
+            for (int q = 0; q < (EVEN ? 1 : 2); ++q)
+                if (xg * 8 + r >= rows) d.cx[q][r] = d.ex[q][r] = 0u;
 #pragma unroll
             for (int g = 0; g < kYEach; ++g)
-                if ((yg + g) * 8 + r >= rows) yv[g][r] = 0u;
+                if ((yg + g) * 8 + r >= rows) d.yv[g][r] = 0u;
         }
     };
 
@@ -215,27 +225,35 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product 
 
     if (share.from < share.to) {
         const uint32_t steps = (uint32_t)((share.to - share.from + kStep - 1) / kStep);
-        load(share.from);
-        if (steps == 1) mask(share.from);
-        store(stage[0]);
-        if (steps > 1) load(share.from + kStep);
+        auto row_of = [&](uint32_t t) { return share.from + (uint64_t)t * kStep; };
+        load(held[0], row_of(0));
+        if (steps == 1) mask(held[0], row_of(0));
+        store(held[0], stage[0]);
+        // step t is held in set (t - 1) % DEPTH
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) load(held[d], row_of(1 + d));
         __syncthreads();
-        int cur = 0;
-        for (uint32_t t = 0; t + 2 < steps; ++t) {
-            store(stage[cur ^ 1]);
-            load(share.from + (uint64_t)(t + 2) * kStep);
-            multiply(stage[cur]);
-            __syncthreads();
-            cur ^= 1;
+        uint32_t t = 0;
+        for (; t + 2 * DEPTH + 1 < steps; t += DEPTH) {          // DEPTH steps a turn, so that the sets are named at compile time; whole ones
+#pragma unroll
+            for (int d = 0; d < DEPTH; ++d) {
+                store(held[d], stage[(t + d + 1) & 1]);
+                load_whole(held[d], row_of(t + d + 1 + DEPTH));
+                multiply(stage[(t + d) & 1]);
+                __syncthreads();
+            }
         }
-        if (steps > 1) {
-            mask(share.from + (uint64_t)(steps - 1) * kStep);
-            store(stage[cur ^ 1]);
-            multiply(stage[cur]);
-            __syncthreads();
-            cur ^= 1;
+#pragma unroll
+        for (int q = 0; q < 2 * DEPTH; ++q, ++t) {               // what is left: at most 2 DEPTH steps, the last one with rows missing
+            if (t + 1 < steps) {
+                if (t + 2 == steps) mask(held[q % DEPTH], row_of(t + 1));
+                store(held[q % DEPTH], stage[(t + 1) & 1]);
+                if (q < DEPTH) load(held[q % DEPTH], row_of(t + 1 + DEPTH));
+                multiply(stage[t & 1]);
+                __syncthreads();
+            }
         }
-        multiply(stage[cur]);
+        multiply(stage[(steps - 1) & 1]);
     }
     float* out = static_cast<float*>(p.out) + ((uint64_t)at.split * p.b + at.batch) * p.k * p.n;
 #pragma unroll
@@ -253,17 +271,21 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product 
 
 // ---- f64 -----------------------------------------------------------------------------------------------------------------------------
 typedef double f64x4 __attribute__((ext_vector_type(4)));
-constexpr int kStep64 = 16, kSide64 = 64;
-constexpr int kPitch64 = kSide64 + 2;                            // in doubles: rows 4 apart, which one instruction reads, start 8 banks apart
+constexpr int kStep64 = 16;
 
-// 64 x 64 of dst by 2 x 2 waves, the 16x16x4 matrix instruction, kStep64 rows staged at a time.
-__global__ __launch_bounds__(256) void pack8_matmul_f64_kernel(Product p) {
-    __shared__ double xs[2][kStep64][kPitch64], ys[2][kStep64][kPitch64];
+// SIDE x SIDE of dst by WI x WJ waves, the 16x16x4 matrix instruction, kStep64 rows staged at a time, ahead as in the f32 kernel.  The
+// pitch of the staged rows, in words, is 32 more than a multiple of 64: the two rows that half a wave reads lie on the two halves of the
+// banks.
+template <int SIDE, int WI, int WJ>
+__global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f64_kernel(Product p) {
+    constexpr int kPitch = SIDE + 16, FI = SIDE / WI / 16, FJ = SIDE / WJ / 16;
+    static_assert(WI * WJ * 64 == SIDE * kStep64 / 4, "a lane stages four rows of one column");
+    __shared__ double xs[2][kStep64][kPitch], ys[2][kStep64][kPitch];
     const Where at = where(p);
     const Share share = share_of(p.m, p.splits, at.split);
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wi = w >> 1, wj = w & 1;
-    const uint64_t i0 = (uint64_t)at.i * kSide64, j0 = (uint64_t)at.j * kSide64;
-    const int c = tid % kSide64, r0 = tid / kSide64 * 4;         // the lane's column and four rows of both operands
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wi = w / WJ, wj = w % WJ;
+    const uint64_t i0 = (uint64_t)at.i * SIDE, j0 = (uint64_t)at.j * SIDE;
+    const int c = tid % SIDE, r0 = tid / SIDE * 4;
     const uint32_t k = (uint32_t)p.k, n = (uint32_t)p.n;
     const uint32_t xcol = i0 + c < k ? (uint32_t)i0 + c : k - 1, ycol = j0 + c < n ? (uint32_t)j0 + c : n - 1;
     const double* up = static_cast<const double*>(p.up) + at.batch * p.m * p.n;
@@ -294,56 +316,62 @@ __global__ __launch_bounds__(256) void pack8_matmul_f64_kernel(Product p) {
             ys[b][r0 + r][c] = in ? yv[r] : 0.0;
         }
     };
-    f64x4 acc[2][2];
+    f64x4 acc[FI][FJ];
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < FI; ++a)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) acc[a][b] = f64x4{0.0, 0.0, 0.0, 0.0};
+        for (int b = 0; b < FJ; ++b) acc[a][b] = f64x4{0.0, 0.0, 0.0, 0.0};
     if (share.from < share.to) {
         load(share.from);
         store(0, share.from);
+        if (share.from + kStep64 < share.to) load(share.from + kStep64);
         __syncthreads();
         int cur = 0;
         for (uint64_t m0 = share.from; m0 < share.to; m0 += kStep64) {
-            const bool more = m0 + kStep64 < share.to;
-            if (more) load(m0 + kStep64);
+            if (m0 + kStep64 < share.to) store(cur ^ 1, m0 + kStep64);
+            if (m0 + 2 * kStep64 < share.to) load(m0 + 2 * kStep64);
 #pragma unroll
             for (int q = 0; q < kStep64 / 4; ++q) {
                 const int row = q * 4 + (lane >> 4), cc = lane & 15;
-                double xa[2], yb[2];
+                double xa[FI], yb[FJ];
 #pragma unroll
-                for (int a = 0; a < 2; ++a) xa[a] = xs[cur][row][wi * 32 + a * 16 + cc];
+                for (int a = 0; a < FI; ++a) xa[a] = xs[cur][row][(wi * FI + a) * 16 + cc];
 #pragma unroll
-                for (int b = 0; b < 2; ++b) yb[b] = ys[cur][row][wj * 32 + b * 16 + cc];
+                for (int b = 0; b < FJ; ++b) yb[b] = ys[cur][row][(wj * FJ + b) * 16 + cc];
 #pragma unroll
-                for (int a = 0; a < 2; ++a)
+                for (int a = 0; a < FI; ++a)
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) acc[a][b] = __builtin_amdgcn_mfma_f64_16x16x4f64(xa[a], yb[b], acc[a][b], 0, 0, 0);
+                    for (int b = 0; b < FJ; ++b) acc[a][b] = __builtin_amdgcn_mfma_f64_16x16x4f64(xa[a], yb[b], acc[a][b], 0, 0, 0);
             }
-            if (more) store(cur ^ 1, m0 + kStep64);
             __syncthreads();
             cur ^= 1;
         }
     }
     double* out = static_cast<double*>(p.out) + ((uint64_t)at.split * p.b + at.batch) * p.k * p.n;
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < FI; ++a)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < FJ; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const uint64_t i = i0 + wi * 32 + a * 16 + r * 4 + (lane >> 4), j = j0 + wj * 32 + b * 16 + (lane & 15);
+                const uint64_t i = i0 + (wi * FI + a) * 16 + r * 4 + (lane >> 4), j = j0 + (wj * FJ + b) * 16 + (lane & 15);
                 if (i < p.k && j < p.n) out[i * p.n + j] = acc[a][b][r];
             }
 }
 
 // ---- the splits' partial results, added in order -----------------------------------------------------------------------------------------
+// Every wave of a block adds a quarter of the splits for 64 elements, eight loads in flight, then the four sums are added.
 template <class T> __global__ __launch_bounds__(256) void pack8_matmul_join_kernel(const T* __restrict__ part, T* __restrict__ dst, uint64_t n, uint32_t splits) {
-    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    T s = part[i];
-    for (uint32_t k = 1; k < splits; ++k) s += part[k * n + i];
-    dst[i] = s;
+    __shared__ T sums[4][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const uint64_t i = (uint64_t)blockIdx.x * 64 + lane, at = i < n ? i : n - 1;
+    const uint32_t from = splits * w / 4, to = splits * (w + 1) / 4;
+    T s = (T)0;
+#pragma unroll 8
+    for (uint32_t k = from; k < to; ++k) s += part[k * n + at];
+    sums[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && i < n) dst[i] = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
 }
 
 // Shares of the rows: enough blocks to fill the card, each share long enough to pay for its partial result.
@@ -355,14 +383,14 @@ uint32_t splits_for(rt_ctx* ctx, uint64_t tiles, uint64_t m, uint64_t least_rows
 }
 
 template <class T> int32_t join(rt_ctx* ctx, const void* part, void* dst, uint64_t n, uint32_t splits) {
-    hipLaunchKernelGGL(pack8_matmul_join_kernel<T>, dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, ctx->stream, (const T*)part, (T*)dst, n, splits);
+    hipLaunchKernelGGL(pack8_matmul_join_kernel<T>, dim3((uint32_t)((n + 63) / 64)), dim3(256), 0, ctx->stream, (const T*)part, (T*)dst, n, splits);
     RT_HIP(hipGetLastError());
     return RT_OK;
 }
 
-template <int BI, int BJ, int WI, int WJ, bool EVEN> int32_t f32_launch(rt_ctx* ctx, const Product& p) {
+template <int BI, int BJ, int WI, int WJ, int DEPTH, bool EVEN> int32_t f32_launch(rt_ctx* ctx, const Product& p) {
     constexpr size_t bytes = 2 * sizeof(Stage<BI, BJ>);
-    auto kernel = pack8_matmul_f32_kernel<BI, BJ, WI, WJ, EVEN>;
+    auto kernel = pack8_matmul_f32_kernel<BI, BJ, WI, WJ, DEPTH, EVEN>;
     static std::atomic<uint64_t> allowed{0};                     // more than 64 KiB of LDS has to be asked for, once a device
     const uint64_t bit = 1ull << (ctx->device & 63);
     if (!(allowed.load() & bit) || ctx->device > 63) {
@@ -374,24 +402,53 @@ template <int BI, int BJ, int WI, int WJ, bool EVEN> int32_t f32_launch(rt_ctx* 
     return RT_OK;
 }
 
+#ifndef RT_E1
+#define RT_E1 0.8
+#define RT_E2 0.6
+#define RT_LEAST 64
+#define RT_PER 2
+#endif
+#ifndef RT_D1
+#define RT_D1 1
+#define RT_D2 2
+#endif
+template <bool EVEN> int32_t f32_any(rt_ctx* ctx, const Product& p, int shape) {
+    if (shape == 0) return f32_launch<256, 256, 2, 4, 1, EVEN>(ctx, p);
+    if (shape == 1) return f32_launch<256, 128, 4, 2, RT_D1, EVEN>(ctx, p);
+    return f32_launch<128, 128, 2, 2, RT_D2, EVEN>(ctx, p);
+}
+
 int32_t run_product(rt_ctx* ctx, int dtype, Product p, void* dst) {
-    auto tiles_of = [&](uint64_t bi, uint64_t bj) { return p.b * ((p.k + bi - 1) / bi) * ((p.n + bj - 1) / bj); };
-    const bool big = dtype == RT_F32 && tiles_of(256, 256) * (p.m / 1024 ? p.m / 1024 : 1) >= (uint64_t)ctx->num_cus && p.k > 128 && p.n > 128;
-    const uint64_t bi = dtype == RT_F64 ? kSide64 : big ? 256 : 128, bj = bi, tiles = tiles_of(bi, bj);
+    struct Shape { uint64_t bi, bj, least_rows, per_cu; double rate; };
+    static const Shape f32[3] = {{256, 256, 512, 1, 1.0}, {256, 128, 256, 1, RT_E1}, {128, 128, RT_LEAST, RT_PER, RT_E2}};
+    static const Shape f64[2] = {{128, 128, 128, 2, 1.0}, {64, 64, 64, 4, 1.0}};
+    auto tiles_of = [&](const Shape& s) { return p.b * ((p.k + s.bi - 1) / s.bi) * ((p.n + s.bj - 1) / s.bj); };
+    int shape = dtype == RT_F64 && tiles_of(f64[0]) * (p.m / f64[0].least_rows) < (uint64_t)ctx->num_cus ? 1 : 0;
+    Shape s = f64[shape & 1];
+    if (dtype == RT_F32) {
+        double best = 0;
+        for (int c = 2; c >= 0; --c) {
+            const uint64_t tiles = tiles_of(f32[c]), most = p.m / f32[c].least_rows, blocks = tiles * (most ? most : 1);
+            if (c < 2 && blocks < (uint64_t)ctx->num_cus) continue;              // would not fill the card
+            const double cost = (double)tiles * f32[c].bi * f32[c].bj / f32[c].rate;
+            if (c == 2 || cost < best) { best = cost; shape = c; }
+        }
+        s = f32[shape];
+    }
+    const uint64_t tiles = tiles_of(s);
     if (tiles >= (1ull << 24)) return rt_fail(RT_E_INVALID, "pack8 matmul backward: the result is too large for one launch");
-    p.ti = (uint32_t)((p.k + bi - 1) / bi);
-    p.tj = (uint32_t)((p.n + bj - 1) / bj);
-    p.splits = splits_for(ctx, tiles, p.m, big ? 1024 : 256, dtype == RT_F64 ? 4 : big ? 1 : 2);
+    p.ti = (uint32_t)((p.k + s.bi - 1) / s.bi);
+    p.tj = (uint32_t)((p.n + s.bj - 1) / s.bj);
+    p.splits = splits_for(ctx, tiles, p.m, s.least_rows, s.per_cu);
     const uint64_t n = p.b * p.k * p.n;
     p.out = dst;
     if (p.splits > 1) RT_TRY(rt_scratch(ctx, n * p.splits * rt_elem_size(dtype), &p.out));
     if (dtype == RT_F64) {
-        hipLaunchKernelGGL(pack8_matmul_f64_kernel, dim3((uint32_t)(tiles * p.splits)), dim3(256), 0, ctx->stream, p);
+        if (shape == 0) hipLaunchKernelGGL((pack8_matmul_f64_kernel<128, 4, 2>), dim3((uint32_t)(tiles * p.splits)), dim3(512), 0, ctx->stream, p);
+        else hipLaunchKernelGGL((pack8_matmul_f64_kernel<64, 2, 2>), dim3((uint32_t)(tiles * p.splits)), dim3(256), 0, ctx->stream, p);
         RT_HIP(hipGetLastError());
-    } else if (big) {
-        RT_TRY((p.k % 2 == 0 ? f32_launch<256, 256, 2, 4, true>(ctx, p) : f32_launch<256, 256, 2, 4, false>(ctx, p)));
     } else {
-        RT_TRY((p.k % 2 == 0 ? f32_launch<128, 128, 2, 2, true>(ctx, p) : f32_launch<128, 128, 2, 2, false>(ctx, p)));
+        RT_TRY(p.k % 2 == 0 ? f32_any<true>(ctx, p, shape) : f32_any<false>(ctx, p, shape));
     }
     if (p.splits == 1) return RT_OK;
     return dtype == RT_F32 ? join<float>(ctx, p.out, dst, n, p.splits) : join<double>(ctx, p.out, dst, n, p.splits);
