@@ -292,60 +292,81 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f64_kernel(Product 
     int32_t cx[4];
     uint32_t ex[4];
     double yv[4];
+    const uint32_t xoff = (uint32_t)r0 * k + xcol, yoff = (uint32_t)r0 * n + ycol;
+    auto load_row = [&](int r, uint64_t from, uint32_t xo, uint32_t yo) {        // from: a wave-uniform row; xo, yo: places from its start
+        const uint64_t e = (at.batch * p.m + from) * k;
+        cx[r] = (p.codes + e)[xo];
+        ex[r] = (p.exps + e / kP8Group)[((uint32_t)e % kP8Group + xo) / kP8Group];
+        yv[r] = (up + from * n)[yo];
+    };
     auto load = [&](uint64_t m0) {
+        if (m0 >= share.to) return;
         const int rows = share.to - m0 < (uint64_t)kStep64 ? (int)(share.to - m0) : kStep64;
-        const uint64_t xe = (at.batch * p.m + m0) * k;
-        const int8_t* codes = p.codes + xe;
-        const uint8_t* exps = p.exps + xe / kP8Group;
-        const double* y = up + m0 * n;
-        const uint32_t rem = (uint32_t)xe % kP8Group;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = r0 + r < rows ? r0 + r : rows - 1;
-            const uint32_t e = (uint32_t)row * k + xcol;
-            cx[r] = codes[e];
-            ex[r] = exps[(rem + e) / kP8Group];
-            yv[r] = y[(uint32_t)row * n + ycol];
+            const uint32_t row = r0 + r < rows ? r0 + r : rows - 1;
+            load_row(r, m0, row * k + xcol, row * n + ycol);
         }
     };
-    auto store = [&](int b, uint64_t m0) {
+    auto store = [&](int b) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const bool in = m0 + r0 + r < share.to;
-            xs[b][r0 + r][c] = in ? p8_value<double>(cx[r], ex[r]) : 0.0;
-            ys[b][r0 + r][c] = in ? yv[r] : 0.0;
+            xs[b][r0 + r][c] = p8_value<double>(cx[r], ex[r]);
+            ys[b][r0 + r][c] = yv[r];
         }
+    };
+    auto mask = [&](uint64_t m0) {                               // rows behind the last one are zeros
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (m0 + r0 + r >= share.to) { cx[r] = 0; ex[r] = 0u; yv[r] = 0.0; }
     };
     f64x4 acc[FI][FJ];
 #pragma unroll
     for (int a = 0; a < FI; ++a)
 #pragma unroll
         for (int b = 0; b < FJ; ++b) acc[a][b] = f64x4{0.0, 0.0, 0.0, 0.0};
-    if (share.from < share.to) {
-        load(share.from);
-        store(0, share.from);
-        if (share.from + kStep64 < share.to) load(share.from + kStep64);
-        __syncthreads();
-        int cur = 0;
-        for (uint64_t m0 = share.from; m0 < share.to; m0 += kStep64) {
-            if (m0 + kStep64 < share.to) store(cur ^ 1, m0 + kStep64);
-            if (m0 + 2 * kStep64 < share.to) load(m0 + 2 * kStep64);
+    auto multiply = [&](int cur) {
 #pragma unroll
-            for (int q = 0; q < kStep64 / 4; ++q) {
-                const int row = q * 4 + (lane >> 4), cc = lane & 15;
-                double xa[FI], yb[FJ];
+        for (int q = 0; q < kStep64 / 4; ++q) {
+            const int row = q * 4 + (lane >> 4), cc = lane & 15;
+            double xa[FI], yb[FJ];
 #pragma unroll
-                for (int a = 0; a < FI; ++a) xa[a] = xs[cur][row][(wi * FI + a) * 16 + cc];
+            for (int a = 0; a < FI; ++a) xa[a] = xs[cur][row][(wi * FI + a) * 16 + cc];
 #pragma unroll
-                for (int b = 0; b < FJ; ++b) yb[b] = ys[cur][row][(wj * FJ + b) * 16 + cc];
+            for (int b = 0; b < FJ; ++b) yb[b] = ys[cur][row][(wj * FJ + b) * 16 + cc];
 #pragma unroll
-                for (int a = 0; a < FI; ++a)
+            for (int a = 0; a < FI; ++a)
 #pragma unroll
-                    for (int b = 0; b < FJ; ++b) acc[a][b] = __builtin_amdgcn_mfma_f64_16x16x4f64(xa[a], yb[b], acc[a][b], 0, 0, 0);
-            }
-            __syncthreads();
-            cur ^= 1;
+                for (int b = 0; b < FJ; ++b) acc[a][b] = __builtin_amdgcn_mfma_f64_16x16x4f64(xa[a], yb[b], acc[a][b], 0, 0, 0);
         }
+    };
+    if (share.from < share.to) {
+        const uint32_t steps = (uint32_t)((share.to - share.from + kStep64 - 1) / kStep64);
+        auto row_of = [&](uint32_t t) { return share.from + (uint64_t)t * kStep64; };
+        load(row_of(0));
+        if (steps == 1) mask(row_of(0));
+        store(0);
+        load(row_of(1));
+        __syncthreads();
+        uint32_t t = 0;
+        for (; t + 3 < steps; ++t) {                             // whole steps
+            store((t + 1) & 1);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) load_row(r, row_of(t + 2) + r, xoff, yoff);
+            multiply(t & 1);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q, ++t) {                       // what is left: at most two steps, the last one with rows missing
+            if (t + 1 < steps) {
+                if (t + 2 == steps) mask(row_of(t + 1));
+                store((t + 1) & 1);
+                if (q == 0) load(row_of(t + 2));
+                multiply(t & 1);
+                __syncthreads();
+            }
+        }
+        multiply((steps - 1) & 1);
     }
     double* out = static_cast<double*>(p.out) + ((uint64_t)at.split * p.b + at.batch) * p.k * p.n;
 #pragma unroll
