@@ -2,6 +2,8 @@
 #include "rt_pack8.h"
 #include "rt_unary_math.h"
 
+#include <atomic>
+
 namespace {
 
 constexpr int kSBlock = 256;
@@ -266,18 +268,19 @@ template <class T, int W> __device__ __forceinline__ uint32_t take_tile(const Ch
 }
 
 // Joins the W stretches of a tile (one a wave, in the order of the waves) with the tiles before it.  (A, H) of the wave's own stretch;
-// cut: nothing crosses the stretch (wave-uniform; A has no meaning then); first: the state before tile 0.  `run(start)` goes through
-// the stretch from its start state and returns the state it ends at; so does this function.
+// cut: nothing crosses the stretch (wave-uniform; A has no meaning then); odd: a product inside the stretch left the range (see below);
+// first: the state before tile 0.  `run(start, serial)` goes through the stretch from its start state and returns the state it ends at;
+// so does this function.
 //
 // A product of factors above 1 can leave the range while the states stay inside it (a start of zero, say).  Where one does, the tile's
 // stretches run one after the other and only its end state is published: the plain loop's result, at the plain loop's pace.
 template <class T, int W, class Run>
-__device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W>& room, uint32_t item, uint32_t k, T A, T H, bool cut, T first, Run run) {
+__device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W>& room, uint32_t item, uint32_t k, T A, T H, bool cut, bool odd, T first, Run run) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const bool last = k == ch.tiles - 1;
     room.A[w][lane] = A;
     room.H[w][lane] = H;
-    if (lane == 0) room.cut[w] = cut ? 1u : 0u;
+    if (lane == 0) room.cut[w] = (cut ? 1u : 0u) | (odd ? 2u : 0u);
     __syncthreads();
     const uint32_t epoch = ch.epoch;
     T ta = (T)1, th = (T)0;
@@ -285,7 +288,8 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W>& room, ui
 #pragma unroll
     for (int v = 0; v < W; ++v) {
         const T av = room.A[v][lane], hv = room.H[v][lane];
-        if (room.cut[v]) {
+        bad = bad || (room.cut[v] & 2u);
+        if (room.cut[v] & 1u) {
             th = hv;
             tcut = true;
         } else {
@@ -321,9 +325,9 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W>& room, ui
         if (!serial || turn == w) {
             if (serial) start = room.start[lane];
             else {
-                for (int v = 0; v < w; ++v) start = room.cut[v] ? room.H[v][lane] : fused(room.A[v][lane], start, room.H[v][lane]);
+                for (int v = 0; v < w; ++v) start = room.cut[v] & 1u ? room.H[v][lane] : fused(room.A[v][lane], start, room.H[v][lane]);
             }
-            end = run(start);
+            end = run(start, serial);
             if (serial) room.start[lane] = end;
         }
         if (serial) __syncthreads();
@@ -388,7 +392,7 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
     }
     const T first = k == 0 && a.state ? a.state[sc] : (T)0;
     T* h = a.h + base;
-    const T end = join_tile<T, W>(ch, room, item, k, A, H, cuts != 0, first, [&](T p) {
+    const T end = join_tile<T, W>(ch, room, item, k, A, H, cuts != 0, false, first, [&](T p, bool) {
         RT_APART;
         if (in) {
 #pragma unroll
@@ -462,7 +466,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
     }
     const T first = k == 0 && a.dlast ? a.dlast[sc] : (T)0;
     T *dg = a.dgate + base, *dx = a.dx + base;
-    const T end = join_tile<T, W>(ch, room, item, k, A, H, cuts != 0, first, [&](T d) {
+    const T end = join_tile<T, W>(ch, room, item, k, A, H, cuts != 0, false, first, [&](T d, bool) {
         RT_APART;
         uint64_t rresets = resets;
         RT_PIN(rresets);
@@ -491,6 +495,285 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
         const T g0 = a.gate[(uint64_t)o * a.steps * row + col];
         const bool none = (a.reset && a.reset[(uint64_t)o * a.steps]) || (FORM == RT_SCAN_LINEAR && !a.state);
         a.dstate[sc] = none ? (T)0 : (FORM == RT_SCAN_SIGMOID ? gate_of(g0).s : g0) * end;
+    }
+}
+
+// ---- few columns: the steps go over the lanes too --------------------------------------------------------------------------------------
+// A tile is one contiguous run of memory, `ls` steps for each of the block's segments; it is staged through LDS, a lane takes one column
+// of one segment, and the segments of a wave are joined with lane exchanges before the waves and the tiles are.  Short rows are taken
+// `rows` at a time as one line with a cut at every row's start.
+struct Narrow {
+    uint64_t rows;           // of `outer`, in one line
+    uint32_t ls;             // steps of a segment, at most kSeg
+    uint32_t shift;          // lanes of one segment: 1 << shift >= inner
+    FastDiv32 by_inner, by_steps;
+};
+template <class T> constexpr int seg_steps() { return sizeof(T) == 4 ? 16 : 8; }
+template <class T, int W> struct Tile {
+    static constexpr uint32_t kMost = W * 64 * seg_steps<T>();   // elements
+    static constexpr uint32_t kLine = 64 / sizeof(T);            // one element of padding for each of these: a wave's segments start in
+                                                                 // different banks
+    static __device__ __forceinline__ uint32_t at(uint32_t e) { return e + e / kLine; }
+    T a[kMost + 64 + (kMost + 64) / kLine], b[kMost + kMost / kLine];
+    uint8_t reset[kMost + 1];
+};
+// What joins a wave's segments: the exclusive prefix of the lane's segment, and the wave's whole.
+template <class T> struct Prefix {
+    T A, H, wholeA, wholeH;
+    bool cut, any_cut, odd;
+};
+template <class T> __device__ __forceinline__ Prefix<T> join_lanes(T A, T H, bool cut, int lane, uint32_t shift) {
+    bool odd = !finite(A);
+    for (uint32_t d = 1u << shift; d < 64; d <<= 1) {
+        const T A1 = __shfl_up(A, d), H1 = __shfl_up(H, d);
+        const bool c1 = __shfl_up((int)cut, d) != 0;
+        if (lane >= (int)d) {
+            H = cut ? H : fused(A, H1, H);
+            cut = cut || c1;
+            A = cut ? (T)0 : A1 * A;
+            odd = odd || !finite(A);
+        }
+    }
+    const int top = 64 - (1 << shift) + (lane & ((1 << shift) - 1));
+    Prefix<T> p;
+    p.wholeA = __shfl(A, top);
+    p.wholeH = __shfl(H, top);
+    p.any_cut = __any(cut);
+    p.odd = __any(odd);
+    const T A0 = __shfl_up(A, 1u << shift), H0 = __shfl_up(H, 1u << shift);
+    const bool c0 = __shfl_up((int)cut, 1u << shift) != 0;
+    const bool head = lane < (1 << shift);
+    p.A = head ? (T)1 : A0;
+    p.H = head ? (T)0 : H0;
+    p.cut = !head && c0;
+    return p;
+}
+// Runs a wave's segments from the wave's start state: `go(start)` goes through the lane's segment and returns where it ends.
+template <class T, class Go> __device__ __forceinline__ T run_lanes(const Prefix<T>& p, T start, bool serial, int lane, uint32_t shift, Go go) {
+    const int c = lane & ((1 << shift) - 1), seg = lane >> shift;
+    T end = start;
+    for (int s = 0; s < (serial ? 64 >> shift : 1); ++s) {
+        if (!serial) end = go(seg == 0 ? start : p.cut ? p.H : fused(p.A, start, p.H));
+        else {
+            if (seg == s) end = go(start);
+            start = __shfl(end, (s << shift) + c);
+        }
+    }
+    return __shfl(end, 64 - (1 << shift) + c);
+}
+
+// Segment of a lane: a wave's lanes hold 64 >> shift consecutive ones.
+__device__ __forceinline__ int tile_segment(int tid, uint32_t shift) { return (tid >> 6) * (64 >> shift) + ((tid & 63) >> shift); }
+
+template <class T, int FORM, int W>
+__global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chain ch, Narrow nw) {
+    constexpr int kSeg = seg_steps<T>(), kThreads = W * 64;
+    __shared__ JoinRoom<T, W> room;
+    extern __shared__ __align__(16) char lds[];
+    Tile<T, W>& tile = *reinterpret_cast<Tile<T, W>*>(lds);
+    typedef Tile<T, W> TT;
+    const uint32_t line = line_of_block(ch), k = take_tile<T, W>(ch, line, room), item = k * ch.lines + line;
+    if (k >= ch.tiles) return;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const uint32_t inner = (uint32_t)a.inner, segs = kThreads >> nw.shift;
+    const uint64_t row0 = (uint64_t)line * nw.rows, rows = a.outer - row0 < nw.rows ? a.outer - row0 : nw.rows, len = rows * a.steps;
+    const uint64_t u0 = (uint64_t)k * segs * nw.ls;              // first step of the tile in the line
+    const uint32_t cnt = len <= u0 ? 0 : (uint32_t)(len - u0 < (uint64_t)segs * nw.ls ? len - u0 : (uint64_t)segs * nw.ls), E = cnt * inner;
+    const uint64_t step0 = row0 * a.steps + u0, base = step0 * inner;
+    {
+        T g[kSeg], x[kSeg];                                      // all loads before the first write
+#pragma unroll
+        for (int q = 0; q < kSeg; ++q) {
+            const uint32_t e = tid + q * kThreads;
+            if (e < E) {
+                g[q] = __builtin_nontemporal_load(a.gate + base + e);
+                x[q] = __builtin_nontemporal_load(a.x + base + e);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < kSeg; ++q) {
+            const uint32_t e = tid + q * kThreads;
+            if (e < E) {
+                tile.a[TT::at(e)] = g[q];
+                tile.b[TT::at(e)] = x[q];
+            }
+        }
+    }
+    if (a.reset)
+        for (uint32_t e = tid; e < cnt; e += kThreads) tile.reset[e] = a.reset[step0 + e];
+    __syncthreads();
+    const uint32_t c = lane & ((1u << nw.shift) - 1), v0 = (uint32_t)tile_segment(tid, nw.shift) * nw.ls;
+    const int n = c >= inner || v0 >= cnt ? 0 : (int)(cnt - v0 < nw.ls ? cnt - v0 : nw.ls);
+    // the row of the segment's first step and the step's place in it
+    const uint64_t row_of = nw.rows == 1 ? 0 : fd_div((uint32_t)u0 + v0, nw.by_steps);
+    const uint64_t rem0 = u0 + v0 - row_of * a.steps;
+    T f[kSeg], b[kSeg], A = (T)1, H = (T)0;
+    uint32_t cuts = 0;
+    {
+        uint64_t rem = rem0, row = row0 + row_of;
+#pragma unroll
+        for (int j = 0; j < kSeg; ++j) {
+            if (j < n) {
+                const uint32_t e = TT::at((v0 + j) * inner + c);
+                f[j] = tile.a[e];
+                b[j] = tile.b[e];
+                if constexpr (FORM == RT_SCAN_SIGMOID) {
+                    const RtGate<T> q = gate_of(f[j]);
+                    f[j] = q.s;
+                    b[j] = q.r * b[j];
+                }
+                const bool head = rem == 0, reset = a.reset && tile.reset[v0 + j];
+                if (head && a.state && !reset) b[j] = fused(f[j], a.state[row * inner + c], b[j]);
+                if (head || reset) cuts |= 1u << j;
+                H = j == 0 || (cuts >> j & 1) ? b[j] : fused(f[j], H, b[j]);
+                A = cuts ? (T)0 : A * f[j];
+                if (++rem == a.steps) { rem = 0; ++row; }
+            }
+        }
+    }
+    const Prefix<T> pre = join_lanes(A, H, cuts != 0, lane, nw.shift);
+    join_tile<T, W>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
+        return run_lanes(pre, start, serial, lane, nw.shift, [&](T p) {
+            uint64_t rem = rem0, row = row0 + row_of;
+#pragma unroll
+            for (int j = 0; j < kSeg; ++j) {
+                if (j < n) {
+                    p = cuts >> j & 1 ? b[j] : fused(f[j], p, b[j]);
+                    tile.b[TT::at((v0 + j) * inner + c)] = p;
+                    if (++rem == a.steps) {
+                        if (a.last) a.last[row * inner + c] = p;
+                        rem = 0;
+                        ++row;
+                    }
+                }
+            }
+            return p;
+        });
+    });
+    __syncthreads();
+    for (uint32_t e = tid; e < E; e += kThreads) __builtin_nontemporal_store(tile.b[TT::at(e)], a.h + base + e);
+}
+
+// Backward: the segments go through the tile from its end.  Only D comes out of the recurrence; the gradients are formed from it element
+// by element afterwards, in memory order.
+template <class T, int FORM, class S, int W>
+__global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T, S> a, Chain ch, Narrow nw) {
+    constexpr int kSeg = seg_steps<T>(), kThreads = W * 64;
+    __shared__ JoinRoom<T, W> room;
+    extern __shared__ __align__(16) char lds[];
+    Tile<T, W>& tile = *reinterpret_cast<Tile<T, W>*>(lds);
+    typedef Tile<T, W> TT;
+    const uint32_t line = line_of_block(ch), k = take_tile<T, W>(ch, line, room), item = k * ch.lines + line;
+    if (k >= ch.tiles) return;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const uint32_t inner = (uint32_t)a.inner, segs = kThreads >> nw.shift;
+    const uint64_t row0 = (uint64_t)line * nw.rows, rows = a.outer - row0 < nw.rows ? a.outer - row0 : nw.rows, len = rows * a.steps;
+    const uint64_t r0 = (uint64_t)k * segs * nw.ls;              // steps of the line behind the tile
+    const uint32_t cnt = len <= r0 ? 0 : (uint32_t)(len - r0 < (uint64_t)segs * nw.ls ? len - r0 : (uint64_t)segs * nw.ls), E = cnt * inner;
+    const uint64_t lo = len - r0 - cnt;                          // first step of the tile in the line
+    const uint64_t step0 = row0 * a.steps + lo, base = step0 * inner;
+    const uint32_t behind = r0 ? inner : 0;                      // the gates of one step more
+    {
+        T g[kSeg], d[kSeg];                                      // all loads before the first write
+#pragma unroll
+        for (int q = 0; q < kSeg; ++q) {
+            const uint32_t e = tid + q * kThreads;
+            if (e < E) {
+                g[q] = a.gate[base + e];
+                d[q] = __builtin_nontemporal_load(a.dh + base + e);
+            }
+        }
+        if ((uint32_t)tid < behind) tile.a[TT::at(E + tid)] = a.gate[base + E + tid];
+#pragma unroll
+        for (int q = 0; q < kSeg; ++q) {
+            const uint32_t e = tid + q * kThreads;
+            if (e < E) {
+                tile.a[TT::at(e)] = g[q];
+                tile.b[TT::at(e)] = d[q];
+            }
+        }
+    }
+    if (a.reset)
+        for (uint32_t e = tid; e < cnt + (r0 ? 1 : 0); e += kThreads) tile.reset[e] = a.reset[step0 + e];
+    __syncthreads();
+    const uint32_t c = lane & ((1u << nw.shift) - 1), q0 = (uint32_t)tile_segment(tid, nw.shift) * nw.ls;
+    const int n = c >= inner || q0 >= cnt ? 0 : (int)(cnt - q0 < nw.ls ? cnt - q0 : nw.ls);
+    const uint32_t v0 = n ? cnt - 1 - q0 : 0;                    // the segment's last step in the tile; it goes down from there
+    const uint64_t row_of = nw.rows == 1 ? 0 : fd_div((uint32_t)lo + v0, nw.by_steps);
+    T f[kSeg], b[kSeg], A = (T)1, H = (T)0;
+    uint32_t cuts = 0;
+    {
+        uint64_t t = lo + v0 - row_of * a.steps, row = row0 + row_of;
+#pragma unroll
+        for (int j = 0; j < kSeg; ++j) {
+            if (j < n) {
+                const uint32_t v = v0 - j;
+                b[j] = tile.b[TT::at(v * inner + c)];
+                f[j] = (T)0;
+                const bool tail = t == a.steps - 1;
+                if (tail) {
+                    if (a.dlast) b[j] += a.dlast[row * inner + c];
+                } else {
+                    f[j] = tile.a[TT::at((v + 1) * inner + c)];
+                    if constexpr (FORM == RT_SCAN_SIGMOID) f[j] = gate_of(f[j]).s;
+                }
+                if (tail || (a.reset && tile.reset[v + 1])) cuts |= 1u << j;
+                H = j == 0 || (cuts >> j & 1) ? b[j] : fused(f[j], H, b[j]);
+                A = cuts ? (T)0 : A * f[j];
+                if (t == 0) { t = a.steps; --row; }
+                --t;
+            }
+        }
+    }
+    const Prefix<T> pre = join_lanes(A, H, cuts != 0, lane, nw.shift);
+    join_tile<T, W>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
+        return run_lanes(pre, start, serial, lane, nw.shift, [&](T d) {
+#pragma unroll
+            for (int j = 0; j < kSeg; ++j) {
+                if (j < n) {
+                    d = cuts >> j & 1 ? b[j] : fused(f[j], d, b[j]);
+                    tile.b[TT::at((v0 - j) * inner + c)] = d;
+                }
+            }
+            return d;
+        });
+    });
+    __syncthreads();
+    constexpr int kBatch = 4;                                    // elements whose h and x are on their way at once
+    for (uint32_t e0 = tid; e0 < E; e0 += kThreads * kBatch) {
+        T p[kBatch], x[kBatch];
+        uint64_t sc[kBatch];
+        bool head[kBatch], reset[kBatch];
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {
+            const uint32_t e = e0 + q * kThreads < E ? e0 + q * kThreads : e0, v = fd_div(e, nw.by_inner);
+            const uint64_t u = lo + v;
+            const uint64_t row = nw.rows == 1 ? 0 : fd_div((uint32_t)u, nw.by_steps);
+            head[q] = u == row * a.steps;
+            reset[q] = a.reset && tile.reset[v];
+            sc[q] = (row0 + row) * inner + (e - v * inner);
+            p[q] = (T)0;
+            if (!head[q]) p[q] = a.h.at(base - inner, e);
+            else if (a.state) p[q] = a.state[sc[q]];
+            if constexpr (FORM == RT_SCAN_SIGMOID) x[q] = a.x.at(base, e);
+        }
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {
+            const uint32_t e = e0 + q * kThreads;
+            if (e >= E) continue;
+            const T d = tile.b[TT::at(e)], g = tile.a[TT::at(e)], before = reset[q] ? (T)0 : p[q];
+            T factor = g;
+            if constexpr (FORM == RT_SCAN_LINEAR) {
+                __builtin_nontemporal_store(reset[q] || (head[q] && !a.state) ? (T)0 : d * before, a.dgate + base + e);
+                __builtin_nontemporal_store(d, a.dx + base + e);
+            } else {
+                const RtGate<T> f = gate_of(g);
+                factor = f.s;
+                __builtin_nontemporal_store(d * (before - x[q]) * (f.s * f.r), a.dgate + base + e);
+                __builtin_nontemporal_store(f.r * d, a.dx + base + e);
+            }
+            if (head[q] && a.dstate) a.dstate[sc[q]] = reset[q] || (FORM == RT_SCAN_LINEAR && !a.state) ? (T)0 : factor * d;
+        }
     }
 }
 
@@ -536,42 +819,94 @@ template <class T> int32_t make_chain(rt_ctx* ctx, uint64_t tiles, uint64_t line
     return RT_OK;
 }
 
-constexpr int kWaves = 8, kBackWaves = 4;         // of a tile
+// A lane holds L steps in registers: two values a step forward, five backward.
+template <class T> constexpr int forward_steps() { return sizeof(T) == 4 ? 32 : 16; }
+template <class T> constexpr int backward_steps() { return sizeof(T) == 4 ? 16 : 8; }
+constexpr uint64_t kWideLeast = 32;             // inner: at least half of a wave's lanes have a column
 constexpr uint64_t kWideMost = 1ull << 22;      // inner: a wave's rows are addressed with 32-bit offsets; beyond it columns alone fill the card
-template <class T> int32_t forward_typed(rt_ctx* ctx, int form, const ScanArgs<T>& a) {
-    constexpr int L = sizeof(T) == 4 ? 32 : 16;
-    const uint64_t cols = a.outer * a.inner;
-    if (a.inner >= 32 && a.inner < kWideMost && a.steps > 8) {
-        const uint64_t cb = (a.inner + 63) / 64;
-        Chain ch;
-        RT_TRY(make_chain<T>(ctx, (a.steps + kWaves * L - 1) / (kWaves * L), a.outer * cb, &ch));
-        const dim3 grid(ch.rounds * ch.lines);
-        if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_wide_kernel<T, RT_SCAN_LINEAR, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
-        else hipLaunchKernelGGL((scan_wide_kernel<T, RT_SCAN_SIGMOID, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
+constexpr uint64_t kFewSteps = 8;               // steps that one lane a column goes through without help
+
+// One lane a column: few steps (a token), or so many columns that they fill the card.
+bool by_columns(uint64_t steps, uint64_t inner) { return steps <= kFewSteps || inner >= kWideMost; }
+
+template <class T, int W> int32_t make_narrow(rt_ctx* ctx, uint64_t outer, uint64_t steps, uint64_t inner, Chain* ch, Narrow* nw) {
+    nw->shift = 0;
+    while ((1ull << nw->shift) < inner) ++nw->shift;
+    const uint64_t segs = (uint64_t)(W * 64) >> nw->shift, most = segs * seg_steps<T>();       // steps of a tile
+    nw->rows = steps >= most ? 1 : most / steps;
+    if (nw->rows > outer) nw->rows = outer;
+    // fewer rows a line where there are too few lines to fill the card
+    const uint64_t lines_wanted = (uint64_t)ctx->num_cus * 2;
+    if (nw->rows > 1 && (outer + nw->rows - 1) / nw->rows < lines_wanted) nw->rows = (outer + lines_wanted - 1) / lines_wanted;
+    const uint64_t len = nw->rows * steps, tiles = (len + most - 1) / most;
+    const uint64_t per = (len + tiles - 1) / tiles;
+    nw->ls = (uint32_t)((per + segs - 1) / segs);
+    nw->by_inner = make_fastdiv((uint32_t)inner);
+    nw->by_steps = make_fastdiv(nw->rows > 1 ? (uint32_t)steps : 1u);
+    return make_chain<T>(ctx, (len + segs * nw->ls - 1) / (segs * nw->ls), (outer + nw->rows - 1) / nw->rows, ch);
+}
+
+// More than 64 KiB of LDS has to be asked for, once a device.
+int32_t allow_lds(rt_ctx* ctx, const void* kernel, size_t bytes, std::atomic<uint64_t>& allowed) {
+    const uint64_t bit = 1ull << (ctx->device & 63);
+    if ((allowed.load() & bit) && ctx->device < 64) return RT_OK;
+    RT_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    allowed.fetch_or(bit);
+    return RT_OK;
+}
+
+template <class T, int FORM> int32_t forward_form(rt_ctx* ctx, const ScanArgs<T>& a) {
+    constexpr int kWaves = 8, L = forward_steps<T>();
+    Chain ch;
+    if (by_columns(a.steps, a.inner)) {
+        hipLaunchKernelGGL((scan_columns_kernel<T, FORM>), dim3(blocks_of(a.outer * a.inner)), dim3(kSBlock), 0, ctx->stream, a);
+    } else if (a.inner < kWideLeast) {
+        Narrow nw;
+        RT_TRY((make_narrow<T, kWaves>(ctx, a.outer, a.steps, a.inner, &ch, &nw)));
+        auto kernel = scan_narrow_kernel<T, FORM, kWaves>;
+        static std::atomic<uint64_t> allowed{0};
+        RT_TRY(allow_lds(ctx, reinterpret_cast<const void*>(kernel), sizeof(Tile<T, kWaves>), allowed));
+        hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(kWaves * 64), sizeof(Tile<T, kWaves>), ctx->stream, a, ch, nw);
     } else {
-        if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_columns_kernel<T, RT_SCAN_LINEAR>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
-        else hipLaunchKernelGGL((scan_columns_kernel<T, RT_SCAN_SIGMOID>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
+        const uint64_t cb = (a.inner + 63) / 64;
+        const uint64_t tile = a.steps <= L ? L : kWaves * L;     // one wave's steps are a tile where they are enough
+        RT_TRY(make_chain<T>(ctx, (a.steps + tile - 1) / tile, a.outer * cb, &ch));
+        const dim3 grid(ch.rounds * ch.lines);
+        if (a.steps <= L) hipLaunchKernelGGL((scan_wide_kernel<T, FORM, 1, L>), grid, dim3(64), 0, ctx->stream, a, ch, (uint32_t)cb);
+        else hipLaunchKernelGGL((scan_wide_kernel<T, FORM, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
     }
     RT_HIP(hipGetLastError());
     return RT_OK;
 }
+template <class T> int32_t forward_typed(rt_ctx* ctx, int form, const ScanArgs<T>& a) {
+    return form == RT_SCAN_LINEAR ? forward_form<T, RT_SCAN_LINEAR>(ctx, a) : forward_form<T, RT_SCAN_SIGMOID>(ctx, a);
+}
 
-template <class T, class S> int32_t backward_typed(rt_ctx* ctx, int form, const BackArgs<T, S>& a) {
-    constexpr int L = sizeof(T) == 4 ? 16 : 8;
-    const uint64_t cols = a.outer * a.inner;
-    if (a.inner >= 32 && a.inner < kWideMost && a.steps > 8) {
-        const uint64_t cb = (a.inner + 63) / 64;
-        Chain ch;
-        RT_TRY(make_chain<T>(ctx, (a.steps + kBackWaves * L - 1) / (kBackWaves * L), a.outer * cb, &ch));
-        const dim3 grid(ch.rounds * ch.lines);
-        if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_backward_wide_kernel<T, RT_SCAN_LINEAR, S, kBackWaves, L>), grid, dim3(kBackWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
-        else hipLaunchKernelGGL((scan_backward_wide_kernel<T, RT_SCAN_SIGMOID, S, kBackWaves, L>), grid, dim3(kBackWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
+template <class T, int FORM, class S> int32_t backward_form(rt_ctx* ctx, const BackArgs<T, S>& a) {
+    constexpr int kWaves = 4, kNarrowWaves = 8, L = backward_steps<T>();
+    Chain ch;
+    if (by_columns(a.steps, a.inner)) {
+        hipLaunchKernelGGL((scan_backward_columns_kernel<T, FORM, S>), dim3(blocks_of(a.outer * a.inner)), dim3(kSBlock), 0, ctx->stream, a);
+    } else if (a.inner < kWideLeast) {
+        Narrow nw;
+        RT_TRY((make_narrow<T, kNarrowWaves>(ctx, a.outer, a.steps, a.inner, &ch, &nw)));
+        auto kernel = scan_backward_narrow_kernel<T, FORM, S, kNarrowWaves>;
+        static std::atomic<uint64_t> allowed{0};
+        RT_TRY(allow_lds(ctx, reinterpret_cast<const void*>(kernel), sizeof(Tile<T, kNarrowWaves>), allowed));
+        hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(kNarrowWaves * 64), sizeof(Tile<T, kNarrowWaves>), ctx->stream, a, ch, nw);
     } else {
-        if (form == RT_SCAN_LINEAR) hipLaunchKernelGGL((scan_backward_columns_kernel<T, RT_SCAN_LINEAR, S>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
-        else hipLaunchKernelGGL((scan_backward_columns_kernel<T, RT_SCAN_SIGMOID, S>), dim3(blocks_of(cols)), dim3(kSBlock), 0, ctx->stream, a);
+        const uint64_t cb = (a.inner + 63) / 64;
+        const uint64_t tile = a.steps <= L ? L : kWaves * L;
+        RT_TRY(make_chain<T>(ctx, (a.steps + tile - 1) / tile, a.outer * cb, &ch));
+        const dim3 grid(ch.rounds * ch.lines);
+        if (a.steps <= L) hipLaunchKernelGGL((scan_backward_wide_kernel<T, FORM, S, 1, L>), grid, dim3(64), 0, ctx->stream, a, ch, (uint32_t)cb);
+        else hipLaunchKernelGGL((scan_backward_wide_kernel<T, FORM, S, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
     }
     RT_HIP(hipGetLastError());
     return RT_OK;
+}
+template <class T, class S> int32_t backward_typed(rt_ctx* ctx, int form, const BackArgs<T, S>& a) {
+    return form == RT_SCAN_LINEAR ? backward_form<T, RT_SCAN_LINEAR, S>(ctx, a) : backward_form<T, RT_SCAN_SIGMOID, S>(ctx, a);
 }
 
 // ---- argument checks ---------------------------------------------------------------------------------------------------------------

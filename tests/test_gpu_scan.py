@@ -269,7 +269,7 @@ def test_two_contexts_at_once(hip):
     other.sync()
 
 
-@pytest.mark.parametrize("inner", [16384])
+@pytest.mark.parametrize("inner", [16384, 1])
 def test_offsets_beyond_32_bits(hip, inner):
     """More than 2^32 bytes and 2^31 elements: h of gate 0.5 and x 1 is 2 - 2^-t."""
     from rtensors_amd import hip as H
