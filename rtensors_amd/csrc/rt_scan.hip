@@ -312,7 +312,7 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W>& room, ui
             Slot<T>::put(slot, 0, th, epoch << 2 | kAgg);
         }
     }
-    if (k > 0) {
+    if (W > 1 && k > 0) {                                        // a tile of one wave is the only one of its line
         start = chain_start<T, W>(ch, room, item, k, w, lane);
         if (w == 0 && !last && !serial && !tcut) Slot<T>::put(slot, 0, fused(ta, start, th), epoch << 2 | kEnd);
     }
@@ -514,7 +514,7 @@ template <class T, int W> struct Tile {
     static constexpr uint32_t kLine = 64 / sizeof(T);            // one element of padding for each of these: a wave's segments start in
                                                                  // different banks
     static __device__ __forceinline__ uint32_t at(uint32_t e) { return e + e / kLine; }
-    T a[kMost + 64 + (kMost + 64) / kLine], b[kMost + kMost / kLine];
+    T a[kMost + 64 + (kMost + 64) / kLine], b[kMost + 64 + (kMost + 64) / kLine];    // lanes without a column read up to 62 further
     uint8_t reset[kMost + 1];
 };
 // What joins a wave's segments: the exclusive prefix of the lane's segment, and the wave's whole.
@@ -562,6 +562,15 @@ template <class T, class Go> __device__ __forceinline__ T run_lanes(const Prefix
     return __shfl(end, 64 - (1 << shift) + c);
 }
 
+// As RT_APART, of a lane's segment.
+#define RT_APART_LANES                          \
+    int rls = ls;                               \
+    uint32_t rcuts = cuts, rinner = inner;      \
+    uint32_t e = v0 * inner + c;                \
+    RT_PIN(rls);                                \
+    RT_PIN(rinner);                             \
+    asm volatile("" : "+v"(rcuts), "+v"(e))
+
 // Segment of a lane: a wave's lanes hold 64 >> shift consecutive ones.
 __device__ __forceinline__ int tile_segment(int tid, uint32_t shift) { return (tid >> 6) * (64 >> shift) + ((tid & 63) >> shift); }
 
@@ -580,11 +589,14 @@ __global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chai
     const uint64_t u0 = (uint64_t)k * segs * nw.ls;              // first step of the tile in the line
     const uint32_t cnt = len <= u0 ? 0 : (uint32_t)(len - u0 < (uint64_t)segs * nw.ls ? len - u0 : (uint64_t)segs * nw.ls), E = cnt * inner;
     const uint64_t step0 = row0 * a.steps + u0, base = step0 * inner;
+    const uint32_t all = segs * nw.ls * inner;                   // with the steps that are not there: they carry a state on as it is
     {
         T g[kSeg], x[kSeg];                                      // all loads before the first write
 #pragma unroll
         for (int q = 0; q < kSeg; ++q) {
             const uint32_t e = tid + q * kThreads;
+            g[q] = FORM == RT_SCAN_SIGMOID ? (T)__builtin_inf() : (T)1;
+            x[q] = (T)0;
             if (e < E) {
                 g[q] = __builtin_nontemporal_load(a.gate + base + e);
                 x[q] = __builtin_nontemporal_load(a.x + base + e);
@@ -593,57 +605,65 @@ __global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chai
 #pragma unroll
         for (int q = 0; q < kSeg; ++q) {
             const uint32_t e = tid + q * kThreads;
-            if (e < E) {
+            if (e < all) {
                 tile.a[TT::at(e)] = g[q];
                 tile.b[TT::at(e)] = x[q];
             }
         }
     }
     if (a.reset)
-        for (uint32_t e = tid; e < cnt; e += kThreads) tile.reset[e] = a.reset[step0 + e];
+        for (uint32_t e = tid; e < segs * nw.ls; e += kThreads) tile.reset[e] = e < cnt ? a.reset[step0 + e] : (uint8_t)0;
     __syncthreads();
     const uint32_t c = lane & ((1u << nw.shift) - 1), v0 = (uint32_t)tile_segment(tid, nw.shift) * nw.ls;
-    const int n = c >= inner || v0 >= cnt ? 0 : (int)(cnt - v0 < nw.ls ? cnt - v0 : nw.ls);
-    // the row of the segment's first step and the step's place in it
-    const uint64_t row_of = nw.rows == 1 ? 0 : fd_div((uint32_t)u0 + v0, nw.by_steps);
-    const uint64_t rem0 = u0 + v0 - row_of * a.steps;
+    const bool own = c < inner;
+    const int ls = (int)nw.ls;
+    // the row of the segment's first step and the step's place in it; bit j of `heads`: step j is the first of its row
+    const uint64_t row_of = nw.rows == 1 ? 0 : fd_div((uint32_t)u0 + v0, nw.by_steps), rem0 = u0 + v0 - row_of * a.steps;
+    const uint32_t steps = a.steps < 64 ? (uint32_t)a.steps : 64u;       // all that a segment can tell
+    uint32_t next = rem0 == 0 ? 0u : a.steps - rem0 < 64 ? (uint32_t)(a.steps - rem0) : 64u;
+    uint32_t heads = 0, cuts = 0;
+    for (; next < (uint32_t)kSeg; next += steps) heads |= 1u << next;
+    if (v0 < cnt) heads &= cnt - v0 < (uint32_t)kSeg ? (1u << (cnt - v0)) - 1 : ~0u;
+    else heads = 0;
+    if (a.reset)
+        for (int j = 0; j < ls; ++j) cuts |= (tile.reset[v0 + j] ? 1u : 0u) << j;
+    const uint32_t states = a.state && own ? heads & ~cuts : 0u; // steps that begin from a given state
+    cuts |= heads;
+    const uint64_t place = (row0 + row_of) * inner + c;          // in (outer, inner), of the segment's first row
     T f[kSeg], b[kSeg], A = (T)1, H = (T)0;
-    uint32_t cuts = 0;
     {
-        uint64_t rem = rem0, row = row0 + row_of;
+        uint32_t e = v0 * inner + c;
 #pragma unroll
         for (int j = 0; j < kSeg; ++j) {
-            if (j < n) {
-                const uint32_t e = TT::at((v0 + j) * inner + c);
-                f[j] = tile.a[e];
-                b[j] = tile.b[e];
+            if (j < ls) {
+                f[j] = tile.a[TT::at(e)];
+                b[j] = tile.b[TT::at(e)];
+                e += inner;
                 if constexpr (FORM == RT_SCAN_SIGMOID) {
                     const RtGate<T> q = gate_of(f[j]);
                     f[j] = q.s;
                     b[j] = q.r * b[j];
                 }
-                const bool head = rem == 0, reset = a.reset && tile.reset[v0 + j];
-                if (head && a.state && !reset) b[j] = fused(f[j], a.state[row * inner + c], b[j]);
-                if (head || reset) cuts |= 1u << j;
+                if (states >> j & 1)                             // rows on from the first: heads up to here, the one at 0 being the first's own
+                    b[j] = fused(f[j], a.state[place + (uint64_t)__popc(heads & ((2u << j) - 1u) & ~1u) * inner], b[j]);
                 H = j == 0 || (cuts >> j & 1) ? b[j] : fused(f[j], H, b[j]);
-                A = cuts ? (T)0 : A * f[j];
-                if (++rem == a.steps) { rem = 0; ++row; }
+                A *= f[j];
             }
         }
+        if (cuts) A = (T)0;
+        if (!own) { A = (T)1; H = (T)0; cuts = 0; }
     }
     const Prefix<T> pre = join_lanes(A, H, cuts != 0, lane, nw.shift);
     join_tile<T, W>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
         return run_lanes(pre, start, serial, lane, nw.shift, [&](T p) {
-            uint64_t rem = rem0, row = row0 + row_of;
+            RT_APART_LANES;
+            if (own) {
 #pragma unroll
-            for (int j = 0; j < kSeg; ++j) {
-                if (j < n) {
-                    p = cuts >> j & 1 ? b[j] : fused(f[j], p, b[j]);
-                    tile.b[TT::at((v0 + j) * inner + c)] = p;
-                    if (++rem == a.steps) {
-                        if (a.last) a.last[row * inner + c] = p;
-                        rem = 0;
-                        ++row;
+                for (int j = 0; j < kSeg; ++j) {
+                    if (j < rls) {
+                        p = rcuts >> j & 1 ? b[j] : fused(f[j], p, b[j]);
+                        tile.b[TT::at(e)] = p;
+                        e += rinner;
                     }
                 }
             }
@@ -651,7 +671,18 @@ __global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chai
         });
     });
     __syncthreads();
-    for (uint32_t e = tid; e < E; e += kThreads) __builtin_nontemporal_store(tile.b[TT::at(e)], a.h + base + e);
+#pragma unroll
+    for (int q = 0; q < kSeg; ++q) {
+        const uint32_t e = tid + q * kThreads;
+        if (e < E) __builtin_nontemporal_store(tile.b[TT::at(e)], a.h + base + e);
+    }
+    if (a.last && u0 + cnt == len) {                             // the end of a line's rows: all of them, or the one whose last tile this is
+        const uint32_t ends = nw.rows == 1 ? inner : (uint32_t)rows * inner, stretch = nw.rows == 1 ? cnt : (uint32_t)a.steps;
+        for (uint32_t q = tid; q < ends; q += kThreads) {
+            const uint32_t r = fd_div(q, nw.by_inner);
+            a.last[row0 * inner + q] = tile.b[TT::at(((r + 1) * stretch - 1) * inner + (q - r * inner))];
+        }
+    }
 }
 
 // Backward: the segments go through the tile from its end.  Only D comes out of the recurrence; the gradients are formed from it element
@@ -673,72 +704,89 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
     const uint64_t lo = len - r0 - cnt;                          // first step of the tile in the line
     const uint64_t step0 = row0 * a.steps + lo, base = step0 * inner;
     const uint32_t behind = r0 ? inner : 0;                      // the gates of one step more
+    // The steps that are not there (they carry a gradient on as it is) lie before the others: step v of the tile is at v + off.
+    const uint32_t off = segs * nw.ls - cnt, eoff = off * inner;
     {
         T g[kSeg], d[kSeg];                                      // all loads before the first write
 #pragma unroll
         for (int q = 0; q < kSeg; ++q) {
             const uint32_t e = tid + q * kThreads;
-            if (e < E) {
-                g[q] = a.gate[base + e];
-                d[q] = __builtin_nontemporal_load(a.dh + base + e);
+            g[q] = FORM == RT_SCAN_SIGMOID ? (T)__builtin_inf() : (T)1;
+            d[q] = (T)0;
+            if (e >= eoff && e < eoff + E) {
+                g[q] = a.gate[base + (e - eoff)];
+                d[q] = __builtin_nontemporal_load(a.dh + base + (e - eoff));
             }
         }
-        if ((uint32_t)tid < behind) tile.a[TT::at(E + tid)] = a.gate[base + E + tid];
+        if ((uint32_t)tid < inner) tile.a[TT::at(eoff + E + tid)] = (uint32_t)tid < behind ? a.gate[base + E + tid] : (T)0;
 #pragma unroll
         for (int q = 0; q < kSeg; ++q) {
             const uint32_t e = tid + q * kThreads;
-            if (e < E) {
+            if (e < eoff + E) {
                 tile.a[TT::at(e)] = g[q];
                 tile.b[TT::at(e)] = d[q];
             }
         }
     }
     if (a.reset)
-        for (uint32_t e = tid; e < cnt + (r0 ? 1 : 0); e += kThreads) tile.reset[e] = a.reset[step0 + e];
+        for (uint32_t e = tid; e <= segs * nw.ls; e += kThreads)
+            tile.reset[e] = e >= off && e < off + cnt + (r0 ? 1 : 0) ? a.reset[step0 + (e - off)] : (uint8_t)0;
     __syncthreads();
     const uint32_t c = lane & ((1u << nw.shift) - 1), q0 = (uint32_t)tile_segment(tid, nw.shift) * nw.ls;
-    const int n = c >= inner || q0 >= cnt ? 0 : (int)(cnt - q0 < nw.ls ? cnt - q0 : nw.ls);
-    const uint32_t v0 = n ? cnt - 1 - q0 : 0;                    // the segment's last step in the tile; it goes down from there
-    const uint64_t row_of = nw.rows == 1 ? 0 : fd_div((uint32_t)lo + v0, nw.by_steps);
+    const bool own = c < inner;
+    const int ls = (int)nw.ls;
+    const uint32_t v0 = segs * nw.ls - 1 - q0;                   // place of the segment's last step; it goes down from there
+    // bit j of `tails`: the step j before the segment's last is the last of its row
+    const uint64_t u_last = q0 < cnt ? lo + (cnt - 1 - q0) : 0;
+    const uint64_t row_of = nw.rows == 1 ? 0 : fd_div((uint32_t)u_last, nw.by_steps), t_last = u_last - row_of * a.steps;
+    const uint32_t steps = a.steps < 64 ? (uint32_t)a.steps : 64u;
+    uint32_t next = t_last + 1 == a.steps ? 0u : t_last + 1 < 64 ? (uint32_t)t_last + 1 : 64u;
+    uint32_t tails = 0, cuts = 0;
+    for (; next < (uint32_t)kSeg; next += steps) tails |= 1u << next;
+    if (q0 < cnt) tails &= cnt - q0 < (uint32_t)kSeg ? (1u << (cnt - q0)) - 1 : ~0u;
+    else tails = 0;
+    if (a.reset)                                                 // a reset of the step behind
+        for (int j = 0; j < ls; ++j) cuts |= (tile.reset[v0 - j + 1] ? 1u : 0u) << j;
+    cuts |= tails;
+    const uint32_t lasts = a.dlast && own ? tails : 0u;
+    const uint64_t place = (row0 + row_of) * inner + c;          // in (outer, inner), of the segment's last row
     T f[kSeg], b[kSeg], A = (T)1, H = (T)0;
-    uint32_t cuts = 0;
     {
-        uint64_t t = lo + v0 - row_of * a.steps, row = row0 + row_of;
+        uint32_t e = v0 * inner + c;
 #pragma unroll
         for (int j = 0; j < kSeg; ++j) {
-            if (j < n) {
-                const uint32_t v = v0 - j;
-                b[j] = tile.b[TT::at(v * inner + c)];
-                f[j] = (T)0;
-                const bool tail = t == a.steps - 1;
-                if (tail) {
-                    if (a.dlast) b[j] += a.dlast[row * inner + c];
-                } else {
-                    f[j] = tile.a[TT::at((v + 1) * inner + c)];
-                    if constexpr (FORM == RT_SCAN_SIGMOID) f[j] = gate_of(f[j]).s;
-                }
-                if (tail || (a.reset && tile.reset[v + 1])) cuts |= 1u << j;
+            if (j < ls) {
+                b[j] = tile.b[TT::at(e)];
+                f[j] = tile.a[TT::at(e + inner)];
+                e -= inner;
+                if constexpr (FORM == RT_SCAN_SIGMOID) f[j] = gate_of(f[j]).s;
+                if (lasts >> j & 1) b[j] += a.dlast[place - (uint64_t)__popc(tails & ((2u << j) - 1u) & ~1u) * inner];
                 H = j == 0 || (cuts >> j & 1) ? b[j] : fused(f[j], H, b[j]);
-                A = cuts ? (T)0 : A * f[j];
-                if (t == 0) { t = a.steps; --row; }
-                --t;
+                A *= f[j];
             }
         }
+        if (cuts) A = (T)0;
+        if (!own) { A = (T)1; H = (T)0; cuts = 0; }
     }
     const Prefix<T> pre = join_lanes(A, H, cuts != 0, lane, nw.shift);
     join_tile<T, W>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
         return run_lanes(pre, start, serial, lane, nw.shift, [&](T d) {
+            RT_APART_LANES;
+            if (own) {
 #pragma unroll
-            for (int j = 0; j < kSeg; ++j) {
-                if (j < n) {
-                    d = cuts >> j & 1 ? b[j] : fused(f[j], d, b[j]);
-                    tile.b[TT::at((v0 - j) * inner + c)] = d;
+                for (int j = 0; j < kSeg; ++j) {
+                    if (j < rls) {
+                        d = rcuts >> j & 1 ? b[j] : fused(f[j], d, b[j]);
+                        tile.b[TT::at(e)] = d;
+                        e -= rinner;
+                    }
                 }
             }
             return d;
         });
     });
     __syncthreads();
+    const uint32_t head1 = lo == 0 ? 0u : ~0u;                   // the step that begins a row, of a line of one row
     constexpr int kBatch = 4;                                    // elements whose h and x are on their way at once
     for (uint32_t e0 = tid; e0 < E; e0 += kThreads * kBatch) {
         T p[kBatch], x[kBatch];
@@ -747,10 +795,9 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
 #pragma unroll
         for (int q = 0; q < kBatch; ++q) {
             const uint32_t e = e0 + q * kThreads < E ? e0 + q * kThreads : e0, v = fd_div(e, nw.by_inner);
-            const uint64_t u = lo + v;
-            const uint64_t row = nw.rows == 1 ? 0 : fd_div((uint32_t)u, nw.by_steps);
-            head[q] = u == row * a.steps;
-            reset[q] = a.reset && tile.reset[v];
+            const uint32_t row = nw.rows == 1 ? 0u : fd_div((uint32_t)lo + v, nw.by_steps);
+            head[q] = nw.rows == 1 ? v == head1 : (uint32_t)lo + v == row * (uint32_t)a.steps;
+            reset[q] = a.reset && tile.reset[v + off];
             sc[q] = (row0 + row) * inner + (e - v * inner);
             p[q] = (T)0;
             if (!head[q]) p[q] = a.h.at(base - inner, e);
@@ -761,7 +808,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
         for (int q = 0; q < kBatch; ++q) {
             const uint32_t e = e0 + q * kThreads;
             if (e >= E) continue;
-            const T d = tile.b[TT::at(e)], g = tile.a[TT::at(e)], before = reset[q] ? (T)0 : p[q];
+            const T d = tile.b[TT::at(e + eoff)], g = tile.a[TT::at(e + eoff)], before = reset[q] ? (T)0 : p[q];
             T factor = g;
             if constexpr (FORM == RT_SCAN_LINEAR) {
                 __builtin_nontemporal_store(reset[q] || (head[q] && !a.state) ? (T)0 : d * before, a.dgate + base + e);
