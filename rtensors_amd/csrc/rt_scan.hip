@@ -2,6 +2,8 @@
 #include "rt_pack8.h"
 #include "rt_unary_math.h"
 
+#include <stddef.h>
+
 #include <atomic>
 
 namespace {
@@ -117,7 +119,6 @@ struct Chain {
 };
 constexpr uint32_t kTicketPitch = 16;
 constexpr uint32_t kAgg = 1, kEnd = 2;                           // what a slot holds: (A, H), or the end state in place of H
-constexpr int kWindowF32 = 16, kWindowF64 = 8;                  // tiles before its own that a tile looks at
 
 __device__ __forceinline__ void put_word(uint64_t* p, uint32_t bits, uint32_t tag) {
     __hip_atomic_store(p, (uint64_t)tag << 32 | bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -182,10 +183,12 @@ __device__ __forceinline__ double fused(double a, double b, double c) { return _
 __device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
 __device__ __forceinline__ bool finite(double v) { return __builtin_fabs(v) < __builtin_inf(); }
 
-template <class T, int W> struct JoinRoom {
-    static constexpr int kWindow = sizeof(T) == 4 ? kWindowF32 : kWindowF64;
-    T A[W][64], H[W][64], start[64];
-    T winA[kWindow][64], winH[kWindow][64];
+// LN: lanes that hold different columns; with 32 the upper half of a wave repeats the lower one.
+template <class T, int W, int LN> struct JoinRoom {
+    // tiles before its own that a tile looks at (with f64 tiles staged through LDS: as many as leave room for two blocks a CU)
+    static constexpr int kWindow = sizeof(T) == 4 ? 16 : LN == 32 ? 4 : 8;
+    T A[W][LN], H[W][LN], start[LN];
+    T winA[kWindow][LN], winH[kWindow][LN];
     uint64_t ends[kWindow];
     uint32_t cut[W];
     uint32_t tile;
@@ -195,8 +198,8 @@ template <class T, int W> struct JoinRoom {
 // The end state of tile k - 1 for this lane's column, for all waves of the block.  Waiting is done by one wave on one word of each of the
 // tiles in the window, read by one lane each: polling whole slots takes the bandwidth that the tiles being waited for need.  Then the
 // waves read the slots between them, again where not all of their words are there yet, and go through them from the farthest.
-template <class T, int W> __device__ __forceinline__ T chain_start(const Chain& ch, JoinRoom<T, W>& room, uint32_t item, uint32_t k, int w, int lane) {
-    constexpr int kWindow = JoinRoom<T, W>::kWindow, kEach = (kWindow + W - 1) / W;
+template <class T, int W, int LN> __device__ __forceinline__ T chain_start(const Chain& ch, JoinRoom<T, W, LN>& room, uint32_t item, uint32_t k, int w, int lane) {
+    constexpr int kWindow = JoinRoom<T, W, LN>::kWindow, kEach = (kWindow + W - 1) / W;
     if (w == 0) {
         const int n = k < (uint32_t)kWindow ? (int)k : kWindow;
         int found;                                               // nearest tile with an end state, all nearer ones having (A, H)
@@ -234,14 +237,14 @@ template <class T, int W> __device__ __forceinline__ T chain_start(const Chain& 
         if (q <= found) {
             // an end state may have taken the place of a nearer tile's (A, H) meanwhile
             const uint64_t ends = __ballot(s[i].kind(ch.epoch) == kEnd);
-            room.winH[q][lane] = s[i].value(0);
-            room.winA[q][lane] = s[i].value(1);
+            room.winH[q][lane & (LN - 1)] = s[i].value(0);
+            room.winA[q][lane & (LN - 1)] = s[i].value(1);
             if (lane == 0) room.ends[q] = ends;
         }
     }
     __syncthreads();
     T c = (T)0;
-    for (int q = found; q >= 0; --q) c = room.ends[q] >> lane & 1 ? room.winH[q][lane] : fused(room.winA[q][lane], c, room.winH[q][lane]);
+    for (int q = found; q >= 0; --q) c = room.ends[q] >> lane & 1 ? room.winH[q][lane & (LN - 1)] : fused(room.winA[q][lane & (LN - 1)], c, room.winH[q][lane & (LN - 1)]);
     return c;
 }
 
@@ -255,7 +258,7 @@ __device__ __forceinline__ uint32_t line_of_block(const Chain& ch) {
     return (b / 8 + (uint32_t)((uint64_t)x * ch.lines / 8)) % ch.lines;
 }
 // The block's tile among those of its line (one that is not there for the blocks too many); whoever takes the last one leaves the counter as the next launch needs it.
-template <class T, int W> __device__ __forceinline__ uint32_t take_tile(const Chain& ch, uint32_t line, JoinRoom<T, W>& room) {
+template <class T, int W, int LN> __device__ __forceinline__ uint32_t take_tile(const Chain& ch, uint32_t line, JoinRoom<T, W, LN>& room) {
     if (ch.tiles == 1) return 0;
     if (threadIdx.x == 0) {
         uint32_t* c = ch.tickets + (uint64_t)line * kTicketPitch;
@@ -274,12 +277,12 @@ template <class T, int W> __device__ __forceinline__ uint32_t take_tile(const Ch
 //
 // A product of factors above 1 can leave the range while the states stay inside it (a start of zero, say).  Where one does, the tile's
 // stretches run one after the other and only its end state is published: the plain loop's result, at the plain loop's pace.
-template <class T, int W, class Run>
-__device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W>& room, uint32_t item, uint32_t k, T A, T H, bool cut, bool odd, T first, Run run) {
+template <class T, int W, int LN, class Run>
+__device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN>& room, uint32_t item, uint32_t k, T A, T H, bool cut, bool odd, T first, Run run) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const bool last = k == ch.tiles - 1;
-    room.A[w][lane] = A;
-    room.H[w][lane] = H;
+    room.A[w][lane & (LN - 1)] = A;
+    room.H[w][lane & (LN - 1)] = H;
     if (lane == 0) room.cut[w] = (cut ? 1u : 0u) | (odd ? 2u : 0u);
     __syncthreads();
     const uint32_t epoch = ch.epoch;
@@ -287,7 +290,7 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W>& room, ui
     bool tcut = false, bad = false;
 #pragma unroll
     for (int v = 0; v < W; ++v) {
-        const T av = room.A[v][lane], hv = room.H[v][lane];
+        const T av = room.A[v][lane & (LN - 1)], hv = room.H[v][lane & (LN - 1)];
         bad = bad || (room.cut[v] & 2u);
         if (room.cut[v] & 1u) {
             th = hv;
@@ -313,26 +316,26 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W>& room, ui
         }
     }
     if (W > 1 && k > 0) {                                        // a tile of one wave is the only one of its line
-        start = chain_start<T, W>(ch, room, item, k, w, lane);
+        start = chain_start(ch, room, item, k, w, lane);
         if (w == 0 && !last && !serial && !tcut) Slot<T>::put(slot, 0, fused(ta, start, th), epoch << 2 | kEnd);
     }
     if (serial) {
-        if (w == 0) room.start[lane] = start;
+        if (w == 0) room.start[lane & (LN - 1)] = start;
         __syncthreads();
     }
     T end = (T)0;
     for (int turn = 0; turn < (serial ? W : 1); ++turn) {
         if (!serial || turn == w) {
-            if (serial) start = room.start[lane];
+            if (serial) start = room.start[lane & (LN - 1)];
             else {
-                for (int v = 0; v < w; ++v) start = room.cut[v] & 1u ? room.H[v][lane] : fused(room.A[v][lane], start, room.H[v][lane]);
+                for (int v = 0; v < w; ++v) start = room.cut[v] & 1u ? room.H[v][lane & (LN - 1)] : fused(room.A[v][lane & (LN - 1)], start, room.H[v][lane & (LN - 1)]);
             }
             end = run(start, serial);
-            if (serial) room.start[lane] = end;
+            if (serial) room.start[lane & (LN - 1)] = end;
         }
         if (serial) __syncthreads();
     }
-    if (serial && w == 0 && !last) Slot<T>::put(slot, 0, room.start[lane], epoch << 2 | kEnd);
+    if (serial && w == 0 && !last) Slot<T>::put(slot, 0, room.start[lane & (LN - 1)], epoch << 2 | kEnd);
     return end;
 }
 
@@ -355,8 +358,8 @@ __device__ __forceinline__ uint64_t reset_bits(const uint8_t* flags, int64_t str
 // the last step and the last column hold, and neither use nor store it.
 template <class T, int FORM, int W, int L>
 __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain ch, uint32_t col_blocks) {
-    __shared__ JoinRoom<T, W> room;
-    const uint32_t line = line_of_block(ch), k = take_tile<T, W>(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
+    __shared__ JoinRoom<T, W, 64> room;
+    const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
     if (k >= ch.tiles) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t row = (uint32_t)a.inner, col0 = (line - o * col_blocks) * 64, col = col0 + lane;
@@ -392,7 +395,7 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
     }
     const T first = k == 0 && a.state ? a.state[sc] : (T)0;
     T* h = a.h + base;
-    const T end = join_tile<T, W>(ch, room, item, k, A, H, cuts != 0, false, first, [&](T p, bool) {
+    const T end = join_tile(ch, room, item, k, A, H, cuts != 0, false, first, [&](T p, bool) {
         RT_APART;
         if (in) {
 #pragma unroll
@@ -412,8 +415,8 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
 // that one's gate.
 template <class T, int FORM, class S, int W, int L>
 __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, S> a, Chain ch, uint32_t col_blocks) {
-    __shared__ JoinRoom<T, W> room;
-    const uint32_t line = line_of_block(ch), k = take_tile<T, W>(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
+    __shared__ JoinRoom<T, W, 64> room;
+    const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
     if (k >= ch.tiles) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t row = (uint32_t)a.inner, col0 = (line - o * col_blocks) * 64, col = col0 + lane;
@@ -466,7 +469,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
     }
     const T first = k == 0 && a.dlast ? a.dlast[sc] : (T)0;
     T *dg = a.dgate + base, *dx = a.dx + base;
-    const T end = join_tile<T, W>(ch, room, item, k, A, H, cuts != 0, false, first, [&](T d, bool) {
+    const T end = join_tile(ch, room, item, k, A, H, cuts != 0, false, first, [&](T d, bool) {
         RT_APART;
         uint64_t rresets = resets;
         RT_PIN(rresets);
@@ -515,8 +518,16 @@ template <class T, int W> struct Tile {
                                                                  // different banks
     static __device__ __forceinline__ uint32_t at(uint32_t e) { return e + e / kLine; }
     T a[kMost + 64 + (kMost + 64) / kLine], b[kMost + 64 + (kMost + 64) / kLine];    // lanes without a column read up to 62 further
-    uint8_t reset[kMost + 1];
+    uint8_t reset[1];                                            // one byte a step and one more, where there are resets
 };
+template <class T, int W> size_t tile_bytes(const Narrow& nw, bool reset) {
+    typedef Tile<T, W> TT;
+    return offsetof(TT, reset) + (reset ? ((size_t)(W * 64) >> nw.shift) * nw.ls + 1 : 0);
+}
+template <class T, int W> constexpr size_t most_tile_bytes() {
+    typedef Tile<T, W> TT;
+    return offsetof(TT, reset) + TT::kMost + 1;
+}
 // What joins a wave's segments: the exclusive prefix of the lane's segment, and the wave's whole.
 template <class T> struct Prefix {
     T A, H, wholeA, wholeH;
@@ -577,11 +588,11 @@ __device__ __forceinline__ int tile_segment(int tid, uint32_t shift) { return (t
 template <class T, int FORM, int W>
 __global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chain ch, Narrow nw) {
     constexpr int kSeg = seg_steps<T>(), kThreads = W * 64;
-    __shared__ JoinRoom<T, W> room;
+    __shared__ JoinRoom<T, W, 32> room;                          // inner is below 32
     extern __shared__ __align__(16) char lds[];
     Tile<T, W>& tile = *reinterpret_cast<Tile<T, W>*>(lds);
     typedef Tile<T, W> TT;
-    const uint32_t line = line_of_block(ch), k = take_tile<T, W>(ch, line, room), item = k * ch.lines + line;
+    const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line;
     if (k >= ch.tiles) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t inner = (uint32_t)a.inner, segs = kThreads >> nw.shift;
@@ -654,7 +665,7 @@ __global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chai
         if (!own) { A = (T)1; H = (T)0; cuts = 0; }
     }
     const Prefix<T> pre = join_lanes(A, H, cuts != 0, lane, nw.shift);
-    join_tile<T, W>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
+    join_tile(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
         return run_lanes(pre, start, serial, lane, nw.shift, [&](T p) {
             RT_APART_LANES;
             if (own) {
@@ -690,11 +701,11 @@ __global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chai
 template <class T, int FORM, class S, int W>
 __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T, S> a, Chain ch, Narrow nw) {
     constexpr int kSeg = seg_steps<T>(), kThreads = W * 64;
-    __shared__ JoinRoom<T, W> room;
+    __shared__ JoinRoom<T, W, 32> room;                          // inner is below 32
     extern __shared__ __align__(16) char lds[];
     Tile<T, W>& tile = *reinterpret_cast<Tile<T, W>*>(lds);
     typedef Tile<T, W> TT;
-    const uint32_t line = line_of_block(ch), k = take_tile<T, W>(ch, line, room), item = k * ch.lines + line;
+    const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line;
     if (k >= ch.tiles) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t inner = (uint32_t)a.inner, segs = kThreads >> nw.shift;
@@ -769,7 +780,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
         if (!own) { A = (T)1; H = (T)0; cuts = 0; }
     }
     const Prefix<T> pre = join_lanes(A, H, cuts != 0, lane, nw.shift);
-    join_tile<T, W>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
+    join_tile(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
         return run_lanes(pre, start, serial, lane, nw.shift, [&](T d) {
             RT_APART_LANES;
             if (own) {
@@ -912,8 +923,9 @@ template <class T, int FORM> int32_t forward_form(rt_ctx* ctx, const ScanArgs<T>
         RT_TRY((make_narrow<T, kWaves>(ctx, a.outer, a.steps, a.inner, &ch, &nw)));
         auto kernel = scan_narrow_kernel<T, FORM, kWaves>;
         static std::atomic<uint64_t> allowed{0};
-        RT_TRY(allow_lds(ctx, reinterpret_cast<const void*>(kernel), sizeof(Tile<T, kWaves>), allowed));
-        hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(kWaves * 64), sizeof(Tile<T, kWaves>), ctx->stream, a, ch, nw);
+        RT_TRY((allow_lds(ctx, reinterpret_cast<const void*>(kernel), most_tile_bytes<T, kWaves>(), allowed)));
+        const size_t bytes = tile_bytes<T, kWaves>(nw, a.reset != nullptr);
+        hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(kWaves * 64), bytes, ctx->stream, a, ch, nw);
     } else {
         const uint64_t cb = (a.inner + 63) / 64;
         const uint64_t tile = a.steps <= L ? L : kWaves * L;     // one wave's steps are a tile where they are enough
@@ -939,8 +951,9 @@ template <class T, int FORM, class S> int32_t backward_form(rt_ctx* ctx, const B
         RT_TRY((make_narrow<T, kNarrowWaves>(ctx, a.outer, a.steps, a.inner, &ch, &nw)));
         auto kernel = scan_backward_narrow_kernel<T, FORM, S, kNarrowWaves>;
         static std::atomic<uint64_t> allowed{0};
-        RT_TRY(allow_lds(ctx, reinterpret_cast<const void*>(kernel), sizeof(Tile<T, kNarrowWaves>), allowed));
-        hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(kNarrowWaves * 64), sizeof(Tile<T, kNarrowWaves>), ctx->stream, a, ch, nw);
+        RT_TRY((allow_lds(ctx, reinterpret_cast<const void*>(kernel), most_tile_bytes<T, kNarrowWaves>(), allowed)));
+        const size_t bytes = tile_bytes<T, kNarrowWaves>(nw, a.reset != nullptr);
+        hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(kNarrowWaves * 64), bytes, ctx->stream, a, ch, nw);
     } else {
         const uint64_t cb = (a.inner + 63) / 64;
         const uint64_t tile = a.steps <= L ? L : kWaves * L;
