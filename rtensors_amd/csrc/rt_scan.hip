@@ -10,16 +10,26 @@ namespace {
 
 constexpr int kSBlock = 256;
 
+// A load that is marked as touched once -- where the wave's stretch is a whole number of cache lines.  Rows that are no multiple of a line
+// share lines between neighbouring columns' waves, and a line that is dropped after the first is fetched again: (1, 50000, 1111) f32
+// forward 179 us with the mark, 158 us without; (1, 65536, 4096) 549 us with it, 558 us without.
+template <bool ONCE, class T> __device__ __forceinline__ T once(const T* p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+
 // x and h of the backward pass: whole values or the 8-bit form
 template <class T> struct Whole {
+    static constexpr bool kHeld = false;
     const T* p;
     // element i of the run that starts at `base` (wave-uniform; base + i does not leave the run, base alone may)
-    __device__ __forceinline__ T at(uint64_t base, uint32_t i) const { return __builtin_nontemporal_load(p + base + i); }
+    template <bool ONCE = true> __device__ __forceinline__ T at(uint64_t base, uint32_t i) const { return once<ONCE>(p + base + i); }
 };
 template <class T> struct Held {
+    static constexpr bool kHeld = true;
     const int8_t* codes;
     const uint8_t* exps;
-    __device__ __forceinline__ T at(uint64_t base, uint32_t i) const {
+    template <bool ONCE = true> __device__ __forceinline__ T at(uint64_t base, uint32_t i) const {
         const uint64_t e = base + i;
         return p8_value<T>(codes[e], exps[e / kP8Group]);
     }
@@ -186,7 +196,7 @@ __device__ __forceinline__ bool finite(double v) { return __builtin_fabs(v) < __
 // LN: lanes that hold different columns; with 32 the upper half of a wave repeats the lower one.
 template <class T, int W, int LN> struct JoinRoom {
     // tiles before its own that a tile looks at (with f64 tiles staged through LDS: as many as leave room for two blocks a CU)
-    static constexpr int kWindow = sizeof(T) == 4 ? 16 : LN == 32 ? 4 : 8;
+    static constexpr int kWindow = W == 1 ? 1 : sizeof(T) == 4 ? 16 : LN == 32 ? 4 : 8;
     T A[W][LN], H[W][LN], start[LN];
     T winA[kWindow][LN], winH[kWindow][LN];
     uint64_t ends[kWindow];
@@ -356,7 +366,7 @@ __device__ __forceinline__ uint64_t reset_bits(const uint8_t* flags, int64_t str
 
 // W waves of 64 columns, L steps each, in registers.  A wave that ends before its L steps, and lanes behind the last column, load what
 // the last step and the last column hold, and neither use nor store it.
-template <class T, int FORM, int W, int L>
+template <class T, int FORM, int W, int L, bool ALIGNED>
 __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain ch, uint32_t col_blocks) {
     __shared__ JoinRoom<T, W, 64> room;
     const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
@@ -376,8 +386,8 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
 #pragma unroll
         for (int j = 0; j < L; ++j) {
             const uint32_t at = lc + (uint32_t)(j < n ? j : n - 1) * row;
-            f[j] = __builtin_nontemporal_load(gate + at);
-            b[j] = __builtin_nontemporal_load(x + at);
+            f[j] = once<ALIGNED>(gate + at);
+            b[j] = once<ALIGNED>(x + at);
         }
         if (a.reset) cuts |= reset_bits(a.reset + (uint64_t)o * a.steps + t0, 1, n, lane);
 #pragma unroll
@@ -411,11 +421,52 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
     if (a.last && in && n && t0 + n == a.steps) a.last[sc] = end;
 }
 
+// What a wave's L rows of 64 columns of a tensor in the 8-bit form take in LDS: the codes, and of each row the exponent bytes of the (at
+// most three) groups that its 64 columns lie in.  Four lanes a row load 16 codes and one exponent byte each, so the rows of a wave come
+// with two loads instead of two a step, and hold no registers until they are used.
+struct HeldRegs {
+    rt_u32x4 codes;
+    uint32_t exp;
+};
+template <int L> struct HeldRows {
+    alignas(16) uint8_t codes[L][64];
+    uint8_t exps[L][4];
+    // rows begin at `first + r * row` (wave-uniform; r from `skip` to n - 1); `total` elements in all
+    template <class T> static __device__ __forceinline__ HeldRegs load(const Held<T>& h, uint64_t first, uint32_t row, int n, int skip, uint64_t total, int lane) {
+        HeldRegs v = {{0u, 0u, 0u, 0u}, 0u};
+        const int r = lane >> 2, c = lane & 3;
+        if (r >= skip && r < n) {
+            const uint64_t start = first + (uint64_t)((uint32_t)r * row), at = start + c * 16, g = start / kP8Group + c;
+            if (at + 16 <= total) v.codes = rt_ld16u<int8_t, false>(h.codes + at);
+            else
+                for (int b = 0; b < 16; ++b)                     // the last rows of the tensor
+                    if (at + b < total) v.codes[b >> 2] |= (uint32_t)(uint8_t)h.codes[at + b] << (8 * (b & 3));
+            if (g * kP8Group < total) v.exp = h.exps[g];
+        }
+        return v;
+    }
+    __device__ __forceinline__ void put(const HeldRegs& v, int lane) {
+        const int r = lane >> 2, c = lane & 3;
+        if (r < L) {
+            *reinterpret_cast<rt_u32x4*>(&codes[r][c * 16]) = v.codes;
+            exps[r][c] = (uint8_t)v.exp;
+        }
+    }
+    // element `lane` of row r, which begins at `start` (wave-uniform)
+    template <class T> __device__ __forceinline__ T get(int r, uint32_t start, int lane) const {
+        return p8_value<T>((int8_t)codes[r][lane], exps[r][(start % kP8Group + lane) / kP8Group]);
+    }
+};
+struct NoRows {};
+
 // The same backward: position r counts from the last step.  A state's gradient D comes to a step from the one behind it (r - 1) times
 // that one's gate.
-template <class T, int FORM, class S, int W, int L>
+template <class T, int FORM, class S, int W, int L, bool ALIGNED>
 __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, S> a, Chain ch, uint32_t col_blocks) {
     __shared__ JoinRoom<T, W, 64> room;
+    constexpr bool kHeld = S::kHeld, kSigmoid = FORM == RT_SCAN_SIGMOID;
+    typedef typename std::conditional<kHeld, HeldRows<L>, NoRows>::type Rows;
+    __shared__ Rows hrows[W], xrows[kSigmoid ? W : 1];
     const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
     if (k >= ch.tiles) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -428,20 +479,29 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
     const bool top = te == 0;
     const uint64_t base = ((uint64_t)o * a.steps + te) * row + col0;                            // of the earliest step: j is n - 1 - j rows on
     const uint64_t sc = (uint64_t)o * row + col0 + lc;
-    T g[L], up[L], hp[L], xv[L], s[L], f0 = (T)1, A = (T)1, H = (T)0;
+    T g[L], up[L], hp[kHeld ? 1 : L], xv[kHeld || !kSigmoid ? 1 : L], s[L], f0 = (T)1, A = (T)1, H = (T)0;
+    T st = (T)0;                                                 // the state before step 0
     uint64_t resets = 0, cuts = 0;                               // bit j: step j is reset; the step behind j is
     if (n) {
         const T *gate = a.gate + base, *dh = a.dh + base;
-        const T st = top && a.state ? a.state[sc] : (T)0;
+        if (top && a.state) st = a.state[sc];
+        HeldRegs hv, xh;
+        if constexpr (kHeld) {
+            const uint64_t total = a.outer * a.steps * row;
+            hv = HeldRows<L>::load(a.h, base - row, row, n, top ? 1 : 0, total, lane);
+            if constexpr (kSigmoid) xh = HeldRows<L>::load(a.x, base, row, n, 0, total, lane);
+        }
         if (r0 > 0) f0 = gate[lc + (uint32_t)n * row];           // the gate of the step behind j = 0
 #pragma unroll
         for (int j = 0; j < L; ++j) {
             const int q = j < n ? n - 1 - j : 0;
             const uint32_t at = lc + (uint32_t)q * row;
-            g[j] = __builtin_nontemporal_load(gate + at);
-            up[j] = __builtin_nontemporal_load(dh + at);
-            if constexpr (FORM == RT_SCAN_SIGMOID) xv[j] = a.x.at(base, at);
-            hp[j] = top && q == 0 ? st : a.h.at(base - row, at);
+            g[j] = once<ALIGNED>(gate + at);
+            up[j] = once<ALIGNED>(dh + at);
+            if constexpr (!kHeld) {
+                if constexpr (kSigmoid) xv[j] = a.x.template at<ALIGNED>(base, at);
+                hp[j] = top && q == 0 ? st : a.h.template at<ALIGNED>(base - row, at);
+            }
         }
         if (a.reset) {
             resets = reset_bits(a.reset + (uint64_t)o * a.steps + tl, -1, n, lane);
@@ -466,6 +526,10 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
             }
             f = s[j];
         }
+        if constexpr (kHeld) {
+            hrows[w].put(hv, lane);
+            if constexpr (kSigmoid) xrows[w].put(xh, lane);
+        }
     }
     const T first = k == 0 && a.dlast ? a.dlast[sc] : (T)0;
     T *dg = a.dgate + base, *dx = a.dx + base;
@@ -479,14 +543,23 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
                 if (j < rn) {
                     d = rcuts >> j & 1 ? up[j] : fused(j == 0 ? f0 : s[j ? j - 1 : 0], d, up[j]);
                     const bool none = rresets >> j & 1;
-                    const T p = none ? (T)0 : hp[j];
-                    const uint32_t at = lane + (uint32_t)(rn - 1 - j) * rrow;
+                    const int q = rn - 1 - j;                    // row of step j among the wave's, in memory order
+                    T hj, xj = (T)0;
+                    if constexpr (kHeld) {
+                        hj = top && q == 0 ? st : hrows[w].template get<T>(q, (uint32_t)base + (uint32_t)(q - 1) * rrow, lane);
+                        if constexpr (kSigmoid) xj = xrows[w].template get<T>(q, (uint32_t)base + (uint32_t)q * rrow, lane);
+                    } else {
+                        hj = hp[j];
+                        if constexpr (kSigmoid) xj = xv[j];
+                    }
+                    const T p = none ? (T)0 : hj;
+                    const uint32_t at = lane + (uint32_t)q * rrow;
                     if constexpr (FORM == RT_SCAN_LINEAR) {
                         const bool unused = none || (top && j == rn - 1 && !a.state);
                         __builtin_nontemporal_store(unused ? (T)0 : d * p, dg + at);
                         __builtin_nontemporal_store(d, dx + at);
                     } else {
-                        __builtin_nontemporal_store(d * (p - xv[j]) * (s[j] * g[j]), dg + at);
+                        __builtin_nontemporal_store(d * (p - xj) * (s[j] * g[j]), dg + at);
                         __builtin_nontemporal_store(g[j] * d, dx + at);
                     }
                 }
@@ -884,6 +957,8 @@ constexpr uint64_t kWideLeast = 32;             // inner: at least half of a wav
 constexpr uint64_t kWideMost = 1ull << 22;      // inner: a wave's rows are addressed with 32-bit offsets; beyond it columns alone fill the card
 constexpr uint64_t kFewSteps = 8;               // steps that one lane a column goes through without help
 
+template <class T> bool whole_lines(uint64_t inner) { return inner * sizeof(T) % 128 == 0; }
+
 // One lane a column: few steps (a token), or so many columns that they fill the card.
 bool by_columns(uint64_t steps, uint64_t inner) { return steps <= kFewSteps || inner >= kWideMost; }
 
@@ -931,8 +1006,10 @@ template <class T, int FORM> int32_t forward_form(rt_ctx* ctx, const ScanArgs<T>
         const uint64_t tile = a.steps <= L ? L : kWaves * L;     // one wave's steps are a tile where they are enough
         RT_TRY(make_chain<T>(ctx, (a.steps + tile - 1) / tile, a.outer * cb, &ch));
         const dim3 grid(ch.rounds * ch.lines);
-        if (a.steps <= L) hipLaunchKernelGGL((scan_wide_kernel<T, FORM, 1, L>), grid, dim3(64), 0, ctx->stream, a, ch, (uint32_t)cb);
-        else hipLaunchKernelGGL((scan_wide_kernel<T, FORM, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
+        const bool whole = whole_lines<T>(a.inner);
+        auto one = whole ? scan_wide_kernel<T, FORM, 1, L, true> : scan_wide_kernel<T, FORM, 1, L, false>;
+        auto many = whole ? scan_wide_kernel<T, FORM, kWaves, L, true> : scan_wide_kernel<T, FORM, kWaves, L, false>;
+        hipLaunchKernelGGL(a.steps <= L ? one : many, grid, dim3(a.steps <= L ? 64 : kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
     }
     RT_HIP(hipGetLastError());
     return RT_OK;
@@ -942,7 +1019,10 @@ template <class T> int32_t forward_typed(rt_ctx* ctx, int form, const ScanArgs<T
 }
 
 template <class T, int FORM, class S> int32_t backward_form(rt_ctx* ctx, const BackArgs<T, S>& a) {
-    constexpr int kWaves = 4, kNarrowWaves = 8, L = backward_steps<T>();
+#ifndef RT_BW
+#define RT_BW 4
+#endif
+    constexpr int kWaves = RT_BW, kNarrowWaves = 8, L = backward_steps<T>();
     Chain ch;
     if (by_columns(a.steps, a.inner)) {
         hipLaunchKernelGGL((scan_backward_columns_kernel<T, FORM, S>), dim3(blocks_of(a.outer * a.inner)), dim3(kSBlock), 0, ctx->stream, a);
@@ -959,8 +1039,10 @@ template <class T, int FORM, class S> int32_t backward_form(rt_ctx* ctx, const B
         const uint64_t tile = a.steps <= L ? L : kWaves * L;
         RT_TRY(make_chain<T>(ctx, (a.steps + tile - 1) / tile, a.outer * cb, &ch));
         const dim3 grid(ch.rounds * ch.lines);
-        if (a.steps <= L) hipLaunchKernelGGL((scan_backward_wide_kernel<T, FORM, S, 1, L>), grid, dim3(64), 0, ctx->stream, a, ch, (uint32_t)cb);
-        else hipLaunchKernelGGL((scan_backward_wide_kernel<T, FORM, S, kWaves, L>), grid, dim3(kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
+        const bool whole = whole_lines<T>(a.inner);
+        auto one = whole ? scan_backward_wide_kernel<T, FORM, S, 1, L, true> : scan_backward_wide_kernel<T, FORM, S, 1, L, false>;
+        auto many = whole ? scan_backward_wide_kernel<T, FORM, S, kWaves, L, true> : scan_backward_wide_kernel<T, FORM, S, kWaves, L, false>;
+        hipLaunchKernelGGL(a.steps <= L ? one : many, grid, dim3(a.steps <= L ? 64 : kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
     }
     RT_HIP(hipGetLastError());
     return RT_OK;
