@@ -423,25 +423,18 @@ template <int BI, int BJ, int WI, int WJ, int DEPTH, bool EVEN> int32_t f32_laun
     return RT_OK;
 }
 
-#ifndef RT_E1
-#define RT_E1 0.8
-#define RT_E2 0.6
-#define RT_LEAST 64
-#define RT_PER 2
-#endif
-#ifndef RT_D1
-#define RT_D1 1
-#define RT_D2 2
-#endif
 template <bool EVEN> int32_t f32_any(rt_ctx* ctx, const Product& p, int shape) {
     if (shape == 0) return f32_launch<256, 256, 2, 4, 1, EVEN>(ctx, p);
-    if (shape == 1) return f32_launch<256, 128, 4, 2, RT_D1, EVEN>(ctx, p);
-    return f32_launch<128, 128, 2, 2, RT_D2, EVEN>(ctx, p);
+    if (shape == 1) return f32_launch<256, 128, 4, 2, 1, EVEN>(ctx, p);
+    return f32_launch<128, 128, 2, 2, 2, EVEN>(ctx, p);
 }
 
 int32_t run_product(rt_ctx* ctx, int dtype, Product p, void* dst) {
     struct Shape { uint64_t bi, bj, least_rows, per_cu; double rate; };
-    static const Shape f32[3] = {{256, 256, 512, 1, 1.0}, {256, 128, 256, 1, RT_E1}, {128, 128, RT_LEAST, RT_PER, RT_E2}};
+    // The tile's shape: the larger, the fewer conversions there are for each matrix instruction.  `rate` is what a shape reaches of the
+    // first one's rate on a result it divides (16384 x 4096 x 4096: 1441, 1633 and 1824 us -- the smaller ones are better than that on
+    // short shares, hence less weight); the shape with the least padded area at its rate is taken, of those that give every CU a block.
+    static const Shape f32[3] = {{256, 256, 512, 1, 1.0}, {256, 128, 256, 1, 0.8}, {128, 128, 64, 2, 0.6}};
     static const Shape f64[2] = {{128, 128, 128, 2, 1.0}, {64, 64, 64, 4, 1.0}};
     auto tiles_of = [&](const Shape& s) { return p.b * ((p.k + s.bi - 1) / s.bi) * ((p.n + s.bj - 1) / s.bj); };
     int shape = dtype == RT_F64 && tiles_of(f64[0]) * (p.m / f64[0].least_rows) < (uint64_t)ctx->num_cus ? 1 : 0;

@@ -254,7 +254,20 @@ template <class T, int W, int LN> __device__ __forceinline__ T chain_start(const
     }
     __syncthreads();
     T c = (T)0;
-    for (int q = found; q >= 0; --q) c = room.ends[q] >> lane & 1 ? room.winH[q][lane & (LN - 1)] : fused(room.winA[q][lane & (LN - 1)], c, room.winH[q][lane & (LN - 1)]);
+    for (int q0 = found; q0 >= 0; q0 -= 4) {                     // four at a time are read before the first is used
+        T A[4], H[4];
+        uint64_t ends[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int q = q0 - i < 0 ? 0 : q0 - i;
+            A[i] = room.winA[q][lane & (LN - 1)];
+            H[i] = room.winH[q][lane & (LN - 1)];
+            ends[i] = room.ends[q];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (q0 - i >= 0) c = ends[i] >> lane & 1 ? H[i] : fused(A[i], c, H[i]);
+    }
     return c;
 }
 
@@ -1019,10 +1032,9 @@ template <class T> int32_t forward_typed(rt_ctx* ctx, int form, const ScanArgs<T
 }
 
 template <class T, int FORM, class S> int32_t backward_form(rt_ctx* ctx, const BackArgs<T, S>& a) {
-#ifndef RT_BW
-#define RT_BW 4
-#endif
-    constexpr int kWaves = RT_BW, kNarrowWaves = 8, L = backward_steps<T>();
+    // waves of a wide tile: with the registers of the linear form two blocks of eight fit a CU, of the other one three of four; longer tiles
+    // make shorter chains (linear from the 8-bit form over (1, 50000, 1088): 195 us with four, 164 with eight; the other one 199 and 215)
+    constexpr int kWaves = FORM == RT_SCAN_LINEAR ? 8 : 4, kNarrowWaves = 8, L = backward_steps<T>();
     Chain ch;
     if (by_columns(a.steps, a.inner)) {
         hipLaunchKernelGGL((scan_backward_columns_kernel<T, FORM, S>), dim3(blocks_of(a.outer * a.inner)), dim3(kSBlock), 0, ctx->stream, a);
