@@ -339,7 +339,7 @@ int32_t rt_matmul(rt_ctx* ctx, int32_t dtype,
  *     D[t] = dh[t] + (reset[t + 1] ? 0 : a[t + 1] * D[t + 1]),   D[steps - 1] = dh[steps - 1] + dlast
  *     RT_SCAN_LINEAR    dx = D,            dgate = D * p   (0 where nothing precedes)
  *     RT_SCAN_SIGMOID   dx = (1 - s) * D,  dgate = D * (p - x) * s * (1 - s)
- *     dstate = a[0] * D[0] (0 where reset[0]); dstate may be null
+ *     dstate = a[0] * D[0] (0 where reset[0]), of a state of zeros where state is null; dstate may be null
  * h is what the forward pass wrote.  x is read by RT_SCAN_SIGMOID alone and may be null for RT_SCAN_LINEAR.  dx may be dh itself or
  * x itself, dstate may be dlast itself.
  * rt_gated_scan_backward_packed8: the same with x and h in the 8-bit form below (codes and exponents of the whole (outer, steps,

@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kSBlock) void scan_backward_columns_kernel(BackArgs
         if constexpr (FORM == RT_SCAN_LINEAR) {
             a.dgate[at] = none ? (T)0 : d * p;
             a.dx[at] = d;
-            carry = none ? (T)0 : g * d;
+            carry = cut ? (T)0 : g * d;
         } else {
             const RtGate<T> q = rt_gate_of(g);
             const T x = a.x.at(at, 0);
@@ -582,7 +582,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
     });
     if (a.dstate && in && n && top) {
         const T g0 = a.gate[(uint64_t)o * a.steps * row + col];
-        const bool none = (a.reset && a.reset[(uint64_t)o * a.steps]) || (FORM == RT_SCAN_LINEAR && !a.state);
+        const bool none = a.reset && a.reset[(uint64_t)o * a.steps];
         a.dstate[sc] = none ? (T)0 : (FORM == RT_SCAN_SIGMOID ? gate_of(g0).s : g0) * end;
     }
 }
@@ -916,7 +916,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
                 __builtin_nontemporal_store(d * (before - x[q]) * (f.s * f.r), a.dgate + base + e);
                 __builtin_nontemporal_store(f.r * d, a.dx + base + e);
             }
-            if (head[q] && a.dstate) a.dstate[sc[q]] = reset[q] || (FORM == RT_SCAN_LINEAR && !a.state) ? (T)0 : factor * d;
+            if (head[q] && a.dstate) a.dstate[sc[q]] = reset[q] ? (T)0 : factor * d;
         }
     }
 }

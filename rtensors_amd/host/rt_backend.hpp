@@ -115,6 +115,7 @@ enum class ReductionOpTypes : int {
     LogSumExp = RT_R_LOGSUMEXP, NormL1 = RT_R_NORM | RT_R_FLAG_L1, NormL2 = RT_R_NORM | RT_R_FLAG_L2,
     ArgMax = RT_R_ARGMAX, ArgMin = RT_R_ARGMIN
 };
+enum class ScanForm : int { Linear = RT_SCAN_LINEAR, Sigmoid = RT_SCAN_SIGMOID };
 enum class NormType { L1, L2 };                                   // ops/reduction/mod.rs:203-206
 
 class Hip;
@@ -311,12 +312,54 @@ class Hip {
                                           dbias.len(), rows, cols));
     }
 
+    // ---- gated linear recurrence and activations held in 8 bits (no counterpart in the trait) -----------------------------------------------
+    void gated_scan(ScanForm form, const HipBuf& gate, const HipBuf& x, const HipBuf* state, const HipBuf* reset, HipBuf& h, HipBuf* last, uint64_t outer,
+                    uint64_t steps, uint64_t inner) const {
+        check(rt_gated_scan(raw(), h.dtype(), (int32_t)form, gate.ptr(), gate.len(), x.ptr(), x.len(), ptr_of(state), len_of(state), ptr_of(reset), len_of(reset),
+                            h.ptr(), h.len(), ptr_of(last), len_of(last), outer, steps, inner));
+    }
+    void gated_scan_backward(ScanForm form, const HipBuf& gate, const HipBuf* x, const HipBuf& h, const HipBuf* state, const HipBuf* reset, const HipBuf& dh,
+                             const HipBuf* dlast, HipBuf& dgate, HipBuf& dx, HipBuf* dstate, uint64_t outer, uint64_t steps, uint64_t inner) const {
+        check(rt_gated_scan_backward(raw(), dx.dtype(), (int32_t)form, gate.ptr(), gate.len(), ptr_of(x), len_of(x), h.ptr(), h.len(), ptr_of(state), len_of(state),
+                                     ptr_of(reset), len_of(reset), dh.ptr(), dh.len(), ptr_of(dlast), len_of(dlast), dgate.ptr(), dgate.len(), dx.ptr(), dx.len(),
+                                     ptr_of(dstate), len_of(dstate), outer, steps, inner));
+    }
+    // x and h as their codes and exponent bytes
+    void gated_scan_backward_packed8(ScanForm form, const HipBuf& gate, const HipBuf* x_codes, const HipBuf* x_exps, const HipBuf& h_codes, const HipBuf& h_exps,
+                                     const HipBuf* state, const HipBuf* reset, const HipBuf& dh, const HipBuf* dlast, HipBuf& dgate, HipBuf& dx, HipBuf* dstate,
+                                     uint64_t outer, uint64_t steps, uint64_t inner) const {
+        check(rt_gated_scan_backward_packed8(raw(), dx.dtype(), (int32_t)form, gate.ptr(), gate.len(), ptr_of(x_codes), len_of(x_codes), ptr_of(x_exps),
+                                             len_of(x_exps), h_codes.ptr(), h_codes.len(), h_exps.ptr(), h_exps.len(), ptr_of(state), len_of(state), ptr_of(reset),
+                                             len_of(reset), dh.ptr(), dh.len(), ptr_of(dlast), len_of(dlast), dgate.ptr(), dgate.len(), dx.ptr(), dx.len(),
+                                             ptr_of(dstate), len_of(dstate), outer, steps, inner));
+    }
+    void pack8(const HipBuf& src, uint64_t start, uint64_t len, HipBuf& codes, HipBuf& exps) const {
+        check(rt_pack8(raw(), src.dtype(), src.ptr(), src.len(), start, len, codes.ptr(), codes.len(), exps.ptr(), exps.len()));
+    }
+    void unpack8(const HipBuf& codes, const HipBuf& exps, uint64_t len, HipBuf& dst) const {
+        check(rt_unpack8(raw(), dst.dtype(), codes.ptr(), codes.len(), exps.ptr(), exps.len(), len, dst.ptr(), dst.len()));
+    }
+    void pack8_unary(int op, const HipBuf& src, uint64_t start, uint64_t len, HipBuf& dst, HipBuf& codes, HipBuf& exps) const {
+        check(rt_pack8_unary(raw(), src.dtype(), op, src.ptr(), src.len(), start, len, dst.ptr(), dst.len(), codes.ptr(), codes.len(), exps.ptr(), exps.len()));
+    }
+    void pack8_unary_backward(int op, const HipBuf& codes, const HipBuf& exps, const HipBuf& upstream, uint64_t len, HipBuf& dst) const {
+        check(rt_pack8_unary_backward(raw(), dst.dtype(), op, codes.ptr(), codes.len(), exps.ptr(), exps.len(), upstream.ptr(), upstream.len(), len, dst.ptr(),
+                                      dst.len()));
+    }
+    void pack8_matmul_backward(const HipBuf& codes, const HipBuf& exps, const HipBuf& upstream, HipBuf& dst, uint64_t b, uint64_t m, uint64_t k, uint64_t n) const {
+        check(rt_pack8_matmul_backward(raw(), dst.dtype(), codes.ptr(), codes.len(), exps.ptr(), exps.len(), upstream.ptr(), upstream.len(), dst.ptr(), dst.len(),
+                                       b, m, k, n));
+    }
+
     // row-major copy of a view (what TensorView::owned needs, core/tensor.rs:299-325) in one launch
     void gather(const HipBuf& src, const MetaTensor& m, HipBuf& dst) const {
         check(rt_gather(raw(), src.dtype(), src.ptr(), src.len(), m.offset, (int32_t)m.rank(), m.shape.data(), m.strides.data(), dst.ptr(), dst.len()));
     }
 
   private:
+    static void* ptr_of(const HipBuf* b) { return b ? b->ptr() : nullptr; }
+    static uint64_t len_of(const HipBuf* b) { return b ? b->len() : 0; }
+
     std::shared_ptr<rt_ctx> ctx_;
 };
 

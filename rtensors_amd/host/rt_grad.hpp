@@ -1,5 +1,5 @@
-// Reverse-mode tape for the broadcast/reduce training step (no matmul): y = relu(x + bias), loss = mean_l1_loss(y, t),
-// backward to d(bias), SGD update.  Follows the reference's engine: grad/mod.rs:269-308 (context, attach), 432-495
+// Reverse-mode tape for the broadcast/reduce training step y = relu(x + bias), loss = mean_l1_loss(y, t), backward to d(bias), SGD
+// update, and for layers of matmul, sigmoid / silu / tanh and the gated scan.  Follows the reference's engine: grad/mod.rs:269-308 (context, attach), 432-495
 // (backwards: toposort, upstream accumulation), grad/backwards.rs:7-42, 148-161, 229-239, 516-538 (node rules),
 // ops/broadcast/l1.rs:16-84 (L1 loss and its gradient map), ops/unary/mod.rs:234-252 (ReLU gradient map),
 // grad/optim.rs:28-50 (SGD).  Every arithmetic step is a backend call issued through rt::Tensor.
@@ -23,7 +23,7 @@ namespace grad {
 //                      upstream buffer.  Kept so the divergence can be shown in a test.
 enum class BroadcastGradMode { Sum, ReferenceLiteral };
 
-enum class NodeKind { None, Leaf, BroadcastAdd, BroadcastSub, ReLU, L1, MatMul };
+enum class NodeKind { None, Leaf, BroadcastAdd, BroadcastSub, ReLU, L1, MatMul, Unary, GatedScan };
 
 struct Node {
     NodeKind kind = NodeKind::None;
@@ -32,6 +32,14 @@ struct Node {
     Shape lhs_shape, rhs_shape;
     Tensor grad_map;                     // ReLU, L1
     Tensor left_input, right_input;      // MatMul (row-major copies, ops/linalg/matmul.rs:126-130)
+    bool packed = false;                 // what this node keeps of its activations is in the 8-bit form
+    Packed8 input8, output8;             // MatMul: the left input;  Unary: the input;  GatedScan: x and h
+    int op = 0;                          // Unary
+    Tensor input, output;                // Unary: the input;  GatedScan: x and h
+    Tensor gate, state, reset;           // GatedScan (state and reset: rank 0 without a buffer where there are none)
+    bool has_state = false, has_reset = false;
+    size_t axis = 0;
+    ScanForm form = ScanForm::Linear;
     Tensor loss;                         // L1
     std::shared_ptr<Tensor> grad;        // Leaf: accumulated gradient (null until the first backward pass)
 };
@@ -45,6 +53,10 @@ class GradContext {
   public:
     BroadcastGradMode mode = BroadcastGradMode::Sum;
     bool seed_with_loss = true;   // grad/mod.rs:442-447 seeds the root with the loss tensor itself, not with 1
+    // Keep the activations that a backward pass reads in 8 bits instead of whole: the left input of a matmul (where it is no parameter), the
+    // input of sigmoid / silu / tanh, x and h of a scan (of an x that is no parameter).  The maps of relu, leaky_relu, abs and the loss stay as they are (their values
+    // are signs), and so do parameters, gates and states.  f32 / f64.
+    bool packed_activations = false;
 
     Var input(const Tensor& t) { return Var{t, -1}; }
     Var param(const Tensor& t) {                        // TensorBase::param + GradNode::Leaf
@@ -93,8 +105,61 @@ class GradContext {
         Node n;
         n.kind = NodeKind::MatMul;
         n.parents = {a.node, b.node};
-        n.left_input = a.t.contiguous();
+        n.packed = packs(a) && b.node >= 0 && a.t.shape().back() < kPackedMost && b.t.shape().back() < kPackedMost;
+        if (n.packed) n.input8 = a.t.pack8();
+        else n.left_input = a.t.contiguous();
         n.right_input = b.t.contiguous();
+        nodes_.push_back(n);
+        return Var{result, (int)nodes_.size() - 1};
+    }
+
+    // sigmoid, silu and tanh on the tape (no counterpart in the reference's, whose unary nodes are relu and abs): the node keeps the input,
+    // whole or in 8 bits; op: RT_U_SIGMOID, RT_U_SILU, RT_U_TANH
+    Var unary(const Var& a, int op) {
+        if (op != RT_U_SIGMOID && op != RT_U_SILU && op != RT_U_TANH) throw TensorError(ErrorKind::UnsupportedOperation, "unary: sigmoid, silu or tanh");
+        if (a.node < 0) return Var{a.t.unary(op), -1};
+        Node n;
+        n.kind = NodeKind::Unary;
+        n.parents = {a.node};
+        n.op = op;
+        n.packed = packs(a);
+        Tensor result;
+        if (n.packed) {
+            result = a.t.unary_pack8(op, n.input8);
+        } else {
+            n.input = a.t.contiguous();
+            result = a.t.unary(op);
+        }
+        nodes_.push_back(n);
+        return Var{result, (int)nodes_.size() - 1};
+    }
+    Var sigmoid(const Var& a) { return unary(a, RT_U_SIGMOID); }
+    Var silu(const Var& a) { return unary(a, RT_U_SILU); }
+    Var tanh(const Var& a) { return unary(a, RT_U_TANH); }
+
+    // h = gated_scan of x by `gate` along `axis` (Tensor::gated_scan).  Gradients flow to x, to the gate and to the state.
+    Var gated_scan(const Var& x, const Var& gate, size_t axis, ScanForm form, const Var* state = nullptr, const Tensor* reset = nullptr) {
+        Tensor result = x.t.gated_scan(gate.t, axis, form, state ? &state->t : nullptr, reset);
+        const int sn = state ? state->node : -1;
+        if (x.node < 0 && gate.node < 0 && sn < 0) return Var{result, -1};
+        Node n;
+        n.kind = NodeKind::GatedScan;
+        n.parents = {x.node, gate.node, sn};
+        n.axis = axis;
+        n.form = form;
+        n.gate = gate.t.contiguous();
+        n.has_state = state != nullptr;
+        n.has_reset = reset != nullptr;
+        if (state) n.state = state->t.contiguous();
+        if (reset) n.reset = reset->contiguous();
+        n.packed = packs(x);
+        if (n.packed) {
+            n.output8 = result.pack8();
+            if (form == ScanForm::Sigmoid) n.input8 = x.t.pack8();
+        } else {
+            n.output = result.owned();
+            if (form == ScanForm::Sigmoid) n.input = x.t.contiguous();
+        }
         nodes_.push_back(n);
         return Var{result, (int)nodes_.size() - 1};
     }
@@ -140,6 +205,18 @@ class GradContext {
                 if (n.parents[p] >= 0) acc[n.parents[p]].push_back(down[p]);
             acc.erase(key);
         }
+    }
+
+    // Bytes that the nodes keep for the backward pass (leaves apart; buffers that two of them share count twice).
+    uint64_t kept_bytes() const {
+        uint64_t n = 0;
+        auto whole = [&](const Tensor& t) { return t.has_buffer() ? t.buf()->len() * (uint64_t)rt_dtype_size(t.dtype()) : 0; };
+        auto packed = [&](const Packed8& p) { return p.codes ? p.codes->len() + p.exps->len() : 0; };
+        for (const Node& d : nodes_) {
+            for (const Tensor* t : {&d.grad_map, &d.left_input, &d.right_input, &d.input, &d.output, &d.gate, &d.state, &d.reset}) n += whole(*t);
+            n += packed(d.input8) + packed(d.output8);
+        }
+        return n;
     }
 
     std::shared_ptr<Tensor> grad_of(const Var& v) const { return v.node >= 0 ? nodes_[(size_t)v.node].grad : nullptr; }
@@ -194,6 +271,50 @@ class GradContext {
         return Var{result, (int)nodes_.size() - 1};
     }
 
+    // whether a node keeps this activation in 8 bits: not a parameter, which is there anyway
+    bool packs(const Var& v) const { return packed_activations && !is_leaf(v) && (v.t.dtype() == RT_F32 || v.t.dtype() == RT_F64); }
+    bool is_leaf(const Var& v) const { return v.node >= 0 && nodes_[(size_t)v.node].kind == NodeKind::Leaf; }
+    static constexpr uint64_t kPackedMost = 1ull << 25;          // columns the packed matmul gradient takes
+
+    // f'(x) of sigmoid, silu and tanh from the ordinary operators
+    static Tensor slope(int op, const Tensor& x) {
+        if (op == RT_U_TANH) {                                   // 1 - tanh^2
+            Tensor t = x.tanh();
+            t.unary_inplace(RT_U_SQUARE);
+            t *= -1.0;
+            t += 1.0;
+            return t;
+        }
+        const Tensor s = x.sigmoid(), rest = (-x).sigmoid();     // 1 - sigmoid(x) without a difference
+        if (op == RT_U_SIGMOID) return s * rest;
+        Tensor f = x * rest;                                     // s (1 + x (1 - s))
+        f += 1.0;
+        return s * f;
+    }
+
+    std::vector<Tensor> scan_backwards(const Node& n, const Tensor& up_any) {
+        const Tensor up = up_any.whole();
+        const Hip& be = up.backend();
+        const Tensor::ScanSizes z = Tensor::scan_sizes(up, n.axis);
+        const int dt = up.dtype();
+        auto fresh = [&](const Shape& shape) { return Tensor(be, be.alloc_uninit(dt, MetaTensor::row_major(shape).size()), MetaTensor::row_major(shape)); };
+        std::vector<Tensor> out = {fresh(up.shape()), fresh(up.shape()), Tensor()};
+        if (n.parents[2] >= 0) out[2] = fresh(z.state);
+        const Tensor gate = n.gate.whole(), state = n.has_state ? n.state.whole() : Tensor(), reset = n.has_reset ? n.reset.whole() : Tensor();
+        const HipBuf *st = n.has_state ? state.buf().get() : nullptr, *rs = n.has_reset ? reset.buf().get() : nullptr;
+        HipBuf* ds = n.parents[2] >= 0 ? out[2].buf().get() : nullptr;
+        const bool sigmoid = n.form == ScanForm::Sigmoid;
+        if (n.packed) {
+            be.gated_scan_backward_packed8(n.form, *gate.buf(), sigmoid ? n.input8.codes.get() : nullptr, sigmoid ? n.input8.exps.get() : nullptr, *n.output8.codes,
+                                           *n.output8.exps, st, rs, *up.buf(), nullptr, *out[1].buf(), *out[0].buf(), ds, z.outer, z.steps, z.inner);
+        } else {
+            const Tensor h = n.output.whole(), x = sigmoid ? n.input.whole() : Tensor();
+            be.gated_scan_backward(n.form, *gate.buf(), sigmoid ? x.buf().get() : nullptr, *h.buf(), st, rs, *up.buf(), nullptr, *out[1].buf(), *out[0].buf(), ds,
+                                   z.outer, z.steps, z.inner);
+        }
+        return out;
+    }
+
     std::vector<Tensor> node_backwards(Node& n, const Tensor& up) {
         switch (n.kind) {
             case NodeKind::Leaf:                                         // accumulate_grad, backwards.rs:7-25
@@ -230,9 +351,14 @@ class GradContext {
                 };
                 std::vector<Tensor> out(2);
                 if (n.parents[0] >= 0) out[0] = up.matmul(swap_last_two(n.right_input));
-                if (n.parents[1] >= 0) out[1] = swap_last_two(n.left_input).matmul(up);
+                if (n.parents[1] >= 0) out[1] = n.packed ? up.matmul_backward_pack8(n.input8) : swap_last_two(n.left_input).matmul(up);
                 return out;
             }
+            case NodeKind::Unary:
+                if (n.packed) return {up.unary_backward_pack8(n.op, n.input8)};
+                return {up * slope(n.op, n.input)};
+            case NodeKind::GatedScan:
+                return scan_backwards(n, up);
             default:
                 return {};
         }

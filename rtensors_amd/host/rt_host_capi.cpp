@@ -174,6 +174,33 @@ int rth_expr_eval(void* first, int nsteps, const int* kinds, const int* ops, con
     });
 }
 
+// ---- gated scan and the 8-bit form of activations ------------------------------------------------------------------------------------
+// state and reset may be null; so may out_last.  form: rt_scan_form.
+int rth_gated_scan(void* x, void* gate, uint64_t axis, int form, void* state, void* reset, void** out, void** out_last) {
+    return guarded([&] {
+        if (form != RT_SCAN_LINEAR && form != RT_SCAN_SIGMOID) throw TensorError(ErrorKind::UnsupportedOperation, "unknown scan form");
+        Tensor last;
+        Tensor h = ((Tensor*)x)->gated_scan(*(Tensor*)gate, (size_t)axis, (ScanForm)form, (Tensor*)state, (Tensor*)reset, out_last ? &last : nullptr);
+        *out = new Tensor(h);
+        if (out_last) *out_last = new Tensor(last);
+    });
+}
+int rth_pack8(void* t, void** out) { return guarded([&] { *out = new Packed8(((Tensor*)t)->pack8()); }); }
+void rth_packed8_free(void* p) { delete (Packed8*)p; }
+int rth_unpack8(void* backend, void* p, void** out) { return guarded([&] { *out = new Tensor(Tensor::unpack8(*(Hip*)backend, *(Packed8*)p)); }); }
+int rth_unary_pack8(void* t, int op, void** out, void** out_packed) {
+    return guarded([&] {
+        Packed8 p;
+        Tensor r = ((Tensor*)t)->unary_pack8(op, p);
+        *out = new Tensor(r);
+        *out_packed = new Packed8(p);
+    });
+}
+int rth_unary_backward_pack8(void* up, int op, void* p, void** out) {
+    return guarded([&] { *out = new Tensor(((Tensor*)up)->unary_backward_pack8(op, *(Packed8*)p)); });
+}
+int rth_matmul_backward_pack8(void* up, void* p, void** out) { return guarded([&] { *out = new Tensor(((Tensor*)up)->matmul_backward_pack8(*(Packed8*)p)); }); }
+
 // ---- the training step of the autograd configuration -----------------------------------------------------------------------
 // y = relu(x + bias); loss = mean_l1_loss(y, target); backward; SGD(lr) on bias (updated in place).
 // mode: 0 = sum over the broadcast dim, 1 = reference-literal metadata rewrite.  seed_with_loss: 1 = the reference's
@@ -215,6 +242,38 @@ int rth_train_step_fused(void* x, void* bias, void* target, double lr, int seed_
         Tensor update = st.dbias * lr;
         Tensor v = ((Tensor*)bias)->view();
         v -= update;
+    });
+}
+
+// A gated recurrent layer over rows of tokens (reset, bool (tokens): where a document starts; null: one document):
+//   h = gated_scan(silu(x @ w_value), x @ w_gate, tokens, Sigmoid);  y = h @ w_out;  loss = mean_l1_loss(y, target)
+// backward, SGD(lr) on the three weights (updated in place).  packed: the tape keeps its activations in 8 bits.  Outputs: the loss, the
+// gradients that were applied (w_gate, w_value, w_out), and the bytes the tape kept for the backward pass.
+int rth_gated_layer_step(void* x, void* w_gate, void* w_value, void* w_out, void* target, void* reset, double lr, int packed, int seed_with_loss, void** out_loss,
+                         void** out_grads, uint64_t* out_kept) {
+    return guarded([&] {
+        grad::GradContext ctx;
+        ctx.seed_with_loss = seed_with_loss != 0;
+        ctx.packed_activations = packed != 0;
+        grad::Var vx = ctx.input(*(Tensor*)x), vt = ctx.input(*(Tensor*)target);
+        grad::Var w[3] = {ctx.param(*(Tensor*)w_gate), ctx.param(*(Tensor*)w_value), ctx.param(*(Tensor*)w_out)};
+        grad::SGD opt(lr);
+        for (grad::Var& v : w) opt.register_parameter(ctx, v);
+        grad::Var gate = ctx.matmul(vx, w[0]);
+        grad::Var value = ctx.silu(ctx.matmul(vx, w[1]));
+        grad::Var h = ctx.gated_scan(value, gate, 0, ScanForm::Sigmoid, nullptr, (Tensor*)reset);
+        grad::Var loss = ctx.mean_l1_loss(ctx.matmul(h, w[2]), vt);
+        *out_kept = ctx.kept_bytes();
+        ctx.backwards(loss);
+        Tensor grads[3];
+        for (int k = 0; k < 3; ++k) {
+            std::shared_ptr<Tensor> g = ctx.grad_of(w[k]);
+            if (!g) throw TensorError(ErrorKind::GradError, "no gradient reached a weight");
+            grads[k] = g->contiguous();
+        }
+        opt.step();
+        for (int k = 0; k < 3; ++k) out_grads[k] = new Tensor(grads[k]);
+        *out_loss = new Tensor(loss.t);
     });
 }
 

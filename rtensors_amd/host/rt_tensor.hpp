@@ -11,12 +11,24 @@
 // like TensorView / TensorViewMut.
 #pragma once
 
+#include <algorithm>
 #include <optional>
+#include <string>
 #include <vector>
 
 #include "rt_backend.hpp"
 
 namespace rt {
+
+class Tensor;
+
+// A tensor's elements in the 8-bit form (include/rt_hip.h, "activations held in 8 bits"): what the autograd tape keeps of an activation.
+struct Packed8 {
+    Buf codes, exps;
+    Shape shape;
+    int dtype = RT_F32;                  // of the tensor that was packed
+    uint64_t size() const { return codes ? codes->len() : 0; }
+};
 
 class Tensor {
   public:
@@ -70,6 +82,7 @@ class Tensor {
     int dtype() const { return buf_->dtype(); }
     const Hip& backend() const { return *backend_; }
     const Buf& buf() const { return buf_; }
+    bool has_buffer() const { return buf_ != nullptr; }
 
     // ---- views: metadata only --------------------------------------------------------------------------------------------
     Tensor view() const { return with_meta(meta_); }
@@ -248,6 +261,101 @@ class Tensor {
         return unsqueeze_at(1).matmul(rhs.unsqueeze_at(0));
     }
 
+    // ---- gated linear recurrence along an axis (no counterpart in the reference): this tensor is x, `gate` has its shape --------------------
+    // h[t] = a * h[t - 1] + b along `axis`, h[-1] = state (zeros without one); form Linear: a = gate, b = x; form Sigmoid: a = sigmoid(gate),
+    // b = (1 - a) * x.  `state` has this shape without the axis; `reset` (bool) has the axes up to and including `axis`: true where the
+    // state before the step does not count.  Views are gathered first.  Where `last` is given it receives the state after the last step.
+    Tensor gated_scan(const Tensor& gate, size_t axis, ScanForm form, const Tensor* state = nullptr, const Tensor* reset = nullptr, Tensor* last = nullptr) const {
+        const ScanSizes z = scan_sizes(*this, axis);
+        check_scan_operand(gate, meta_.shape, "gate");
+        if (state) check_scan_operand(*state, z.state, "state");
+        if (reset) check_scan_reset(*reset, z);
+        const Tensor x = whole(), g = gate.whole();
+        const Tensor s = state ? state->whole() : Tensor(), r = reset ? reset->whole() : Tensor();
+        Tensor out = like_row_major();
+        Tensor end;
+        if (last) end = Tensor(*backend_, backend_->alloc_uninit(dtype(), z.outer * z.inner), MetaTensor::row_major(z.state));
+        backend_->gated_scan(form, *g.buf_, *x.buf_, state ? s.buf_.get() : nullptr, reset ? r.buf_.get() : nullptr, *out.buf_, last ? end.buf_.get() : nullptr,
+                             z.outer, z.steps, z.inner);
+        if (last) *last = end;
+        return out;
+    }
+
+    // ---- the 8-bit form (f32 / f64; views are gathered first) --------------------------------------------------------------------------------
+    Packed8 pack8() const {
+        const Tensor t = whole();
+        Packed8 p = empty_pack8();
+        backend_->pack8(*t.buf_, 0, size(), *p.codes, *p.exps);
+        return p;
+    }
+    static Tensor unpack8(const Hip& backend, const Packed8& p) {
+        Tensor t(backend, backend.alloc_uninit(p.dtype, p.size()), MetaTensor::row_major(p.shape));
+        backend.unpack8(*p.codes, *p.exps, p.size(), *t.buf_);
+        return t;
+    }
+    // op(this) and the 8-bit form of this in one pass; op: RT_U_SIGMOID, RT_U_SILU, RT_U_TANH
+    Tensor unary_pack8(int op, Packed8& p) const {
+        const Tensor t = whole();
+        p = empty_pack8();
+        Tensor r = like_row_major();
+        backend_->pack8_unary(op, *t.buf_, 0, size(), *r.buf_, *p.codes, *p.exps);
+        return r;
+    }
+    // this * op'(restored): this is the upstream gradient
+    Tensor unary_backward_pack8(int op, const Packed8& p) const {
+        if (p.shape != meta_.shape) throw TensorError(ErrorKind::InvalidShape, "The upstream gradient has another shape than the packed activation");
+        const Tensor t = whole();
+        Tensor r = like_row_major();
+        backend_->pack8_unary_backward(op, *p.codes, *p.exps, *t.buf_, size(), *r.buf_);
+        return r;
+    }
+    // restored^T @ this over the last two dims: the weight gradient of y = x @ w with x held in 8 bits, this being the gradient of y
+    Tensor matmul_backward_pack8(const Packed8& x) const {
+        const size_t r = rank();
+        if (r < 2 || x.shape.size() != r || !std::equal(x.shape.begin(), x.shape.end() - 1, meta_.shape.begin()))
+            throw TensorError(ErrorKind::InvalidShape, "The upstream gradient does not fit the packed input of the matmul");
+        uint64_t b = 1;
+        for (size_t i = 0; i + 2 < r; ++i) b *= meta_.shape[i];
+        const uint64_t m = meta_.shape[r - 2], n = meta_.shape[r - 1], k = x.shape[r - 1];
+        Shape out = meta_.shape;
+        out[r - 2] = k;
+        const Tensor up = whole();
+        Tensor d(*backend_, backend_->alloc_uninit(dtype(), b * k * n), MetaTensor::row_major(out));
+        backend_->pack8_matmul_backward(*x.codes, *x.exps, *up.buf_, *d.buf_, b, m, k, n);
+        return d;
+    }
+
+    // A tensor seen along an axis: (outer, steps, inner) and the shape without the axis.
+    struct ScanSizes {
+        uint64_t outer = 1, steps = 0, inner = 1;
+        Shape state, lead;               // lead: the axes up to and including `axis`
+    };
+    static ScanSizes scan_sizes(const Tensor& t, size_t axis) {
+        if (axis >= t.rank()) throw TensorError(ErrorKind::InvalidDim, "scan axis out of range");
+        ScanSizes z;
+        z.steps = t.shape()[axis];
+        for (size_t i = 0; i < t.rank(); ++i) {
+            if (i < axis) z.outer *= t.shape()[i];
+            if (i > axis) z.inner *= t.shape()[i];
+            if (i != axis) z.state.push_back(t.shape()[i]);
+            if (i <= axis) z.lead.push_back(t.shape()[i]);
+        }
+        return z;
+    }
+    // This tensor as a row-major run from element 0 of a buffer of its own size: itself, or a copy.
+    Tensor whole() const {
+        if (meta_.offset == 0 && buf_->len() == size() && (size() == 0 || (meta_.is_forward_contiguous() && meta_.strides == shape_to_stride(meta_.shape)))) return *this;
+        return gathered();
+    }
+    void check_scan_operand(const Tensor& t, const Shape& want, const char* what) const {
+        if (t.shape() != want) throw TensorError(ErrorKind::InvalidShape, std::string("scan: ") + what + " has another shape than the axis leaves");
+        if (t.dtype() != dtype()) throw TensorError(ErrorKind::UnsupportedOperation, std::string("scan: ") + what + " has another dtype");
+    }
+    static void check_scan_reset(const Tensor& t, const ScanSizes& z) {
+        if (t.shape() != z.lead) throw TensorError(ErrorKind::InvalidShape, "scan: reset has the axes up to and including the scanned one");
+        if (t.dtype() != RT_BOOL) throw TensorError(ErrorKind::UnsupportedOperation, "scan: reset is a bool tensor");
+    }
+
     // ---- reductions ----------------------------------------------------------------------------------------------------------------------
     // Non-contiguous inputs are copied first (ops/reduction/mod.rs:346-408).  "Contiguous" here means a forward
     // row-major run: a reversed view is |stride|-contiguous for the reference and would reach its kernels with the
@@ -331,6 +439,14 @@ class Tensor {
     void set_meta(const MetaTensor& m) { meta_ = m; }
 
   private:
+    Packed8 empty_pack8() const {
+        Packed8 p;
+        p.codes = backend_->alloc_uninit(RT_I8, size());
+        p.exps = backend_->alloc_uninit(RT_U8, (size() + RT_PACK8_GROUP - 1) / RT_PACK8_GROUP);
+        p.shape = meta_.shape;
+        p.dtype = dtype();
+        return p;
+    }
     Tensor with_meta(const MetaTensor& m) const {
         Tensor t = *this;
         t.meta_ = m;

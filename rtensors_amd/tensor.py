@@ -9,14 +9,14 @@ from typing import Optional, Sequence
 
 import numpy as np
 
-from .hip import BINARY, DTYPE_BY_NAME, NP_DTYPE, REDUCE, SCALAR, UNARY
+from .hip import BINARY, DTYPE_BY_NAME, NP_DTYPE, REDUCE, SCALAR, SCAN_FORM, UNARY
 
 _LIB = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "librt_host.so")
 if not os.path.exists(_LIB):
     raise ImportError(f"{_LIB} is missing: build it with `python -m rtensors_amd.build`")
 _h = C.CDLL(_LIB)
 _h.rth_last_error.restype = C.c_char_p
-for _n in ("rth_backend_destroy", "rth_free"):
+for _n in ("rth_backend_destroy", "rth_free", "rth_packed8_free"):
     getattr(_h, _n).restype = None
     getattr(_h, _n).argtypes = [C.c_void_p]
 
@@ -280,6 +280,36 @@ class Tensor:
     def argmax(self): return self.reduce("argmax")
     def argmin(self): return self.reduce("argmin")
 
+    def gated_scan(self, gate, axis, form="linear", state=None, reset=None, want_last=False):
+        """h[t] = a * h[t - 1] + b along `axis`, this tensor being x: form "linear" (a = gate, b = x) or "sigmoid" (a = sigmoid(gate),
+        b = (1 - a) * x).  state: the shape without the axis; reset: bool, the axes up to and including `axis`, true where the state before
+        the step does not count.  Returns h, or (h, the state after the last step)."""
+        p, last = C.c_void_p(), C.c_void_p()
+        _ck(_h.rth_gated_scan(self._p, gate._p, C.c_uint64(axis), SCAN_FORM[form], state._p if state is not None else None,
+                              reset._p if reset is not None else None, C.byref(p), C.byref(last) if want_last else None))
+        h = Tensor(p, self.backend)
+        return (h, Tensor(last, self.backend)) if want_last else h
+
+    def pack8(self):
+        """The elements in 8 bits, one exponent for each 32 of them (a `Packed8`)."""
+        p = C.c_void_p()
+        _ck(_h.rth_pack8(self._p, C.byref(p)))
+        return Packed8(p, self.backend)
+
+    def unary_pack8(self, op):
+        """(op(self), the 8-bit form of self) in one pass; op is sigmoid, silu or tanh."""
+        p, q = C.c_void_p(), C.c_void_p()
+        _ck(_h.rth_unary_pack8(self._p, UNARY[op], C.byref(p), C.byref(q)))
+        return Tensor(p, self.backend), Packed8(q, self.backend)
+
+    def unary_backward_pack8(self, op, packed):
+        """self * op'(packed), self being the upstream gradient."""
+        return self._new(_h.rth_unary_backward_pack8, UNARY[op], packed._p)
+
+    def matmul_backward_pack8(self, packed):
+        """packed^T @ self over the last two dims: the gradient of w in y = x @ w, x held in 8 bits and self the gradient of y."""
+        return self._new(_h.rth_matmul_backward_pack8, packed._p)
+
     def fill(self, v): _ck(_h.rth_fill(self._p, C.c_double(v)))
 
     def get(self, idx):
@@ -306,6 +336,26 @@ class Tensor:
         r = C.c_int(0)
         _ck(_h.rth_equals(self._p, o._p, C.byref(r)))
         return bool(r.value)
+
+
+class Packed8:
+    """A tensor's elements held in 8 bits (rt::Packed8)."""
+
+    def __init__(self, handle, backend: Backend):
+        self._p, self.backend = handle, backend
+
+    def __del__(self):
+        try:
+            if self._p:
+                _h.rth_packed8_free(self._p)
+        except Exception:
+            pass
+        self._p = None
+
+    def unpack8(self) -> Tensor:
+        p = C.c_void_p()
+        _ck(_h.rth_unpack8(self.backend._p, self._p, C.byref(p)))
+        return Tensor(p, self.backend)
 
 
 class Expr:
@@ -375,3 +425,15 @@ def linear_step(x: Tensor, w: Tensor, target: Tensor, lr: float, seed_with_loss:
     pl, pg = C.c_void_p(), C.c_void_p()
     _ck(_h.rth_linear_step(x._p, w._p, target._p, C.c_double(lr), 1 if seed_with_loss else 0, C.byref(pl), C.byref(pg)))
     return Tensor(pl, x.backend), Tensor(pg, x.backend)
+
+
+def gated_layer_step(x: Tensor, w_gate: Tensor, w_value: Tensor, w_out: Tensor, target: Tensor, lr: float, reset: Optional[Tensor] = None,
+                     packed: bool = False, seed_with_loss: bool = True):
+    """A gated recurrent layer over rows of tokens: h = gated_scan(silu(x @ w_value), x @ w_gate) along the tokens (form "sigmoid"),
+    loss = mean_l1_loss(h @ w_out, target); backward; SGD(lr) on the three weights in place.  reset: bool (tokens), true where a document
+    starts.  packed: the tape keeps its activations in 8 bits.  Returns (loss, [d_w_gate, d_w_value, d_w_out], bytes the tape kept)."""
+    pl, kept = C.c_void_p(), C.c_uint64(0)
+    grads = (C.c_void_p * 3)()
+    _ck(_h.rth_gated_layer_step(x._p, w_gate._p, w_value._p, w_out._p, target._p, reset._p if reset is not None else None, C.c_double(lr), 1 if packed else 0,
+                                1 if seed_with_loss else 0, C.byref(pl), grads, C.byref(kept)))
+    return Tensor(pl, x.backend), [Tensor(C.c_void_p(g), x.backend) for g in grads], kept.value

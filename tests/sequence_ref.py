@@ -63,8 +63,8 @@ def scan_backward(form, gate, x, h, dh, state=None, reset=None, dlast=None):
         d = dh[:, t].astype(W)
         D[:, t], M[:, t] = d + carry, np.abs(d) + m
         S[:, t] = s + M[:, t]
-        carry = np.where(cut[:, t], 0, a[:, t] * D[:, t])
-        m, s = np.where(cut[:, t], 0, np.abs(a[:, t]) * M[:, t]), np.where(cut[:, t], 0, np.abs(a[:, t]) * S[:, t])
+        carry = np.where(none[:, t], 0, a[:, t] * D[:, t])
+        m, s = np.where(none[:, t], 0, np.abs(a[:, t]) * M[:, t]), np.where(none[:, t], 0, np.abs(a[:, t]) * S[:, t])
     first = np.zeros((outer, 1, inner), dtype=W) if state is None else state.astype(W)[:, None]
     before = np.concatenate([first, h.astype(W)[:, :-1]], axis=1) if steps else h.astype(W)
     before = np.where(none, 0, before)
