@@ -71,11 +71,29 @@ def _pl(buf):
     return (None, 0) if buf is None else (buf.ptr, buf.len)
 
 
-class HipBuf:
-    """Owns `len` elements of `dtype` in device memory; returned to the context's allocator when dropped."""
+def _same(what: str, dtype: int, *bufs):
+    for b in bufs:
+        if b is not None and b.dtype != dtype:
+            raise TensorError(2, f"{what}: operands of different dtypes")
+
+
+def _code(what: str, dtype: int, *bufs):
+    for b in bufs:
+        if b is not None and b.dtype != dtype:
+            raise TensorError(2, f"{what}: an operand has dtype code {b.dtype}, expected {dtype}")
+
+
+class HipView:
+    """`len` elements of `dtype` in device memory that something else owns."""
+    __slots__ = ("backend", "ptr", "len", "dtype")
 
     def __init__(self, backend: "Hip", ptr: int, length: int, dtype: int):
         self.backend, self.ptr, self.len, self.dtype = backend, ptr, length, dtype
+
+
+class HipBuf(HipView):
+    """Owns `len` elements of `dtype` in device memory; returned to the context's allocator when dropped."""
+    __slots__ = ("__weakref__",)
 
     def __del__(self):
         try:
@@ -129,11 +147,11 @@ class Hip:
         _check(lib.rt_alloc_from_slice(self._ctx, dtype, src.ctypes.data_as(C.c_void_p), src.size, C.byref(p)))
         return HipBuf(self, p.value, src.size, dtype)
 
-    def borrow(self, ptr: int, length: int, dtype: int) -> HipBuf:
+    def borrow(self, ptr: int, length: int, dtype: int) -> HipView:
         """`length` elements of device memory that something else owns (a buffer of another library, a part of a larger one): usable in
         every call, never freed from here.  The owner keeps it alive, and orders its own work on it against this context's stream
         (`sync()`, or its own wait, where another stream wrote it)."""
-        return HipBuf(None, ptr, length, dtype)
+        return HipView(self, ptr, length, dtype)
 
     def copy_from_slice(self, dst: HipBuf, src: np.ndarray):
         src = np.ascontiguousarray(src, dtype=NP_DTYPE[dst.dtype]).reshape(-1)
@@ -319,16 +337,16 @@ class Hip:
                    reset: HipBuf = None, last: HipBuf = None):
         """rt_gated_scan: h[t] = a[t] * h[t - 1] + b[t] along `steps` of (outer, steps, inner); form "linear" (a = gate, b = x) or "sigmoid"
         (a = sigmoid(gate), b = (1 - a) * x).  state / last: (outer, inner); reset: bool (outer, steps)."""
-        self._same("gated scan", gate.dtype, x, h, state, last)
-        self._code("gated scan", BOOL, reset)
+        _same("gated scan", gate.dtype, x, h, state, last)
+        _code("gated scan", BOOL, reset)
         _check(lib.rt_gated_scan(self._ctx, gate.dtype, SCAN_FORM[form], *_pl(gate), *_pl(x), *_pl(state), *_pl(reset), *_pl(h), *_pl(last),
                                  outer, steps, inner))
 
     def gated_scan_backward(self, form: str, gate: HipBuf, x: HipBuf, h: HipBuf, dh: HipBuf, dgate: HipBuf, dx: HipBuf, outer: int, steps: int,
                             inner: int, state: HipBuf = None, reset: HipBuf = None, dlast: HipBuf = None, dstate: HipBuf = None):
         """rt_gated_scan_backward: the gradients of gate, x and state; x may be None for form "linear"."""
-        self._same("gated scan backward", gate.dtype, x, h, dh, dgate, dx, state, dlast, dstate)
-        self._code("gated scan backward", BOOL, reset)
+        _same("gated scan backward", gate.dtype, x, h, dh, dgate, dx, state, dlast, dstate)
+        _code("gated scan backward", BOOL, reset)
         _check(lib.rt_gated_scan_backward(self._ctx, gate.dtype, SCAN_FORM[form], *_pl(gate), *_pl(x), *_pl(h), *_pl(state), *_pl(reset), *_pl(dh),
                                           *_pl(dlast), *_pl(dgate), *_pl(dx), *_pl(dstate), outer, steps, inner))
 
@@ -337,10 +355,10 @@ class Hip:
         """The same with x and h as (codes, exps) pairs of their 8-bit form; x8 may be None for form "linear"."""
         xc, xe = x8 if x8 is not None else (None, None)
         hc, he = h8
-        self._same("gated scan backward", gate.dtype, dh, dgate, dx, state, dlast, dstate)
-        self._code("gated scan backward", BOOL, reset)
-        self._code("gated scan backward", I8, xc, hc)
-        self._code("gated scan backward", U8, xe, he)
+        _same("gated scan backward", gate.dtype, dh, dgate, dx, state, dlast, dstate)
+        _code("gated scan backward", BOOL, reset)
+        _code("gated scan backward", I8, xc, hc)
+        _code("gated scan backward", U8, xe, he)
         _check(lib.rt_gated_scan_backward_packed8(self._ctx, gate.dtype, SCAN_FORM[form], *_pl(gate), *_pl(xc), *_pl(xe), *_pl(hc), *_pl(he), *_pl(state),
                                                   *_pl(reset), *_pl(dh), *_pl(dlast), *_pl(dgate), *_pl(dx), *_pl(dstate), outer, steps, inner))
 
@@ -349,47 +367,35 @@ class Hip:
         return self.alloc_uninit(I8, length), self.alloc_uninit(U8, -(-length // PACK8_GROUP))
 
     def pack8(self, src: HipBuf, start: int, length: int, codes: HipBuf, exps: HipBuf):
-        self._code("pack8", I8, codes)
-        self._code("pack8", U8, exps)
+        _code("pack8", I8, codes)
+        _code("pack8", U8, exps)
         _check(lib.rt_pack8(self._ctx, src.dtype, *_pl(src), start, length, *_pl(codes), *_pl(exps)))
 
     def unpack8(self, codes: HipBuf, exps: HipBuf, length: int, dst: HipBuf):
-        self._code("unpack8", I8, codes)
-        self._code("unpack8", U8, exps)
+        _code("unpack8", I8, codes)
+        _code("unpack8", U8, exps)
         _check(lib.rt_unpack8(self._ctx, dst.dtype, *_pl(codes), *_pl(exps), length, *_pl(dst)))
 
     def pack8_unary(self, op: str, src: HipBuf, start: int, length: int, dst: HipBuf, codes: HipBuf, exps: HipBuf):
         """dst = op(src run) and the 8-bit form of the run in one pass; op is sigmoid, silu or tanh."""
-        self._same("pack8 unary", src.dtype, dst)
-        self._code("pack8 unary", I8, codes)
-        self._code("pack8 unary", U8, exps)
+        _same("pack8 unary", src.dtype, dst)
+        _code("pack8 unary", I8, codes)
+        _code("pack8 unary", U8, exps)
         _check(lib.rt_pack8_unary(self._ctx, src.dtype, UNARY[op], *_pl(src), start, length, *_pl(dst), *_pl(codes), *_pl(exps)))
 
     def pack8_unary_backward(self, op: str, codes: HipBuf, exps: HipBuf, upstream: HipBuf, length: int, dst: HipBuf):
         """dst = upstream * op'(restored)."""
-        self._same("pack8 unary backward", dst.dtype, upstream)
-        self._code("pack8 unary backward", I8, codes)
-        self._code("pack8 unary backward", U8, exps)
+        _same("pack8 unary backward", dst.dtype, upstream)
+        _code("pack8 unary backward", I8, codes)
+        _code("pack8 unary backward", U8, exps)
         _check(lib.rt_pack8_unary_backward(self._ctx, dst.dtype, UNARY[op], *_pl(codes), *_pl(exps), *_pl(upstream), length, *_pl(dst)))
 
     def pack8_matmul_backward(self, codes: HipBuf, exps: HipBuf, upstream: HipBuf, dst: HipBuf, b: int, m: int, k: int, n: int):
         """dst[b] (k x n) = restored[b]^T * upstream[b]: the weight gradient of a projection whose input (b, m, k) is held in 8 bits."""
-        self._same("pack8 matmul backward", dst.dtype, upstream)
-        self._code("pack8 matmul backward", I8, codes)
-        self._code("pack8 matmul backward", U8, exps)
+        _same("pack8 matmul backward", dst.dtype, upstream)
+        _code("pack8 matmul backward", I8, codes)
+        _code("pack8 matmul backward", U8, exps)
         _check(lib.rt_pack8_matmul_backward(self._ctx, dst.dtype, *_pl(codes), *_pl(exps), *_pl(upstream), *_pl(dst), b, m, k, n))
-
-    @staticmethod
-    def _same(what: str, dtype: int, *bufs):
-        for b in bufs:
-            if b is not None and b.dtype != dtype:
-                raise TensorError(2, f"{what}: operands of different dtypes")
-
-    @staticmethod
-    def _code(what: str, dtype: int, *bufs):
-        for b in bufs:
-            if b is not None and b.dtype != dtype:
-                raise TensorError(2, f"{what}: an operand has dtype code {b.dtype}, expected {dtype}")
 
     # ---- timing -----------------------------------------------------------------------------------------------------------
     def event(self):
