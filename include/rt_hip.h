@@ -332,8 +332,11 @@ int32_t rt_matmul(rt_ctx* ctx, int32_t dtype,
  * `state` and `last` are (outer, inner); `reset` (RT_BOOL, non-zero = a new document starts at this step) is (outer, steps); each of
  * the three may be null.  last = h[steps - 1]; for steps = 0 the state (zeros when null).  steps = 1 with state and last is the
  * single-token form of serving; last may be the state buffer itself.  h may be x itself or gate itself; any other overlap of an
- * output is RT_E_INVALID.  The state is held and summed in the tensor's own dtype (f32 / f64); how the steps are grouped for the
- * sum depends on the sizes alone, so equal calls give equal bits.
+ * output is RT_E_INVALID.  The state is held and summed in the tensor's own dtype (f32 / f64).  Long runs are cut into stretches that are
+ * summed apart and joined by the products of their factors; how they are cut depends on the sizes (and the device), so equal calls give
+ * equal bits.  A product that leaves the range upwards makes its stretch run step by step; one that falls below the smallest normal
+ * number loses what of an earlier state it carries (less than 2^-126 of that state, 2^-1022 for f64), and 0 times an infinite state is
+ * NaN.  Workspace: about 1 / 100 of the operands where a run is cut over several blocks, kept by the context and grown on demand.
  *
  * rt_gated_scan_backward: from dh (gradient of h) and dlast (gradient of last, null = 0), with a[t] the factor of p[t]:
  *     D[t] = dh[t] + (reset[t + 1] ? 0 : a[t + 1] * D[t + 1]),   D[steps - 1] = dh[steps - 1] + dlast

@@ -646,6 +646,103 @@ impl Hip {
         })
     }
 
+    /// Gated linear recurrence along `steps` of `(outer, steps, inner)` runs: `h[t] = a * h[t - 1] + b`, `form` one of `ffi::RT_SCAN_*`
+    /// (LINEAR: `a = gate, b = x`; SIGMOID: `a = sigmoid(gate), b = (1 - a) * x`).  `state` and `last` are `(outer, inner)`, `reset`
+    /// is `(outer, steps)`; each may be left out.
+    #[allow(clippy::too_many_arguments)]
+    pub fn gated_scan<T: WeightValue>(&self, form: i32, gate: &HipBuf<T>, x: &HipBuf<T>, state: Option<&HipBuf<T>>,
+        reset: Option<&HipBuf<bool>>, h: &mut HipBuf<T>, last: Option<&mut HipBuf<T>>, sizes: (usize, usize, usize))
+        -> Result<(), TensorError> {
+        let (sp, sl) = opt(state);
+        let (rp, rl) = opt(reset);
+        let (lp, ll) = opt(last.as_deref());
+        check(unsafe {
+            ffi::rt_gated_scan(self.raw(), dt::<T>(), form, gate.ptr, gate.len as u64, x.ptr, x.len as u64, sp, sl, rp, rl, h.ptr,
+                h.len as u64, lp, ll, sizes.0 as u64, sizes.1 as u64, sizes.2 as u64)
+        })
+    }
+
+    /// The gradients of `gate`, `x` and `state` of `gated_scan` from those of `h` and `last`.  `x` is needed for SIGMOID alone.
+    #[allow(clippy::too_many_arguments)]
+    pub fn gated_scan_backward<T: WeightValue>(&self, form: i32, gate: &HipBuf<T>, x: Option<&HipBuf<T>>, h: &HipBuf<T>,
+        state: Option<&HipBuf<T>>, reset: Option<&HipBuf<bool>>, dh: &HipBuf<T>, dlast: Option<&HipBuf<T>>, dgate: &mut HipBuf<T>,
+        dx: &mut HipBuf<T>, dstate: Option<&mut HipBuf<T>>, sizes: (usize, usize, usize)) -> Result<(), TensorError> {
+        let (xp, xl) = opt(x);
+        let (sp, sl) = opt(state);
+        let (rp, rl) = opt(reset);
+        let (dlp, dll) = opt(dlast);
+        let (dsp, dsl) = opt(dstate.as_deref());
+        check(unsafe {
+            ffi::rt_gated_scan_backward(self.raw(), dt::<T>(), form, gate.ptr, gate.len as u64, xp, xl, h.ptr, h.len as u64, sp, sl, rp,
+                rl, dh.ptr, dh.len as u64, dlp, dll, dgate.ptr, dgate.len as u64, dx.ptr, dx.len as u64, dsp, dsl, sizes.0 as u64,
+                sizes.1 as u64, sizes.2 as u64)
+        })
+    }
+
+    /// As `gated_scan_backward`, with `x` and `h` as the codes and exponents of their 8-bit form.
+    #[allow(clippy::too_many_arguments)]
+    pub fn gated_scan_backward_packed8<T: WeightValue>(&self, form: i32, gate: &HipBuf<T>, x: Option<(&HipBuf<i8>, &HipBuf<u8>)>,
+        h: (&HipBuf<i8>, &HipBuf<u8>), state: Option<&HipBuf<T>>, reset: Option<&HipBuf<bool>>, dh: &HipBuf<T>,
+        dlast: Option<&HipBuf<T>>, dgate: &mut HipBuf<T>, dx: &mut HipBuf<T>, dstate: Option<&mut HipBuf<T>>,
+        sizes: (usize, usize, usize)) -> Result<(), TensorError> {
+        let (xcp, xcl) = opt(x.map(|p| p.0));
+        let (xep, xel) = opt(x.map(|p| p.1));
+        let (sp, sl) = opt(state);
+        let (rp, rl) = opt(reset);
+        let (dlp, dll) = opt(dlast);
+        let (dsp, dsl) = opt(dstate.as_deref());
+        check(unsafe {
+            ffi::rt_gated_scan_backward_packed8(self.raw(), dt::<T>(), form, gate.ptr, gate.len as u64, xcp, xcl, xep, xel, h.0.ptr,
+                h.0.len as u64, h.1.ptr, h.1.len as u64, sp, sl, rp, rl, dh.ptr, dh.len as u64, dlp, dll, dgate.ptr, dgate.len as u64,
+                dx.ptr, dx.len as u64, dsp, dsl, sizes.0 as u64, sizes.1 as u64, sizes.2 as u64)
+        })
+    }
+
+    /// `len` elements from `start` in 8 bits: `codes` (one each) and `exps` (one for each `ffi::RT_PACK8_GROUP` of them).
+    pub fn pack8<T: WeightValue>(&self, src: &HipBuf<T>, start: usize, len: usize, codes: &mut HipBuf<i8>, exps: &mut HipBuf<u8>)
+        -> Result<(), TensorError> {
+        check(unsafe {
+            ffi::rt_pack8(self.raw(), dt::<T>(), src.ptr, src.len as u64, start as u64, len as u64, codes.ptr, codes.len as u64,
+                exps.ptr, exps.len as u64)
+        })
+    }
+
+    /// The values that codes and exponents stand for.
+    pub fn unpack8<T: WeightValue>(&self, codes: &HipBuf<i8>, exps: &HipBuf<u8>, len: usize, dst: &mut HipBuf<T>) -> Result<(), TensorError> {
+        check(unsafe {
+            ffi::rt_unpack8(self.raw(), dt::<T>(), codes.ptr, codes.len as u64, exps.ptr, exps.len as u64, len as u64, dst.ptr,
+                dst.len as u64)
+        })
+    }
+
+    /// `dst = op(src run)` and the run's 8-bit form in one pass; `op` is `ffi::RT_U_SIGMOID`, `RT_U_SILU` or `RT_U_TANH`.
+    #[allow(clippy::too_many_arguments)]
+    pub fn pack8_unary<T: WeightValue>(&self, op: i32, src: &HipBuf<T>, start: usize, len: usize, dst: &mut HipBuf<T>,
+        codes: &mut HipBuf<i8>, exps: &mut HipBuf<u8>) -> Result<(), TensorError> {
+        check(unsafe {
+            ffi::rt_pack8_unary(self.raw(), dt::<T>(), op, src.ptr, src.len as u64, start as u64, len as u64, dst.ptr, dst.len as u64,
+                codes.ptr, codes.len as u64, exps.ptr, exps.len as u64)
+        })
+    }
+
+    /// `dst = upstream * op'(restored)`.
+    pub fn pack8_unary_backward<T: WeightValue>(&self, op: i32, codes: &HipBuf<i8>, exps: &HipBuf<u8>, upstream: &HipBuf<T>, len: usize,
+        dst: &mut HipBuf<T>) -> Result<(), TensorError> {
+        check(unsafe {
+            ffi::rt_pack8_unary_backward(self.raw(), dt::<T>(), op, codes.ptr, codes.len as u64, exps.ptr, exps.len as u64, upstream.ptr,
+                upstream.len as u64, len as u64, dst.ptr, dst.len as u64)
+        })
+    }
+
+    /// `dst[b] = restored[b]^T * upstream[b]`: the weight gradient of a projection whose input `(b, m, k)` is held in 8 bits.
+    pub fn pack8_matmul_backward<T: WeightValue>(&self, codes: &HipBuf<i8>, exps: &HipBuf<u8>, upstream: &HipBuf<T>, dst: &mut HipBuf<T>,
+        sizes: (usize, usize, usize, usize)) -> Result<(), TensorError> {
+        check(unsafe {
+            ffi::rt_pack8_matmul_backward(self.raw(), dt::<T>(), codes.ptr, codes.len as u64, exps.ptr, exps.len as u64, upstream.ptr,
+                upstream.len as u64, dst.ptr, dst.len as u64, sizes.0 as u64, sizes.1 as u64, sizes.2 as u64, sizes.3 as u64)
+        })
+    }
+
     /// Dense row-major copy of a view in one launch (`view_to_contiguous`, core/tensor.rs:299-325, issues one
     /// `copy_range_within` per contiguous run).
     pub fn gather<T: TensorValue>(&self, src: &HipBuf<T>, meta: &MetaTensor, dst: &mut HipBuf<T>) -> Result<(), TensorError> {
@@ -655,6 +752,11 @@ impl Hip {
                 dst.len as u64)
         })
     }
+}
+
+/// Pointer and length of an operand that may be left out.
+fn opt<T: TensorValue>(b: Option<&HipBuf<T>>) -> (*mut c_void, u64) {
+    b.map_or((std::ptr::null_mut(), 0), |b| (b.ptr, b.len as u64))
 }
 
 /// One step of `Hip::fused_chain`.

@@ -34,6 +34,9 @@ pub const RT_CHAIN_BINARY: i32 = 2;
 pub const RT_CHAIN_BINARY_REV: i32 = 3;
 pub const RT_CHAIN_MAX_STEPS: i32 = 8;
 pub const RT_CHAIN_MAX_INPUTS: i32 = 4;
+pub const RT_SCAN_LINEAR: i32 = 0;
+pub const RT_SCAN_SIGMOID: i32 = 1;
+pub const RT_PACK8_GROUP: i32 = 32;
 
 // rt_status
 pub const RT_OK: i32 = 0;

@@ -280,7 +280,8 @@ __device__ __forceinline__ uint32_t line_of_block(const Chain& ch) {
     const uint32_t x = b % 8;
     return (b / 8 + (uint32_t)((uint64_t)x * ch.lines / 8)) % ch.lines;
 }
-// The block's tile among those of its line (one that is not there for the blocks too many); whoever takes the last one leaves the counter as the next launch needs it.
+// The block's tile among those of its line (one that is not there for the blocks too many); whoever takes the last one leaves the counter
+// as the next launch needs it.
 template <class T, int W, int LN> __device__ __forceinline__ uint32_t take_tile(const Chain& ch, uint32_t line, JoinRoom<T, W, LN>& room) {
     if (ch.tiles == 1) return 0;
     if (threadIdx.x == 0) {
@@ -921,7 +922,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
     }
 }
 
-// dst = src, or zeros: the states of a run of no steps
+// dst = src, or zeros: the states of a run of no steps, and copies of states
 template <class T> __global__ void scan_no_steps_kernel(const T* src, T* dst, uint64_t n) {
     const uint64_t i = (uint64_t)blockIdx.x * kSBlock + threadIdx.x;
     if (i < n) dst[i] = src ? src[i] : (T)0;
@@ -1063,6 +1064,17 @@ template <class T, class S> int32_t backward_typed(rt_ctx* ctx, int form, const 
     return form == RT_SCAN_LINEAR ? backward_form<T, RT_SCAN_LINEAR, S>(ctx, a) : backward_form<T, RT_SCAN_SIGMOID, S>(ctx, a);
 }
 
+// A state that is replaced in place: its first tile reads it and its last tile writes it, and where a reset lies between them the last one
+// does not wait for the first.  The state is then read from a copy.
+template <class T> int32_t apart(rt_ctx* ctx, const void** in, const void* out, const void* reset, uint64_t outer, uint64_t steps, uint64_t inner) {
+    if (!*in || *in != out || !reset || by_columns(steps, inner)) return RT_OK;
+    void* copy = nullptr;
+    RT_TRY(rt_scratch(ctx, outer * inner * sizeof(T), &copy));
+    RT_TRY(no_steps<T>(ctx, *in, copy, outer * inner));
+    *in = copy;
+    return RT_OK;
+}
+
 // ---- argument checks ---------------------------------------------------------------------------------------------------------------
 struct Operand {
     const char* name;
@@ -1125,10 +1137,12 @@ int32_t check_backward(const BackwardCall& c) {
 template <class T, class S> int32_t run_backward(const BackwardCall& c, S x, S h) {
     if (c.steps == 0) return no_steps<T>(c.ctx, c.dlast.p, const_cast<void*>(c.dstate.p), c.outer * c.inner);
     if (c.outer * c.inner == 0) return RT_OK;
+    const void* dlast = c.dlast.p;
+    RT_TRY(apart<T>(c.ctx, &dlast, c.dstate.p, c.reset.p, c.outer, c.steps, c.inner));
     BackArgs<T, S> a;
     a.gate = (const T*)c.gate.p; a.x = x; a.h = h;
     a.state = (const T*)c.state.p; a.reset = (const uint8_t*)c.reset.p;
-    a.dh = (const T*)c.dh.p; a.dlast = (const T*)c.dlast.p;
+    a.dh = (const T*)c.dh.p; a.dlast = (const T*)dlast;
     a.dgate = (T*)const_cast<void*>(c.dgate.p); a.dx = (T*)const_cast<void*>(c.dx.p); a.dstate = (T*)const_cast<void*>(c.dstate.p);
     a.outer = c.outer; a.steps = c.steps; a.inner = c.inner;
     return backward_typed<T, S>(c.ctx, c.form, a);
@@ -1154,6 +1168,7 @@ extern "C" int32_t rt_gated_scan(rt_ctx* ctx, int32_t dtype, int32_t form, const
     CtxGuard g(ctx);
     if (steps == 0) return dtype == RT_F32 ? no_steps<float>(ctx, state, last, cols) : no_steps<double>(ctx, state, last, cols);
     if (cols == 0) return RT_OK;
+    RT_TRY(dtype == RT_F32 ? apart<float>(ctx, &state, last, reset, outer, steps, inner) : apart<double>(ctx, &state, last, reset, outer, steps, inner));
     if (dtype == RT_F32) {
         const ScanArgs<float> a = {(const float*)gate, (const float*)x, (const float*)state, (const uint8_t*)reset, (float*)h, (float*)last, outer, steps, inner};
         return forward_typed<float>(ctx, form, a);
