@@ -304,6 +304,7 @@ class Tensor {
     // this * op'(restored): this is the upstream gradient
     Tensor unary_backward_pack8(int op, const Packed8& p) const {
         if (p.shape != meta_.shape) throw TensorError(ErrorKind::InvalidShape, "The upstream gradient has another shape than the packed activation");
+        if (p.dtype != dtype()) throw TensorError(ErrorKind::UnsupportedOperation, "The upstream gradient has another dtype than the packed activation");
         const Tensor t = whole();
         Tensor r = like_row_major();
         backend_->pack8_unary_backward(op, *p.codes, *p.exps, *t.buf_, size(), *r.buf_);
@@ -314,6 +315,7 @@ class Tensor {
         const size_t r = rank();
         if (r < 2 || x.shape.size() != r || !std::equal(x.shape.begin(), x.shape.end() - 1, meta_.shape.begin()))
             throw TensorError(ErrorKind::InvalidShape, "The upstream gradient does not fit the packed input of the matmul");
+        if (x.dtype != dtype()) throw TensorError(ErrorKind::UnsupportedOperation, "The upstream gradient has another dtype than the packed input of the matmul");
         uint64_t b = 1;
         for (size_t i = 0; i + 2 < r; ++i) b *= meta_.shape[i];
         const uint64_t m = meta_.shape[r - 2], n = meta_.shape[r - 1], k = x.shape[r - 1];

@@ -71,7 +71,9 @@ def test_errors(be):
                        (lambda: x.gated_scan(z(3, 4, 5), 1, reset=z(3, 5, dt="bool")), "InvalidShape"),
                        (lambda: z(3, 4, dt="i32").gated_scan(z(3, 4, dt="i32"), 0), "UnsupportedOperation"), (lambda: z(3, dt="i32").pack8(), "UnsupportedOperation"),
                        (lambda: x.unary_pack8("relu"), "UnsupportedOperation"), (lambda: z(3, 4).unary_backward_pack8("silu", x.pack8()), "InvalidShape"),
-                       (lambda: z(3, 6, 5).matmul_backward_pack8(x.pack8()), "InvalidShape"), (lambda: z(4, 5).matmul_backward_pack8(x.pack8()), "InvalidShape")):
+                       (lambda: z(3, 6, 5).matmul_backward_pack8(x.pack8()), "InvalidShape"), (lambda: z(4, 5).matmul_backward_pack8(x.pack8()), "InvalidShape"),
+                       (lambda: z(3, 4, 5, dt="f64").unary_backward_pack8("silu", x.pack8()), "UnsupportedOperation"),
+                       (lambda: z(3, 4, 5, dt="f64").matmul_backward_pack8(x.pack8()), "UnsupportedOperation")):
         with pytest.raises(T.TensorError) as e:
             call()
         assert e.value.kind == kind, (e.value.kind, str(e.value))
