@@ -255,7 +255,11 @@ int32_t rt_chain_room(rt_ctx* ctx, int which, size_t bytes, void** out) {
         }
         c.bytes = cap;
         ctx->device_allocs += 1;
-        RT_TRY(rt_chain_clear(ctx, which));
+        const int32_t rc = rt_chain_clear(ctx, which);
+        if (rc != RT_OK) {                                       // counters and tags that may hold anything are not kept
+            c.bytes = 0;
+            return rc;
+        }
     }
     *out = c.p;
     return RT_OK;
