@@ -159,16 +159,25 @@ __global__ __launch_bounds__(kPBlock) void unpack8_kernel(const int8_t* __restri
     }
 }
 
+// Elements of one launch, whole groups and whole blocks: the lanes of a grid are numbered in 32 bits.
+constexpr uint64_t kMostOfLaunch = 1ull << 33;
+
 template <class T, int OP> int32_t pack_launch(rt_ctx* ctx, const T* src, T* dst, void* codes, void* exps, uint64_t len) {
-    const uint64_t blocks = (len + kPBlockElems - 1) / kPBlockElems;
-    hipLaunchKernelGGL((pack8_kernel<T, OP>), dim3((uint32_t)blocks), dim3(kPBlock), 0, ctx->stream, src, dst, (int8_t*)codes, (uint8_t*)exps, len);
-    RT_HIP(hipGetLastError());
+    for (uint64_t at = 0; at < len; at += kMostOfLaunch) {
+        const uint64_t n = len - at < kMostOfLaunch ? len - at : kMostOfLaunch;
+        hipLaunchKernelGGL((pack8_kernel<T, OP>), dim3((uint32_t)((n + kPBlockElems - 1) / kPBlockElems)), dim3(kPBlock), 0, ctx->stream, src + at,
+                           OP == kNoOp ? dst : dst + at, (int8_t*)codes + at, (uint8_t*)exps + at / kP8Group, n);
+        RT_HIP(hipGetLastError());
+    }
     return RT_OK;
 }
 template <class T, int OP> int32_t unpack_launch(rt_ctx* ctx, const void* codes, const void* exps, const T* up, T* dst, uint64_t len) {
-    const uint64_t blocks = (len + kPBlockElems - 1) / kPBlockElems;
-    hipLaunchKernelGGL((unpack8_kernel<T, OP>), dim3((uint32_t)blocks), dim3(kPBlock), 0, ctx->stream, (const int8_t*)codes, (const uint8_t*)exps, up, dst, len);
-    RT_HIP(hipGetLastError());
+    for (uint64_t at = 0; at < len; at += kMostOfLaunch) {
+        const uint64_t n = len - at < kMostOfLaunch ? len - at : kMostOfLaunch;
+        hipLaunchKernelGGL((unpack8_kernel<T, OP>), dim3((uint32_t)((n + kPBlockElems - 1) / kPBlockElems)), dim3(kPBlock), 0, ctx->stream,
+                           (const int8_t*)codes + at, (const uint8_t*)exps + at / kP8Group, OP == kNoOp ? up : up + at, dst + at, n);
+        RT_HIP(hipGetLastError());
+    }
     return RT_OK;
 }
 template <class T> int32_t pack_typed(rt_ctx* ctx, int op, const T* src, T* dst, void* codes, void* exps, uint64_t len) {

@@ -40,6 +40,7 @@ template <class T> struct ScanArgs {
     const uint8_t* reset;
     T *h, *last;
     uint64_t outer, steps, inner;
+    uint64_t col0;           // first column of a launch with one lane a column
 };
 template <class T, class S> struct BackArgs {
     const T* gate;
@@ -49,12 +50,13 @@ template <class T, class S> struct BackArgs {
     const T *dh, *dlast;
     T *dgate, *dx, *dstate;
     uint64_t outer, steps, inner;
+    uint64_t col0;
 };
 
 // One lane per column, the steps one after the other.
 template <class T, int FORM>
 __global__ __launch_bounds__(kSBlock) void scan_columns_kernel(ScanArgs<T> a) {
-    const uint64_t col = (uint64_t)blockIdx.x * kSBlock + threadIdx.x;
+    const uint64_t col = a.col0 + (uint64_t)blockIdx.x * kSBlock + threadIdx.x;
     if (col >= a.outer * a.inner) return;
     const uint64_t o = col / a.inner, i = col - o * a.inner;
     T p = a.state ? a.state[col] : (T)0;
@@ -77,7 +79,7 @@ __global__ __launch_bounds__(kSBlock) void scan_columns_kernel(ScanArgs<T> a) {
 
 template <class T, int FORM, class S>
 __global__ __launch_bounds__(kSBlock) void scan_backward_columns_kernel(BackArgs<T, S> a) {
-    const uint64_t col = (uint64_t)blockIdx.x * kSBlock + threadIdx.x;
+    const uint64_t col = a.col0 + (uint64_t)blockIdx.x * kSBlock + threadIdx.x;
     if (col >= a.outer * a.inner) return;
     const uint64_t o = col / a.inner, i = col - o * a.inner;
     T carry = a.dlast ? a.dlast[col] : (T)0;          // a[t + 1] * D[t + 1]
@@ -124,6 +126,7 @@ struct Chain {
     uint64_t* words;
     uint32_t tiles;          // along the steps
     uint32_t lines;          // sets of columns that are chained on their own
+    uint32_t line0;          // the first of them in the operands: a launch takes no more than its lanes can be numbered for
     uint32_t epoch;          // the launch's number, 30 bits
     uint32_t rounds;         // blocks a line gets: `tiles`, or the next multiple of 8
 };
@@ -378,15 +381,18 @@ __device__ __forceinline__ uint64_t reset_bits(const uint8_t* flags, int64_t str
     RT_PIN(rcuts);                      \
     RT_PIN(rrow)
 
+// Every wave of the first tile has its state before any of them hands one on: the last tile may write over the state's buffer.
+#define RT_PIN_LANE(v) asm volatile("" : "+v"(v))
+
 // W waves of 64 columns, L steps each, in registers.  A wave that ends before its L steps, and lanes behind the last column, load what
 // the last step and the last column hold, and neither use nor store it.
 template <class T, int FORM, int W, int L, bool ALIGNED>
 __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain ch, uint32_t col_blocks) {
     __shared__ JoinRoom<T, W, 64> room;
-    const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
+    const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line, at_line = ch.line0 + line, o = at_line / col_blocks;
     if (k >= ch.tiles) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const uint32_t row = (uint32_t)a.inner, col0 = (line - o * col_blocks) * 64, col = col0 + lane;
+    const uint32_t row = (uint32_t)a.inner, col0 = (at_line - o * col_blocks) * 64, col = col0 + lane;
     const bool in = col < row;
     const uint32_t lc = in ? lane : row - 1 - col0;
     const uint64_t t0 = ((uint64_t)k * W + w) * L;
@@ -417,7 +423,8 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
             }
         }
     }
-    const T first = k == 0 && a.state ? a.state[sc] : (T)0;
+    T first = k == 0 && a.state ? a.state[sc] : (T)0;
+    RT_PIN_LANE(first);
     T* h = a.h + base;
     const T end = join_tile(ch, room, item, k, A, H, cuts != 0, false, first, [&](T p, bool) {
         RT_APART;
@@ -481,10 +488,10 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
     constexpr bool kHeld = S::kHeld, kSigmoid = FORM == RT_SCAN_SIGMOID;
     typedef typename std::conditional<kHeld, HeldRows<L>, NoRows>::type Rows;
     __shared__ Rows hrows[W], xrows[kSigmoid ? W : 1];
-    const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line, o = line / col_blocks;
+    const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line, at_line = ch.line0 + line, o = at_line / col_blocks;
     if (k >= ch.tiles) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const uint32_t row = (uint32_t)a.inner, col0 = (line - o * col_blocks) * 64, col = col0 + lane;
+    const uint32_t row = (uint32_t)a.inner, col0 = (at_line - o * col_blocks) * 64, col = col0 + lane;
     const bool in = col < row;
     const uint32_t lc = in ? lane : row - 1 - col0;
     const uint64_t r0 = ((uint64_t)k * W + w) * L;
@@ -545,7 +552,8 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
             if constexpr (kSigmoid) xrows[w].put(xh, lane);
         }
     }
-    const T first = k == 0 && a.dlast ? a.dlast[sc] : (T)0;
+    T first = k == 0 && a.dlast ? a.dlast[sc] : (T)0;
+    RT_PIN_LANE(first);
     T *dg = a.dgate + base, *dx = a.dx + base;
     const T end = join_tile(ch, room, item, k, A, H, cuts != 0, false, first, [&](T d, bool) {
         RT_APART;
@@ -683,7 +691,7 @@ __global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chai
     if (k >= ch.tiles) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t inner = (uint32_t)a.inner, segs = kThreads >> nw.shift;
-    const uint64_t row0 = (uint64_t)line * nw.rows, rows = a.outer - row0 < nw.rows ? a.outer - row0 : nw.rows, len = rows * a.steps;
+    const uint64_t row0 = (uint64_t)(ch.line0 + line) * nw.rows, rows = a.outer - row0 < nw.rows ? a.outer - row0 : nw.rows, len = rows * a.steps;
     const uint64_t u0 = (uint64_t)k * segs * nw.ls;              // first step of the tile in the line
     const uint32_t cnt = len <= u0 ? 0 : (uint32_t)(len - u0 < (uint64_t)segs * nw.ls ? len - u0 : (uint64_t)segs * nw.ls), E = cnt * inner;
     const uint64_t step0 = row0 * a.steps + u0, base = step0 * inner;
@@ -796,7 +804,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
     if (k >= ch.tiles) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t inner = (uint32_t)a.inner, segs = kThreads >> nw.shift;
-    const uint64_t row0 = (uint64_t)line * nw.rows, rows = a.outer - row0 < nw.rows ? a.outer - row0 : nw.rows, len = rows * a.steps;
+    const uint64_t row0 = (uint64_t)(ch.line0 + line) * nw.rows, rows = a.outer - row0 < nw.rows ? a.outer - row0 : nw.rows, len = rows * a.steps;
     const uint64_t r0 = (uint64_t)k * segs * nw.ls;              // steps of the line behind the tile
     const uint32_t cnt = len <= r0 ? 0 : (uint32_t)(len - r0 < (uint64_t)segs * nw.ls ? len - r0 : (uint64_t)segs * nw.ls), E = cnt * inner;
     const uint64_t lo = len - r0 - cnt;                          // first step of the tile in the line
@@ -928,31 +936,45 @@ template <class T> __global__ void scan_no_steps_kernel(const T* src, T* dst, ui
     if (i < n) dst[i] = src ? src[i] : (T)0;
 }
 
+constexpr uint64_t kMostLanes = 1ull << 31;     // of one launch: the lanes of a grid are numbered in 32 bits
+
 uint32_t blocks_of(uint64_t n) { return (uint32_t)((n + kSBlock - 1) / kSBlock); }
 
 template <class T> int32_t no_steps(rt_ctx* ctx, const void* src, void* dst, uint64_t n) {
     if (!dst || !n || src == dst) return RT_OK;
-    hipLaunchKernelGGL(scan_no_steps_kernel<T>, dim3(blocks_of(n)), dim3(kSBlock), 0, ctx->stream, (const T*)src, (T*)dst, n);
-    RT_HIP(hipGetLastError());
+    for (uint64_t at = 0; at < n; at += kMostLanes) {
+        const uint64_t len = n - at < kMostLanes ? n - at : kMostLanes;
+        hipLaunchKernelGGL(scan_no_steps_kernel<T>, dim3(blocks_of(len)), dim3(kSBlock), 0, ctx->stream, src ? (const T*)src + at : nullptr, (T*)dst + at, len);
+        RT_HIP(hipGetLastError());
+    }
+    return RT_OK;
+}
+// One lane a column, over as many launches as that takes.
+template <class Args, class Kernel> int32_t columns_launches(rt_ctx* ctx, Args a, Kernel kernel) {
+    const uint64_t cols = a.outer * a.inner;
+    for (a.col0 = 0; a.col0 < cols; a.col0 += kMostLanes) {
+        const uint64_t len = cols - a.col0 < kMostLanes ? cols - a.col0 : kMostLanes;
+        hipLaunchKernelGGL(kernel, dim3(blocks_of(len)), dim3(kSBlock), 0, ctx->stream, a);
+        RT_HIP(hipGetLastError());
+    }
     return RT_OK;
 }
 
 // The chain of a launch: `tiles` along the steps for each of `lines` sets of columns; a workspace only where there is more than one tile.
-template <class T> int32_t make_chain(rt_ctx* ctx, uint64_t tiles, uint64_t lines, Chain* out) {
-    if (tiles + 7 >= (1ull << 31) / lines) return rt_fail(RT_E_INVALID, "gated scan: too long for one launch");
-    out->tiles = (uint32_t)tiles;
-    out->lines = (uint32_t)lines;
+template <class T> int32_t make_chain(rt_ctx* ctx, uint32_t tiles, uint32_t rounds, uint32_t lines, Chain* out) {
+    out->tiles = tiles;
+    out->lines = lines;
     out->tickets = nullptr;
     out->words = nullptr;
     out->epoch = 0;
-    out->rounds = (uint32_t)(tiles >= 16 ? (tiles + 7) / 8 * 8 : tiles);
+    out->rounds = rounds;
     if (tiles == 1) return RT_OK;
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
     RT_HIP(hipStreamIsCapturing(ctx->stream, &capture));
     if (capture != hipStreamCaptureStatusNone) return rt_fail(RT_E_INVALID, "gated scan: a launch that hands states from tile to tile cannot be captured");
     void *tickets = nullptr, *words = nullptr;
-    RT_TRY(rt_chain_room(ctx, 0, lines * kTicketPitch * sizeof(uint32_t), &tickets));
-    RT_TRY(rt_chain_room(ctx, 1, tiles * lines * Slot<T>::kWords * sizeof(uint64_t), &words));
+    RT_TRY(rt_chain_room(ctx, 0, (uint64_t)lines * kTicketPitch * sizeof(uint32_t), &tickets));
+    RT_TRY(rt_chain_room(ctx, 1, (uint64_t)tiles * lines * Slot<T>::kWords * sizeof(uint64_t), &words));
     // the slots are cleared, and old tags with them, before numbers come round
     if (++ctx->chain_launches == 1u << 29) {
         RT_TRY(rt_chain_clear(ctx, 1));
@@ -961,6 +983,20 @@ template <class T> int32_t make_chain(rt_ctx* ctx, uint64_t tiles, uint64_t line
     out->tickets = (uint32_t*)tickets;
     out->words = (uint64_t*)words;
     out->epoch = ctx->chain_launches;
+    return RT_OK;
+}
+// `launch(chain)` for all lines, by blocks of `threads`, over as many launches as that takes.
+template <class T, class Launch> int32_t chain_launches(rt_ctx* ctx, uint64_t tiles, uint64_t lines, uint32_t threads, Launch launch) {
+    const uint64_t rounds = tiles >= 16 ? (tiles + 7) / 8 * 8 : tiles;
+    if (lines >= 1ull << 31 || rounds >= kMostLanes / threads) return rt_fail(RT_E_INVALID, "gated scan: too long for one launch");
+    const uint64_t most = kMostLanes / (rounds * threads);
+    Chain ch;
+    for (uint64_t at = 0; at < lines; at += most) {
+        RT_TRY(make_chain<T>(ctx, (uint32_t)tiles, (uint32_t)rounds, (uint32_t)(lines - at < most ? lines - at : most), &ch));
+        ch.line0 = (uint32_t)at;
+        launch(ch);
+        RT_HIP(hipGetLastError());
+    }
     return RT_OK;
 }
 
@@ -976,7 +1012,8 @@ template <class T> bool whole_lines(uint64_t inner) { return inner * sizeof(T) %
 // One lane a column: few steps (a token), or so many columns that they fill the card.
 bool by_columns(uint64_t steps, uint64_t inner) { return steps <= kFewSteps || inner >= kWideMost; }
 
-template <class T, int W> int32_t make_narrow(rt_ctx* ctx, uint64_t outer, uint64_t steps, uint64_t inner, Chain* ch, Narrow* nw) {
+// Cuts the operands into lines and tiles.
+template <class T, int W> void make_narrow(rt_ctx* ctx, uint64_t outer, uint64_t steps, uint64_t inner, Narrow* nw, uint64_t* out_tiles, uint64_t* out_lines) {
     nw->shift = 0;
     while ((1ull << nw->shift) < inner) ++nw->shift;
     const uint64_t segs = (uint64_t)(W * 64) >> nw->shift, most = segs * seg_steps<T>();       // steps of a tile
@@ -990,7 +1027,8 @@ template <class T, int W> int32_t make_narrow(rt_ctx* ctx, uint64_t outer, uint6
     nw->ls = (uint32_t)((per + segs - 1) / segs);
     nw->by_inner = make_fastdiv((uint32_t)inner);
     nw->by_steps = make_fastdiv(nw->rows > 1 ? (uint32_t)steps : 1u);
-    return make_chain<T>(ctx, (len + segs * nw->ls - 1) / (segs * nw->ls), (outer + nw->rows - 1) / nw->rows, ch);
+    *out_tiles = (len + segs * nw->ls - 1) / (segs * nw->ls);
+    *out_lines = (outer + nw->rows - 1) / nw->rows;
 }
 
 // More than 64 KiB of LDS has to be asked for, once a device.
@@ -1004,29 +1042,28 @@ int32_t allow_lds(rt_ctx* ctx, const void* kernel, size_t bytes, std::atomic<uin
 
 template <class T, int FORM> int32_t forward_form(rt_ctx* ctx, const ScanArgs<T>& a) {
     constexpr int kWaves = 8, L = forward_steps<T>();
-    Chain ch;
-    if (by_columns(a.steps, a.inner)) {
-        hipLaunchKernelGGL((scan_columns_kernel<T, FORM>), dim3(blocks_of(a.outer * a.inner)), dim3(kSBlock), 0, ctx->stream, a);
-    } else if (a.inner < kWideLeast) {
+    if (by_columns(a.steps, a.inner)) return columns_launches(ctx, a, scan_columns_kernel<T, FORM>);
+    if (a.inner < kWideLeast) {
         Narrow nw;
-        RT_TRY((make_narrow<T, kWaves>(ctx, a.outer, a.steps, a.inner, &ch, &nw)));
+        uint64_t tiles, lines;
+        make_narrow<T, kWaves>(ctx, a.outer, a.steps, a.inner, &nw, &tiles, &lines);
         auto kernel = scan_narrow_kernel<T, FORM, kWaves>;
         static std::atomic<uint64_t> allowed{0};
         RT_TRY((allow_lds(ctx, reinterpret_cast<const void*>(kernel), most_tile_bytes<T, kWaves>(), allowed)));
         const size_t bytes = tile_bytes<T, kWaves>(nw, a.reset != nullptr);
-        hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(kWaves * 64), bytes, ctx->stream, a, ch, nw);
-    } else {
-        const uint64_t cb = (a.inner + 63) / 64;
-        const uint64_t tile = a.steps <= L ? L : kWaves * L;     // one wave's steps are a tile where they are enough
-        RT_TRY(make_chain<T>(ctx, (a.steps + tile - 1) / tile, a.outer * cb, &ch));
-        const dim3 grid(ch.rounds * ch.lines);
-        const bool whole = whole_lines<T>(a.inner);
-        auto one = whole ? scan_wide_kernel<T, FORM, 1, L, true> : scan_wide_kernel<T, FORM, 1, L, false>;
-        auto many = whole ? scan_wide_kernel<T, FORM, kWaves, L, true> : scan_wide_kernel<T, FORM, kWaves, L, false>;
-        hipLaunchKernelGGL(a.steps <= L ? one : many, grid, dim3(a.steps <= L ? 64 : kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
+        return chain_launches<T>(ctx, tiles, lines, kWaves * 64, [&](const Chain& ch) {
+            hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(kWaves * 64), bytes, ctx->stream, a, ch, nw);
+        });
     }
-    RT_HIP(hipGetLastError());
-    return RT_OK;
+    const uint64_t cb = (a.inner + 63) / 64;
+    const uint64_t tile = a.steps <= L ? L : kWaves * L;         // one wave's steps are a tile where they are enough
+    const uint32_t threads = a.steps <= L ? 64 : kWaves * 64;
+    const bool whole = whole_lines<T>(a.inner);
+    auto one = whole ? scan_wide_kernel<T, FORM, 1, L, true> : scan_wide_kernel<T, FORM, 1, L, false>;
+    auto many = whole ? scan_wide_kernel<T, FORM, kWaves, L, true> : scan_wide_kernel<T, FORM, kWaves, L, false>;
+    return chain_launches<T>(ctx, (a.steps + tile - 1) / tile, a.outer * cb, threads, [&](const Chain& ch) {
+        hipLaunchKernelGGL(a.steps <= L ? one : many, dim3(ch.rounds * ch.lines), dim3(threads), 0, ctx->stream, a, ch, (uint32_t)cb);
+    });
 }
 template <class T> int32_t forward_typed(rt_ctx* ctx, int form, const ScanArgs<T>& a) {
     return form == RT_SCAN_LINEAR ? forward_form<T, RT_SCAN_LINEAR>(ctx, a) : forward_form<T, RT_SCAN_SIGMOID>(ctx, a);
@@ -1036,29 +1073,28 @@ template <class T, int FORM, class S> int32_t backward_form(rt_ctx* ctx, const B
     // waves of a wide tile: with the registers of the linear form two blocks of eight fit a CU, of the other one three of four; longer tiles
     // make shorter chains (linear from the 8-bit form over (1, 50000, 1088): 195 us with four, 164 with eight; the other one 199 and 215)
     constexpr int kWaves = FORM == RT_SCAN_LINEAR ? 8 : 4, kNarrowWaves = 8, L = backward_steps<T>();
-    Chain ch;
-    if (by_columns(a.steps, a.inner)) {
-        hipLaunchKernelGGL((scan_backward_columns_kernel<T, FORM, S>), dim3(blocks_of(a.outer * a.inner)), dim3(kSBlock), 0, ctx->stream, a);
-    } else if (a.inner < kWideLeast) {
+    if (by_columns(a.steps, a.inner)) return columns_launches(ctx, a, scan_backward_columns_kernel<T, FORM, S>);
+    if (a.inner < kWideLeast) {
         Narrow nw;
-        RT_TRY((make_narrow<T, kNarrowWaves>(ctx, a.outer, a.steps, a.inner, &ch, &nw)));
+        uint64_t tiles, lines;
+        make_narrow<T, kNarrowWaves>(ctx, a.outer, a.steps, a.inner, &nw, &tiles, &lines);
         auto kernel = scan_backward_narrow_kernel<T, FORM, S, kNarrowWaves>;
         static std::atomic<uint64_t> allowed{0};
         RT_TRY((allow_lds(ctx, reinterpret_cast<const void*>(kernel), most_tile_bytes<T, kNarrowWaves>(), allowed)));
         const size_t bytes = tile_bytes<T, kNarrowWaves>(nw, a.reset != nullptr);
-        hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(kNarrowWaves * 64), bytes, ctx->stream, a, ch, nw);
-    } else {
-        const uint64_t cb = (a.inner + 63) / 64;
-        const uint64_t tile = a.steps <= L ? L : kWaves * L;
-        RT_TRY(make_chain<T>(ctx, (a.steps + tile - 1) / tile, a.outer * cb, &ch));
-        const dim3 grid(ch.rounds * ch.lines);
-        const bool whole = whole_lines<T>(a.inner);
-        auto one = whole ? scan_backward_wide_kernel<T, FORM, S, 1, L, true> : scan_backward_wide_kernel<T, FORM, S, 1, L, false>;
-        auto many = whole ? scan_backward_wide_kernel<T, FORM, S, kWaves, L, true> : scan_backward_wide_kernel<T, FORM, S, kWaves, L, false>;
-        hipLaunchKernelGGL(a.steps <= L ? one : many, grid, dim3(a.steps <= L ? 64 : kWaves * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
+        return chain_launches<T>(ctx, tiles, lines, kNarrowWaves * 64, [&](const Chain& ch) {
+            hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(kNarrowWaves * 64), bytes, ctx->stream, a, ch, nw);
+        });
     }
-    RT_HIP(hipGetLastError());
-    return RT_OK;
+    const uint64_t cb = (a.inner + 63) / 64;
+    const uint64_t tile = a.steps <= L ? L : kWaves * L;
+    const uint32_t threads = a.steps <= L ? 64 : kWaves * 64;
+    const bool whole = whole_lines<T>(a.inner);
+    auto one = whole ? scan_backward_wide_kernel<T, FORM, S, 1, L, true> : scan_backward_wide_kernel<T, FORM, S, 1, L, false>;
+    auto many = whole ? scan_backward_wide_kernel<T, FORM, S, kWaves, L, true> : scan_backward_wide_kernel<T, FORM, S, kWaves, L, false>;
+    return chain_launches<T>(ctx, (a.steps + tile - 1) / tile, a.outer * cb, threads, [&](const Chain& ch) {
+        hipLaunchKernelGGL(a.steps <= L ? one : many, dim3(ch.rounds * ch.lines), dim3(threads), 0, ctx->stream, a, ch, (uint32_t)cb);
+    });
 }
 template <class T, class S> int32_t backward_typed(rt_ctx* ctx, int form, const BackArgs<T, S>& a) {
     return form == RT_SCAN_LINEAR ? backward_form<T, RT_SCAN_LINEAR, S>(ctx, a) : backward_form<T, RT_SCAN_SIGMOID, S>(ctx, a);
@@ -1144,7 +1180,7 @@ template <class T, class S> int32_t run_backward(const BackwardCall& c, S x, S h
     a.state = (const T*)c.state.p; a.reset = (const uint8_t*)c.reset.p;
     a.dh = (const T*)c.dh.p; a.dlast = (const T*)dlast;
     a.dgate = (T*)const_cast<void*>(c.dgate.p); a.dx = (T*)const_cast<void*>(c.dx.p); a.dstate = (T*)const_cast<void*>(c.dstate.p);
-    a.outer = c.outer; a.steps = c.steps; a.inner = c.inner;
+    a.outer = c.outer; a.steps = c.steps; a.inner = c.inner; a.col0 = 0;
     return backward_typed<T, S>(c.ctx, c.form, a);
 }
 
@@ -1170,10 +1206,10 @@ extern "C" int32_t rt_gated_scan(rt_ctx* ctx, int32_t dtype, int32_t form, const
     if (cols == 0) return RT_OK;
     RT_TRY(dtype == RT_F32 ? apart<float>(ctx, &state, last, reset, outer, steps, inner) : apart<double>(ctx, &state, last, reset, outer, steps, inner));
     if (dtype == RT_F32) {
-        const ScanArgs<float> a = {(const float*)gate, (const float*)x, (const float*)state, (const uint8_t*)reset, (float*)h, (float*)last, outer, steps, inner};
+        const ScanArgs<float> a = {(const float*)gate, (const float*)x, (const float*)state, (const uint8_t*)reset, (float*)h, (float*)last, outer, steps, inner, 0};
         return forward_typed<float>(ctx, form, a);
     }
-    const ScanArgs<double> a = {(const double*)gate, (const double*)x, (const double*)state, (const uint8_t*)reset, (double*)h, (double*)last, outer, steps, inner};
+    const ScanArgs<double> a = {(const double*)gate, (const double*)x, (const double*)state, (const uint8_t*)reset, (double*)h, (double*)last, outer, steps, inner, 0};
     return forward_typed<double>(ctx, form, a);
 }
 

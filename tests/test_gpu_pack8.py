@@ -225,3 +225,20 @@ def test_matmul_over_the_range_of_exponents(hip):
         # 2^-126 per product: a part of an element below the normal range may be dropped
         bound = (m + 4) * 2.0 ** -24 * 1.01 * mag + np.abs(xr).T @ np.full((m, n), 2.0 ** -126)
         assert (np.abs(hip.dump(out).reshape(k, n) - want) <= bound).all(), scale
+
+
+def test_more_elements_than_a_launch_has_lanes():
+    """More than 2^33 elements: 3 is 96 steps of 2^-5."""
+    from rtensors_amd import hip as H
+    be, n = H.Hip.new(0), (1 << 33) + 100
+    src, (codes, exps) = be.alloc_uninit(H.F32, n), be.alloc_pack8(n)
+    be.fill_contiguous(src, 3.0, 0, n)
+    be.fill_contiguous(codes, 0, 0, n)
+    be.pack8(src, 0, n, codes, exps)
+    places = (0, (1 << 33) - 1, 1 << 33, n - 1)
+    for i in places:
+        assert be.read(codes, i) == 96 and be.read(exps, i // 32) == 122, i
+    be.fill_contiguous(src, -1.0, 0, n)
+    be.unpack8(codes, exps, n, src)
+    for i in places:
+        assert be.read(src, i) == 3, i

@@ -286,3 +286,44 @@ def test_offsets_beyond_32_bits(hip, inner):
     hip.gated_scan_backward("linear", gate, None, h, x, hip.alloc_uninit(H.F32, n), x, 1, steps, inner)
     for t in (0, steps // 2, steps - 2, steps - 1):
         assert hip.read(x, t * inner + inner - 1) == np.float32(2 - 2.0 ** -(steps - 1 - t)), t
+
+
+def test_more_columns_than_a_launch_has_lanes():
+    """One token over more than 2^31 columns: h = 0.5 * 2 + 1, in place of x, and the new state in place of the old one."""
+    from rtensors_amd import hip as H
+    be, n = H.Hip.new(0), (1 << 31) + 1000
+    gate, x, state = (be.alloc_uninit(H.F32, n) for _ in range(3))
+    for b, v in ((gate, 0.5), (x, 1.0), (state, 2.0)):
+        be.fill_contiguous(b, v, 0, n)
+    places = (0, 12345, (1 << 31) - 1, 1 << 31, n - 1)
+    be.gated_scan("linear", gate, x, x, 1, 1, n, state=state, last=state)
+    for i in places:
+        assert be.read(x, i) == 2 and be.read(state, i) == 2, i
+    be.fill_contiguous(state, 4.0, 0, n)
+    dgate, dstate = be.alloc_uninit(H.F32, n), be.alloc_uninit(H.F32, n)
+    be.gated_scan_backward("linear", gate, None, x, x, dgate, be.alloc_uninit(H.F32, n), 1, 1, n, state=state, dstate=dstate)
+    for i in places:
+        assert be.read(dgate, i) == 8 and be.read(dstate, i) == 1, i
+    be.gated_scan("linear", gate, x, x, 1, 0, n, last=state)                       # no steps and no state: zeros
+    for i in places:
+        assert be.read(state, i) == 0, i
+
+
+def test_more_rows_than_a_launch_has_lanes():
+    """512 lanes a row and more than 2^22 rows."""
+    from rtensors_amd import hip as H
+    be, (outer, steps, inner) = H.Hip.new(0), ((1 << 22) + 3, 33, 33)
+    n = outer * steps * inner
+    gate, x, h = (be.alloc_uninit(H.F32, n) for _ in range(3))
+    for b, v in ((gate, 0.5), (x, 1.0), (h, -1.0)):
+        be.fill_contiguous(b, v, 0, n)
+    rows = (0, 1000, (1 << 22) - 1, 1 << 22, outer - 1)
+    be.gated_scan("linear", gate, x, h, outer, steps, inner)
+    for o in rows:
+        for t in (0, 1, steps - 1):
+            for i in (0, inner - 1):
+                assert be.read(h, (o * steps + t) * inner + i) == np.float32(2 - 2.0 ** -t), (o, t, i)
+    be.gated_scan_backward("linear", gate, None, h, x, be.alloc_uninit(H.F32, n), x, outer, steps, inner)
+    for o in rows:
+        for t in (0, 1, steps - 1):
+            assert be.read(x, (o * steps + t) * inner + inner - 1) == np.float32(2 - 2.0 ** -(steps - 1 - t)), (o, t)
