@@ -198,8 +198,8 @@ __device__ __forceinline__ bool finite(double v) { return __builtin_fabs(v) < __
 
 // LN: lanes that hold different columns; with 32 the upper half of a wave repeats the lower one.
 template <class T, int W, int LN> struct JoinRoom {
-    // tiles before its own that a tile looks at (with f64 tiles staged through LDS: as many as leave room for two blocks a CU)
-    static constexpr int kWindow = W == 1 ? 1 : sizeof(T) == 4 ? 16 : LN == 32 ? 4 : 8;
+    // tiles before its own that a tile looks at (f64: as many as leave room for the blocks that the registers allow)
+    static constexpr int kWindow = W == 1 ? 1 : sizeof(T) == 4 || W == 16 ? 16 : LN == 32 && W == 8 ? 4 : 8;
     T A[W][LN], H[W][LN], start[LN];
     T winA[kWindow][LN], winH[kWindow][LN];
     uint64_t ends[kWindow];
@@ -612,17 +612,21 @@ template <class T, int W> struct Tile {
     static constexpr uint32_t kLine = 64 / sizeof(T);            // one element of padding for each of these: a wave's segments start in
                                                                  // different banks
     static __device__ __forceinline__ uint32_t at(uint32_t e) { return e + e / kLine; }
-    T a[kMost + 64 + (kMost + 64) / kLine], b[kMost + 64 + (kMost + 64) / kLine];    // lanes without a column read up to 62 further
+    static constexpr uint32_t kRoom = kMost + 64 + (kMost + 64) / kLine;             // lanes without a column read up to 62 further
+};
+// Forward, the gates and then x go through the same room: twice the blocks on a CU.  Backward, both are needed at the end.
+template <class T, int W> struct ForwardTile : Tile<T, W> {
+    T v[Tile<T, W>::kRoom];
     uint8_t reset[1];                                            // one byte a step and one more, where there are resets
 };
-template <class T, int W> size_t tile_bytes(const Narrow& nw, bool reset) {
-    typedef Tile<T, W> TT;
+template <class T, int W> struct BackwardTile : Tile<T, W> {
+    T a[Tile<T, W>::kRoom], b[Tile<T, W>::kRoom];
+    uint8_t reset[1];
+};
+template <class TT, int W> size_t tile_bytes(const Narrow& nw, bool reset) {
     return offsetof(TT, reset) + (reset ? ((size_t)(W * 64) >> nw.shift) * nw.ls + 1 : 0);
 }
-template <class T, int W> constexpr size_t most_tile_bytes() {
-    typedef Tile<T, W> TT;
-    return offsetof(TT, reset) + TT::kMost + 1;
-}
+template <class TT> constexpr size_t most_tile_bytes() { return offsetof(TT, reset) + TT::kMost + 1; }
 // What joins a wave's segments: the exclusive prefix of the lane's segment, and the wave's whole.
 template <class T> struct Prefix {
     T A, H, wholeA, wholeH;
@@ -680,13 +684,14 @@ template <class T, class Go> __device__ __forceinline__ T run_lanes(const Prefix
 // Segment of a lane: a wave's lanes hold 64 >> shift consecutive ones.
 __device__ __forceinline__ int tile_segment(int tid, uint32_t shift) { return (tid >> 6) * (64 >> shift) + ((tid & 63) >> shift); }
 
+// Four waves a tile and six on a SIMD, so that there are blocks in every phase; longer tiles for few rows.
 template <class T, int FORM, int W>
-__global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chain ch, Narrow nw) {
+__global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void scan_narrow_kernel(ScanArgs<T> a, Chain ch, Narrow nw) {
     constexpr int kSeg = seg_steps<T>(), kThreads = W * 64;
     __shared__ JoinRoom<T, W, 32> room;                          // inner is below 32
     extern __shared__ __align__(16) char lds[];
-    Tile<T, W>& tile = *reinterpret_cast<Tile<T, W>*>(lds);
-    typedef Tile<T, W> TT;
+    typedef ForwardTile<T, W> TT;
+    TT& tile = *reinterpret_cast<TT*>(lds);
     const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line;
     if (k >= ch.tiles) return;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -696,8 +701,9 @@ __global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chai
     const uint32_t cnt = len <= u0 ? 0 : (uint32_t)(len - u0 < (uint64_t)segs * nw.ls ? len - u0 : (uint64_t)segs * nw.ls), E = cnt * inner;
     const uint64_t step0 = row0 * a.steps + u0, base = step0 * inner;
     const uint32_t all = segs * nw.ls * inner;                   // with the steps that are not there: they carry a state on as it is
+    T x[kSeg];
     {
-        T g[kSeg], x[kSeg];                                      // all loads before the first write
+        T g[kSeg];                                               // all loads before the first write
 #pragma unroll
         for (int q = 0; q < kSeg; ++q) {
             const uint32_t e = tid + q * kThreads;
@@ -711,10 +717,7 @@ __global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chai
 #pragma unroll
         for (int q = 0; q < kSeg; ++q) {
             const uint32_t e = tid + q * kThreads;
-            if (e < all) {
-                tile.a[TT::at(e)] = g[q];
-                tile.b[TT::at(e)] = x[q];
-            }
+            if (e < all) tile.v[TT::at(e)] = g[q];
         }
     }
     if (a.reset)
@@ -740,10 +743,25 @@ __global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chai
     {
         uint32_t e = v0 * inner + c;
 #pragma unroll
+        for (int j = 0; j < kSeg; ++j)
+            if (j < ls) {
+                f[j] = tile.v[TT::at(e)];
+                e += inner;
+            }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kSeg; ++q) {
+        const uint32_t e = tid + q * kThreads;
+        if (e < all) tile.v[TT::at(e)] = x[q];
+    }
+    __syncthreads();
+    {
+        uint32_t e = v0 * inner + c;
+#pragma unroll
         for (int j = 0; j < kSeg; ++j) {
             if (j < ls) {
-                f[j] = tile.a[TT::at(e)];
-                b[j] = tile.b[TT::at(e)];
+                b[j] = tile.v[TT::at(e)];
                 e += inner;
                 if constexpr (FORM == RT_SCAN_SIGMOID) {
                     const RtGate<T> q = gate_of(f[j]);
@@ -768,7 +786,7 @@ __global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chai
                 for (int j = 0; j < kSeg; ++j) {
                     if (j < rls) {
                         p = rcuts >> j & 1 ? b[j] : fused(f[j], p, b[j]);
-                        tile.b[TT::at(e)] = p;
+                        tile.v[TT::at(e)] = p;
                         e += rinner;
                     }
                 }
@@ -780,13 +798,13 @@ __global__ __launch_bounds__(W * 64) void scan_narrow_kernel(ScanArgs<T> a, Chai
 #pragma unroll
     for (int q = 0; q < kSeg; ++q) {
         const uint32_t e = tid + q * kThreads;
-        if (e < E) __builtin_nontemporal_store(tile.b[TT::at(e)], a.h + base + e);
+        if (e < E) __builtin_nontemporal_store(tile.v[TT::at(e)], a.h + base + e);
     }
     if (a.last && u0 + cnt == len) {                             // the end of a line's rows: all of them, or the one whose last tile this is
         const uint32_t ends = nw.rows == 1 ? inner : (uint32_t)rows * inner, stretch = nw.rows == 1 ? cnt : (uint32_t)a.steps;
         for (uint32_t q = tid; q < ends; q += kThreads) {
             const uint32_t r = fd_div(q, nw.by_inner);
-            a.last[row0 * inner + q] = tile.b[TT::at(((r + 1) * stretch - 1) * inner + (q - r * inner))];
+            a.last[row0 * inner + q] = tile.v[TT::at(((r + 1) * stretch - 1) * inner + (q - r * inner))];
         }
     }
 }
@@ -798,8 +816,8 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
     constexpr int kSeg = seg_steps<T>(), kThreads = W * 64;
     __shared__ JoinRoom<T, W, 32> room;                          // inner is below 32
     extern __shared__ __align__(16) char lds[];
-    Tile<T, W>& tile = *reinterpret_cast<Tile<T, W>*>(lds);
-    typedef Tile<T, W> TT;
+    typedef BackwardTile<T, W> TT;
+    TT& tile = *reinterpret_cast<TT*>(lds);
     const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line;
     if (k >= ch.tiles) return;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -1007,6 +1025,11 @@ constexpr uint64_t kWideLeast = 32;             // inner: at least half of a wav
 constexpr uint64_t kWideMost = 1ull << 22;      // inner: a wave's rows are addressed with 32-bit offsets; beyond it columns alone fill the card
 constexpr uint64_t kFewSteps = 8;               // steps that one lane a column goes through without help
 
+// Rows of few columns that are too few to hide the chain's latency take longer tiles.  f32 with 16, 8 and 4 waves a tile: one row of 2^25
+// 296, 636 and 1484 us; 4 rows of 2^23 154, 181 and 395 us; 8 of 2^22 153, 117 and 211 us; 16 of 2^21 153, 107 and 122 us; 32 of 2^20
+// 154, 104 and 102 us.  f64 (16 and 4 waves): 8 rows of 2^21 152 and 222 us; 16 of 2^20 148 and 164 us; 2048 of 4097 100 and 48 us.
+constexpr uint64_t kFewRows = 16;
+
 template <class T> bool whole_lines(uint64_t inner) { return inner * sizeof(T) % 128 == 0; }
 
 // One lane a column: few steps (a token), or so many columns that they fill the card.
@@ -1040,20 +1063,28 @@ int32_t allow_lds(rt_ctx* ctx, const void* kernel, size_t bytes, std::atomic<uin
     return RT_OK;
 }
 
+template <class T, int FORM, int W> int32_t forward_narrow(rt_ctx* ctx, const ScanArgs<T>& a) {
+    typedef ForwardTile<T, W> TT;
+    Narrow nw;
+    uint64_t tiles, lines;
+    make_narrow<T, W>(ctx, a.outer, a.steps, a.inner, &nw, &tiles, &lines);
+    auto kernel = scan_narrow_kernel<T, FORM, W>;
+    static std::atomic<uint64_t> allowed{0};
+    RT_TRY(allow_lds(ctx, reinterpret_cast<const void*>(kernel), most_tile_bytes<TT>(), allowed));
+    const size_t bytes = tile_bytes<TT, W>(nw, a.reset != nullptr);
+    return chain_launches<T>(ctx, tiles, lines, W * 64, [&](const Chain& ch) {
+        hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(W * 64), bytes, ctx->stream, a, ch, nw);
+    });
+}
+
 template <class T, int FORM> int32_t forward_form(rt_ctx* ctx, const ScanArgs<T>& a) {
     constexpr int kWaves = 8, L = forward_steps<T>();
     if (by_columns(a.steps, a.inner)) return columns_launches(ctx, a, scan_columns_kernel<T, FORM>);
     if (a.inner < kWideLeast) {
-        Narrow nw;
-        uint64_t tiles, lines;
-        make_narrow<T, kWaves>(ctx, a.outer, a.steps, a.inner, &nw, &tiles, &lines);
-        auto kernel = scan_narrow_kernel<T, FORM, kWaves>;
-        static std::atomic<uint64_t> allowed{0};
-        RT_TRY((allow_lds(ctx, reinterpret_cast<const void*>(kernel), most_tile_bytes<T, kWaves>(), allowed)));
-        const size_t bytes = tile_bytes<T, kWaves>(nw, a.reset != nullptr);
-        return chain_launches<T>(ctx, tiles, lines, kWaves * 64, [&](const Chain& ch) {
-            hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(kWaves * 64), bytes, ctx->stream, a, ch, nw);
-        });
+        if (a.outer > kFewRows) return forward_narrow<T, FORM, 4>(ctx, a);
+        if constexpr (sizeof(T) == 4)
+            if (a.outer > kFewRows / 4) return forward_narrow<T, FORM, 8>(ctx, a);
+        return forward_narrow<T, FORM, 16>(ctx, a);
     }
     const uint64_t cb = (a.inner + 63) / 64;
     const uint64_t tile = a.steps <= L ? L : kWaves * L;         // one wave's steps are a tile where they are enough
@@ -1080,8 +1111,8 @@ template <class T, int FORM, class S> int32_t backward_form(rt_ctx* ctx, const B
         make_narrow<T, kNarrowWaves>(ctx, a.outer, a.steps, a.inner, &nw, &tiles, &lines);
         auto kernel = scan_backward_narrow_kernel<T, FORM, S, kNarrowWaves>;
         static std::atomic<uint64_t> allowed{0};
-        RT_TRY((allow_lds(ctx, reinterpret_cast<const void*>(kernel), most_tile_bytes<T, kNarrowWaves>(), allowed)));
-        const size_t bytes = tile_bytes<T, kNarrowWaves>(nw, a.reset != nullptr);
+        RT_TRY((allow_lds(ctx, reinterpret_cast<const void*>(kernel), most_tile_bytes<BackwardTile<T, kNarrowWaves>>(), allowed)));
+        const size_t bytes = tile_bytes<BackwardTile<T, kNarrowWaves>, kNarrowWaves>(nw, a.reset != nullptr);
         return chain_launches<T>(ctx, tiles, lines, kNarrowWaves * 64, [&](const Chain& ch) {
             hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(kNarrowWaves * 64), bytes, ctx->stream, a, ch, nw);
         });
