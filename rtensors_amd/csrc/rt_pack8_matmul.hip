@@ -70,12 +70,13 @@ struct Product {
     uint32_t ti, tj, splits;          // tiles of dst, shares of the rows
 };
 // Tile of a block: batch-major, then the splits; within one (batch, split) the tiles in bands of eight along i, so that blocks that run
-// at the same time on one XCD (every eighth block) share columns of both operands in its L2.
+// at the same time on one XCD (every eighth block) share columns of both operands in its L2: XCD x takes the x-th eighth of the tiles.
 struct Where { uint64_t batch; uint32_t split, i, j; };
 __device__ __forceinline__ Where where(const Product& p) {
     const uint32_t tiles = p.ti * p.tj, total = gridDim.x;
     uint32_t t = blockIdx.x;
-    if (total % 8 == 0) t = t % 8 * (total / 8) + t / 8;
+    const uint32_t xcd = t % 8, more = total % 8;
+    t = xcd * (total / 8) + (xcd < more ? xcd : more) + t / 8;
     Where w;
     const uint32_t bs = t / tiles;
     t -= bs * tiles;
@@ -90,7 +91,9 @@ __device__ __forceinline__ Where where(const Product& p) {
 
 // One step of the loop works on three steps of the rows at once: the matrix instructions take the one in the current buffer, the next one
 // is turned into parts and written to the other buffer, and the one after that is on its way from memory into registers.  EVEN: k is
-// even, so a lane's two codes lie in one group.
+// even, so a lane's two codes lie in one group.  The matrix instructions come first, so that the loads have all of them to arrive behind
+// (16384 x 4096 x 4096 1400 -> 1320 us); not so with odd k and its twice as many loads (16000 x 2001 x 2003 410 us, the other way round
+// 430 us).
 template <int BI, int BJ, int WI, int WJ, int DEPTH, bool EVEN>
 __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product p) {
     constexpr int kThreads = WI * WJ * 64, FI = BI / WI / 32, FJ = BJ / WJ / 32;             // 32 x 32 pieces of a wave
@@ -100,7 +103,7 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product 
     Stage<BI, BJ>* stage = reinterpret_cast<Stage<BI, BJ>*>(lds);
     const Where at = where(p);
     const Share share = share_of(p.m, p.splits, at.split);
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wi = w / WJ, wj = w % WJ;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wi = w / WJ, wj = w % WJ;
     const uint64_t i0 = (uint64_t)at.i * BI, j0 = (uint64_t)at.j * BJ;
     // staging: the lane's two columns of x and one row group; kYEach row groups of one column of y
     const int xc = tid % (BI / 2) * 2, xg = tid / (BI / 2);
@@ -237,9 +240,10 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product 
         for (; t + 2 * DEPTH + 1 < steps; t += DEPTH) {          // DEPTH steps a turn, so that the sets are named at compile time; whole ones
 #pragma unroll
             for (int d = 0; d < DEPTH; ++d) {
+                if constexpr (EVEN) multiply(stage[(t + d) & 1]);
                 store(held[d], stage[(t + d + 1) & 1]);
                 load_whole(held[d], row_of(t + d + 1 + DEPTH));
-                multiply(stage[(t + d) & 1]);
+                if constexpr (!EVEN) multiply(stage[(t + d) & 1]);
                 __syncthreads();
             }
         }
@@ -425,14 +429,14 @@ template <int BI, int BJ, int WI, int WJ, int DEPTH, bool EVEN> int32_t f32_laun
 
 template <bool EVEN> int32_t f32_any(rt_ctx* ctx, const Product& p, int shape) {
     if (shape == 0) return f32_launch<256, 256, 2, 4, 1, EVEN>(ctx, p);
-    if (shape == 1) return f32_launch<256, 128, 4, 2, 1, EVEN>(ctx, p);
+    if (shape == 1) return f32_launch<256, 128, 4, 2, 2, EVEN>(ctx, p);
     return f32_launch<128, 128, 2, 2, 2, EVEN>(ctx, p);
 }
 
 int32_t run_product(rt_ctx* ctx, int dtype, Product p, void* dst) {
     struct Shape { uint64_t bi, bj, least_rows, per_cu; double rate; };
     // The tile's shape: the larger, the fewer conversions there are for each matrix instruction.  `rate` is what a shape reaches of the
-    // first one's rate on a result it divides (16384 x 4096 x 4096: 1441, 1633 and 1824 us -- the smaller ones are better than that on
+    // first one's rate on a result it divides (16384 x 4096 x 4096: 1318, 1569 and 1765 us -- the smaller ones are better than that on
     // short shares, hence less weight); the shape with the least padded area at its rate is taken, of those that give every CU a block.
     static const Shape f32[3] = {{256, 256, 512, 1, 1.0}, {256, 128, 256, 1, 0.8}, {128, 128, 64, 2, 0.6}};
     static const Shape f64[2] = {{128, 128, 128, 2, 1.0}, {64, 64, 64, 4, 1.0}};
