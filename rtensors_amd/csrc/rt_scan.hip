@@ -18,6 +18,14 @@ template <bool ONCE, class T> __device__ __forceinline__ T once(const T* p) {
     else return *p;
 }
 
+// The same for a store: the backward pass, with two outputs, gains from lines that wait in the L2 for their other half ((32, 1000, 1500)
+// f32 284 -> 246 us, (1, 50000, 1111) from the 8-bit form 287 -> 279 us), the forward pass does not (158 -> 165 us), nor does f64, whose
+// stretches are twice as long ((2, 8192, 1000) backward 166 -> 174 us).
+template <bool ONCE, class T> __device__ __forceinline__ void put_once(T v, T* p) {
+    if constexpr (ONCE) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
+
 // x and h of the backward pass: whole values or the 8-bit form
 template <class T> struct Whole {
     static constexpr bool kHeld = false;
@@ -276,12 +284,13 @@ template <class T, int W, int LN> __device__ __forceinline__ T chain_start(const
 
 // The line a block works on.  Blocks go to the eight XCDs in turn, each with an L2 of its own, and lines that are neighbours in memory
 // share the cache lines at their borders (all of them where rows are no multiple of 128 bytes): every XCD goes through all lines in
-// order, the XCDs an eighth of the lines apart, so that neighbouring lines mostly get the same tile in the same L2.
-__device__ __forceinline__ uint32_t line_of_block(const Chain& ch) {
+// order, so that neighbouring lines mostly get the same tile in the same L2.  SPREAD: the XCDs start an eighth of the lines apart, else
+// all at the first.  Forward over (1, 65536, 4096) f32 545 us spread, 575 us not; backward over (8, 2048, 2048) 154 and 146 us, over
+// (32, 1000, 1500), rows of no whole lines, 246 and 271 us.
+template <bool SPREAD> __device__ __forceinline__ uint32_t line_of_block(const Chain& ch) {
     const uint32_t b = blockIdx.x;
     if (ch.rounds % 8 != 0 || ch.tiles == 1) return b % ch.lines;
-    const uint32_t x = b % 8;
-    return (b / 8 + (uint32_t)((uint64_t)x * ch.lines / 8)) % ch.lines;
+    return (b / 8 + (SPREAD ? (uint32_t)((uint64_t)(b % 8) * ch.lines / 8) : 0u)) % ch.lines;
 }
 // The block's tile among those of its line (one that is not there for the blocks too many); whoever takes the last one leaves the counter
 // as the next launch needs it.
@@ -389,7 +398,7 @@ __device__ __forceinline__ uint64_t reset_bits(const uint8_t* flags, int64_t str
 template <class T, int FORM, int W, int L, bool ALIGNED>
 __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain ch, uint32_t col_blocks) {
     __shared__ JoinRoom<T, W, 64> room;
-    const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line, at_line = ch.line0 + line, o = at_line / col_blocks;
+    const uint32_t line = line_of_block<true>(ch), k = take_tile(ch, line, room), item = k * ch.lines + line, at_line = ch.line0 + line, o = at_line / col_blocks;
     if (k >= ch.tiles) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t row = (uint32_t)a.inner, col0 = (at_line - o * col_blocks) * 64, col = col0 + lane;
@@ -488,7 +497,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
     constexpr bool kHeld = S::kHeld, kSigmoid = FORM == RT_SCAN_SIGMOID;
     typedef typename std::conditional<kHeld, HeldRows<L>, NoRows>::type Rows;
     __shared__ Rows hrows[W], xrows[kSigmoid ? W : 1];
-    const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line, at_line = ch.line0 + line, o = at_line / col_blocks;
+    const uint32_t line = line_of_block<!ALIGNED>(ch), k = take_tile(ch, line, room), item = k * ch.lines + line, at_line = ch.line0 + line, o = at_line / col_blocks;
     if (k >= ch.tiles) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t row = (uint32_t)a.inner, col0 = (at_line - o * col_blocks) * 64, col = col0 + lane;
@@ -578,11 +587,11 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
                     const uint32_t at = lane + (uint32_t)q * rrow;
                     if constexpr (FORM == RT_SCAN_LINEAR) {
                         const bool unused = none || (top && j == rn - 1 && !a.state);
-                        __builtin_nontemporal_store(unused ? (T)0 : d * p, dg + at);
-                        __builtin_nontemporal_store(d, dx + at);
+                        put_once<ALIGNED || sizeof(T) == 8>(unused ? (T)0 : d * p, dg + at);
+                        put_once<ALIGNED || sizeof(T) == 8>(d, dx + at);
                     } else {
-                        __builtin_nontemporal_store(d * (p - xj) * (s[j] * g[j]), dg + at);
-                        __builtin_nontemporal_store(g[j] * d, dx + at);
+                        put_once<ALIGNED || sizeof(T) == 8>(d * (p - xj) * (s[j] * g[j]), dg + at);
+                        put_once<ALIGNED || sizeof(T) == 8>(g[j] * d, dx + at);
                     }
                 }
             }
@@ -692,7 +701,7 @@ __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void scan_narrow_kernel(Sc
     extern __shared__ __align__(16) char lds[];
     typedef ForwardTile<T, W> TT;
     TT& tile = *reinterpret_cast<TT*>(lds);
-    const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line;
+    const uint32_t line = line_of_block<true>(ch), k = take_tile(ch, line, room), item = k * ch.lines + line;
     if (k >= ch.tiles) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t inner = (uint32_t)a.inner, segs = kThreads >> nw.shift;
@@ -818,7 +827,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
     extern __shared__ __align__(16) char lds[];
     typedef BackwardTile<T, W> TT;
     TT& tile = *reinterpret_cast<TT*>(lds);
-    const uint32_t line = line_of_block(ch), k = take_tile(ch, line, room), item = k * ch.lines + line;
+    const uint32_t line = line_of_block<true>(ch), k = take_tile(ch, line, room), item = k * ch.lines + line;
     if (k >= ch.tiles) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t inner = (uint32_t)a.inner, segs = kThreads >> nw.shift;
