@@ -43,6 +43,10 @@ __device__ __forceinline__ Parts parts_of(const uint32_t (&v)[8]) {
     return out;
 }
 
+// Bound by the matrix instructions: 16384 x 4096 x 4096 takes 1318 us, three bf16 products at 1250 TFLOP/s (the card's bf16 matmul of 8192^3
+// runs at 1154), 417 TFLOP/s of f32; short shares by what surrounds them: 65536 x 256 x 320 takes 50 us, of which 6 are the join, about
+// 10 the first loads and the partial results, and 24 steps of 1.4 us the rest.
+//
 // dst tile of BI x BJ by WI x WJ waves, kStep rows of both operands staged in LDS at a time, two buffers.  LDS holds 16-byte pieces of
 // eight rows of one column, [part][row group][column]: what a lane of the 32x32x16 matrix instruction takes is one piece, and neither
 // the writes nor the reads of a wave meet in a bank.
@@ -277,6 +281,7 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 constexpr int kStep64 = 16;
 
+// Bound by the f64 matrix instructions: 8192 x 2048 x 2048 takes 1123 us, 61 TFLOP/s (the card's f64 matmul reaches 73).
 // SIDE x SIDE of dst by WI x WJ waves, the 16x16x4 matrix instruction, kStep64 rows staged at a time, ahead as in the f32 kernel.  The
 // pitch of the staged rows, in words, is 32 more than a multiple of 64: the two rows that half a wave reads lie on the two halves of the
 // banks.
@@ -385,7 +390,8 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f64_kernel(Product 
 }
 
 // ---- the splits' partial results, added in order -----------------------------------------------------------------------------------------
-// Every wave of a block adds a quarter of the splits for 64 elements, eight loads in flight, then the four sums are added.
+// Every wave of a block adds a quarter of the splits for 64 elements, eight loads in flight, then the four sums are added.  85 splits of
+// 256 x 320 f32: 6 us, 28 MB out of the caches and 1280 short blocks.
 template <class T> __global__ __launch_bounds__(256) void pack8_matmul_join_kernel(const T* __restrict__ part, T* __restrict__ dst, uint64_t n, uint32_t splits) {
     __shared__ T sums[4][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
