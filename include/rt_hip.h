@@ -336,7 +336,8 @@ int32_t rt_matmul(rt_ctx* ctx, int32_t dtype,
  * summed apart and joined by the products of their factors; how they are cut depends on the sizes (and the device), so equal calls give
  * equal bits.  A product that leaves the range upwards makes its stretch run step by step; one that falls below the smallest normal
  * number loses what of an earlier state it carries (less than 2^-126 of that state, 2^-1022 for f64), and 0 times an infinite state is
- * NaN.  Workspace: about 1 / 100 of the operands where a run is cut over several blocks, kept by the context and grown on demand.
+ * NaN.  Workspace: 1 / 200 to 1 / 25 of the operands (few columns of f64) where a run is cut over several blocks, kept by the
+ * context and grown on demand.
  *
  * rt_gated_scan_backward: from dh (gradient of h) and dlast (gradient of last, null = 0), with a[t] the factor of p[t]:
  *     D[t] = dh[t] + (reset[t + 1] ? 0 : a[t + 1] * D[t + 1]),   D[steps - 1] = dh[steps - 1] + dlast
