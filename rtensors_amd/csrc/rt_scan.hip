@@ -208,7 +208,7 @@ __device__ __forceinline__ bool finite(double v) { return __builtin_fabs(v) < __
 // LN: lanes that hold different columns; with 32 the upper half of a wave repeats the lower one.
 template <class T, int W, int LN> struct JoinRoom {
     // tiles before its own that a tile looks at (f64: as many as leave room for the blocks that the registers allow)
-    static constexpr int kWindow = W == 1 ? 1 : sizeof(T) == 4 || W == 16 ? 16 : LN == 32 && W == 8 ? 4 : 8;
+    static constexpr int kWindow = W <= 2 ? 1 : sizeof(T) == 4 || W == 16 ? 16 : LN == 32 && W == 8 ? 4 : 8;
     T A[W][LN], H[W][LN], start[LN];
     T winA[kWindow][LN], winH[kWindow][LN];
     uint64_t ends[kWindow];
@@ -396,8 +396,8 @@ __device__ __forceinline__ uint64_t reset_bits(const uint8_t* flags, int64_t str
 
 // W waves of 64 columns, L steps each, in registers: 2 L values a lane, all of them loaded before the first is used, so that the one pass
 // over the data is bound by HBM: (1, 65536, 4096) f32 547 us, 5.9 TB/s; (1, 8192, 1024) 22 us, of which about 7 are the launch and the
-// chain.  Shorter or longer tiles lose to more joins or to fewer blocks.  A wave that ends before its L steps, and lanes behind the last column, load what
-// the last step and the last column hold, and neither use nor store it.
+// chain.  Shorter or longer tiles lose to more joins or to fewer blocks.  Lanes behind the last column load what the last column holds, and
+// neither use nor store it.
 template <class T, int FORM, int W, int L, bool ALIGNED>
 __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain ch, uint32_t col_blocks) {
     __shared__ JoinRoom<T, W, 64> room;
@@ -415,11 +415,21 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
     uint64_t cuts = t0 == 0 && !a.state ? 1 : 0;
     if (n) {
         const T *gate = a.gate + base, *x = a.x + base;
+        if (n == L) {
 #pragma unroll
-        for (int j = 0; j < L; ++j) {
-            const uint32_t at = lc + (uint32_t)(j < n ? j : n - 1) * row;
-            f[j] = once<ALIGNED>(gate + at);
-            b[j] = once<ALIGNED>(x + at);
+            for (int j = 0; j < L; ++j) {
+                f[j] = once<ALIGNED>(gate + (lc + (uint32_t)j * row));
+                b[j] = once<ALIGNED>(x + (lc + (uint32_t)j * row));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < L; ++j) {
+                f[j] = b[j] = (T)0;
+                if (j < n) {
+                    f[j] = once<ALIGNED>(gate + (lc + (uint32_t)j * row));
+                    b[j] = once<ALIGNED>(x + (lc + (uint32_t)j * row));
+                }
+            }
         }
         if (a.reset) cuts |= reset_bits(a.reset + (uint64_t)o * a.steps + t0, 1, n, lane);
 #pragma unroll
@@ -529,7 +539,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
         if (r0 > 0) f0 = gate[lc + (uint32_t)n * row];           // the gate of the step behind j = 0
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-            const int q = j < n ? n - 1 - j : 0;
+            const int q = j < n ? n - 1 - j : 0;                 // steps that are not there load the earliest one
             const uint32_t at = lc + (uint32_t)q * row;
             g[j] = once<ALIGNED>(gate + at);
             up[j] = once<ALIGNED>(dh + at);
@@ -1079,6 +1089,22 @@ int32_t allow_lds(rt_ctx* ctx, const void* kernel, size_t bytes, std::atomic<uin
     return RT_OK;
 }
 
+template <class T, int W, int L, class Args> int32_t wide_launches(rt_ctx* ctx, const Args& a, void (*kernel)(Args, Chain, uint32_t)) {
+    const uint64_t cb = (a.inner + 63) / 64;
+    return chain_launches<T>(ctx, (a.steps + W * L - 1) / (W * L), a.outer * cb, W * 64, [&](const Chain& ch) {
+        hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(W * 64), 0, ctx->stream, a, ch, (uint32_t)cb);
+    });
+}
+// Few steps are one tile of as many waves as they need, which leaves room for more blocks: (4000, 33, 512) f32 forward 374 us with eight
+// waves, 145 us with two, (500, 100, 2048) 260 us with eight, 221 us with four.
+template <int MOST, class Launch> int32_t by_waves(uint64_t steps, int L, Launch launch) {
+    if (steps <= (uint64_t)L) return launch(std::integral_constant<int, 1>());
+    if (steps <= (uint64_t)L * 2) return launch(std::integral_constant<int, 2>());
+    if constexpr (MOST > 4)
+        if (steps <= (uint64_t)L * 4) return launch(std::integral_constant<int, 4>());
+    return launch(std::integral_constant<int, MOST>());
+}
+
 template <class T, int FORM, int W> int32_t forward_narrow(rt_ctx* ctx, const ScanArgs<T>& a) {
     typedef ForwardTile<T, W> TT;
     Narrow nw;
@@ -1102,15 +1128,11 @@ template <class T, int FORM> int32_t forward_form(rt_ctx* ctx, const ScanArgs<T>
             if (a.outer > kFewRows / 4) return forward_narrow<T, FORM, 8>(ctx, a);
         return forward_narrow<T, FORM, 16>(ctx, a);
     }
-    const uint64_t cb = (a.inner + 63) / 64;
-    const uint64_t tile = a.steps <= L ? L : kWaves * L;         // one wave's steps are a tile where they are enough
-    const uint32_t threads = a.steps <= L ? 64 : kWaves * 64;
-    const bool whole = whole_lines<T>(a.inner);
-    auto one = whole ? scan_wide_kernel<T, FORM, 1, L, true> : scan_wide_kernel<T, FORM, 1, L, false>;
-    auto many = whole ? scan_wide_kernel<T, FORM, kWaves, L, true> : scan_wide_kernel<T, FORM, kWaves, L, false>;
-    return chain_launches<T>(ctx, (a.steps + tile - 1) / tile, a.outer * cb, threads, [&](const Chain& ch) {
-        hipLaunchKernelGGL(a.steps <= L ? one : many, dim3(ch.rounds * ch.lines), dim3(threads), 0, ctx->stream, a, ch, (uint32_t)cb);
-    });
+    auto launch = [&](auto waves) {
+        constexpr int W = decltype(waves)::value;
+        return wide_launches<T, W, L>(ctx, a, whole_lines<T>(a.inner) ? scan_wide_kernel<T, FORM, W, L, true> : scan_wide_kernel<T, FORM, W, L, false>);
+    };
+    return by_waves<kWaves>(a.steps, L, launch);
 }
 template <class T> int32_t forward_typed(rt_ctx* ctx, int form, const ScanArgs<T>& a) {
     return form == RT_SCAN_LINEAR ? forward_form<T, RT_SCAN_LINEAR>(ctx, a) : forward_form<T, RT_SCAN_SIGMOID>(ctx, a);
@@ -1133,15 +1155,11 @@ template <class T, int FORM, class S> int32_t backward_form(rt_ctx* ctx, const B
             hipLaunchKernelGGL(kernel, dim3(ch.rounds * ch.lines), dim3(kNarrowWaves * 64), bytes, ctx->stream, a, ch, nw);
         });
     }
-    const uint64_t cb = (a.inner + 63) / 64;
-    const uint64_t tile = a.steps <= L ? L : kWaves * L;
-    const uint32_t threads = a.steps <= L ? 64 : kWaves * 64;
-    const bool whole = whole_lines<T>(a.inner);
-    auto one = whole ? scan_backward_wide_kernel<T, FORM, S, 1, L, true> : scan_backward_wide_kernel<T, FORM, S, 1, L, false>;
-    auto many = whole ? scan_backward_wide_kernel<T, FORM, S, kWaves, L, true> : scan_backward_wide_kernel<T, FORM, S, kWaves, L, false>;
-    return chain_launches<T>(ctx, (a.steps + tile - 1) / tile, a.outer * cb, threads, [&](const Chain& ch) {
-        hipLaunchKernelGGL(a.steps <= L ? one : many, dim3(ch.rounds * ch.lines), dim3(threads), 0, ctx->stream, a, ch, (uint32_t)cb);
-    });
+    auto launch = [&](auto waves) {
+        constexpr int W = decltype(waves)::value;
+        return wide_launches<T, W, L>(ctx, a, whole_lines<T>(a.inner) ? scan_backward_wide_kernel<T, FORM, S, W, L, true> : scan_backward_wide_kernel<T, FORM, S, W, L, false>);
+    };
+    return by_waves<kWaves>(a.steps, L, launch);
 }
 template <class T, class S> int32_t backward_typed(rt_ctx* ctx, int form, const BackArgs<T, S>& a) {
     return form == RT_SCAN_LINEAR ? backward_form<T, RT_SCAN_LINEAR, S>(ctx, a) : backward_form<T, RT_SCAN_SIGMOID, S>(ctx, a);

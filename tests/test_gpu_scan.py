@@ -101,6 +101,22 @@ def test_backward(hip, shape, held, form, dtype):
             near(hip.dump(got).reshape(w.shape), w, bound, (name, shape, state, reset, held))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("form", ["linear", "sigmoid"])
+@pytest.mark.parametrize("steps", [9, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65, 96, 127, 128, 129, 255, 256, 257])
+def test_lengths_around_those_of_waves_and_tiles(hip, steps, form, dtype):
+    test_forward(hip, (2, steps, 70), form, dtype)
+    test_backward(hip, (2, steps, 70), False, form, dtype)
+    test_backward(hip, (2, steps, 70), True, form, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("form", ["linear", "sigmoid"])
+@pytest.mark.parametrize("shape", [(4, 20000, 1), (5, 9000, 2), (16, 9000, 1), (17, 3000, 2), (40, 4097, 1), (17, 900, 31)])
+def test_few_columns_and_few_or_many_rows(hip, shape, form, dtype):
+    test_forward(hip, shape, form, dtype)
+
+
 @pytest.mark.parametrize("form", ["linear", "sigmoid"])
 def test_gradients_against_differences(hip, form):
     """Central differences of sum(h * w) + sum(last * v) in doubles: the step's own error is eps^2 * |third derivative| / 6, with
