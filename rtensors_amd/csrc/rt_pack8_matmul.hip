@@ -390,19 +390,24 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f64_kernel(Product 
 }
 
 // ---- the splits' partial results, added in order -----------------------------------------------------------------------------------------
-// Every wave of a block adds a quarter of the splits for 64 elements, eight loads in flight, then the four sums are added.  85 splits of
-// 256 x 320 f32: 6 us, 28 MB out of the caches and 1280 short blocks.
-template <class T> __global__ __launch_bounds__(256) void pack8_matmul_join_kernel(const T* __restrict__ part, T* __restrict__ dst, uint64_t n, uint32_t splits) {
-    __shared__ T sums[4][64];
+// The W waves of a block add a W-th of the splits each for 64 elements, eight loads in flight, then their sums are added in order.
+// 85 splits of 256 x 320 f32: 6 us, 28 MB out of the caches and 1280 short blocks.
+template <class T, int W> __global__ __launch_bounds__(W * 64) void pack8_matmul_join_kernel(const T* __restrict__ part, T* __restrict__ dst, uint64_t n, uint32_t splits) {
+    __shared__ T sums[W][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const uint64_t i = (uint64_t)blockIdx.x * 64 + lane, at = i < n ? i : n - 1;
-    const uint32_t from = splits * w / 4, to = splits * (w + 1) / 4;
+    const uint32_t from = splits * w / W, to = splits * (w + 1) / W;
     T s = (T)0;
 #pragma unroll 8
     for (uint32_t k = from; k < to; ++k) s += part[k * n + at];
     sums[w][lane] = s;
     __syncthreads();
-    if (w == 0 && i < n) dst[i] = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+    if (w == 0 && i < n) {
+        T all = sums[0][lane];
+#pragma unroll
+        for (int v = 1; v < W; ++v) all += sums[v][lane];
+        dst[i] = all;
+    }
 }
 
 // Shares of the rows: enough blocks to fill the card, each share long enough to pay for its partial result.
@@ -414,7 +419,11 @@ uint32_t splits_for(rt_ctx* ctx, uint64_t tiles, uint64_t m, uint64_t least_rows
 }
 
 template <class T> int32_t join(rt_ctx* ctx, const void* part, void* dst, uint64_t n, uint32_t splits) {
-    hipLaunchKernelGGL(pack8_matmul_join_kernel<T>, dim3((uint32_t)((n + 63) / 64)), dim3(256), 0, ctx->stream, (const T*)part, (T*)dst, n, splits);
+    const dim3 grid((uint32_t)((n + 63) / 64));
+    // many splits of a small result: more waves for each, where blocks are few (512 splits of 64 x 64 f32 26 -> 22 us with the product; 85 of
+    // 256 x 320 would lose 2 us)
+    if (splits >= 32 && grid.x <= (uint32_t)ctx->num_cus) hipLaunchKernelGGL((pack8_matmul_join_kernel<T, 16>), grid, dim3(1024), 0, ctx->stream, (const T*)part, (T*)dst, n, splits);
+    else hipLaunchKernelGGL((pack8_matmul_join_kernel<T, 4>), grid, dim3(256), 0, ctx->stream, (const T*)part, (T*)dst, n, splits);
     RT_HIP(hipGetLastError());
     return RT_OK;
 }
@@ -434,9 +443,12 @@ template <int BI, int BJ, int WI, int WJ, int DEPTH, bool EVEN> int32_t f32_laun
 }
 
 template <bool EVEN> int32_t f32_any(rt_ctx* ctx, const Product& p, int shape) {
+    // steps that are on their way from memory: two, but for an odd k and its twice as many registers (65536 x 257 x 320 145 us with two,
+    // 90 us with one; 65536 x 256 x 320 50.3 and 51.1 us)
+    constexpr int kDepth = EVEN ? 2 : 1;
     if (shape == 0) return f32_launch<256, 256, 2, 4, 1, EVEN>(ctx, p);
-    if (shape == 1) return f32_launch<256, 128, 4, 2, 2, EVEN>(ctx, p);
-    return f32_launch<128, 128, 2, 2, 2, EVEN>(ctx, p);
+    if (shape == 1) return f32_launch<256, 128, 4, 2, kDepth, EVEN>(ctx, p);
+    return f32_launch<128, 128, 2, 2, kDepth, EVEN>(ctx, p);
 }
 
 int32_t run_product(rt_ctx* ctx, int dtype, Product p, void* dst) {
@@ -463,8 +475,8 @@ int32_t run_product(rt_ctx* ctx, int dtype, Product p, void* dst) {
     if (tiles >= (1ull << 24)) return rt_fail(RT_E_INVALID, "pack8 matmul backward: the result is too large for one launch");
     p.ti = (uint32_t)((p.k + s.bi - 1) / s.bi);
     p.tj = (uint32_t)((p.n + s.bj - 1) / s.bj);
-    p.splits = splits_for(ctx, tiles, p.m, s.least_rows, s.per_cu);
     const uint64_t n = p.b * p.k * p.n;
+    p.splits = splits_for(ctx, tiles, p.m, s.least_rows, s.per_cu);
     p.out = dst;
     if (p.splits > 1) RT_TRY(rt_scratch(ctx, n * p.splits * rt_elem_size(dtype), &p.out));
     if (dtype == RT_F64) {
