@@ -235,6 +235,15 @@ def test_in_place_and_equal_bits(hip, shape):
             assert got == plain, over
 
 
+@pytest.mark.parametrize("shape", [(20, 9000, 1), (6, 9000, 1), (17, 5000, 2), (3, 60, 70), (3, 110, 33)])
+def test_tiles_of_other_widths(hip, shape):
+    """The tests above where rows or steps give tiles of two, four, eight and sixteen waves."""
+    test_growing_gates(hip, shape)
+    test_in_place_and_equal_bits(hip, shape)
+    for form in ("linear", "sigmoid"):
+        test_nothing_crosses_a_reset(hip, form, shape)
+
+
 def test_no_steps_and_no_columns(hip):
     from rtensors_amd import hip as H
     st = np.arange(6, dtype=np.float32)
