@@ -757,8 +757,7 @@ __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void scan_narrow_kernel(Sc
     uint32_t next = rem0 == 0 ? 0u : a.steps - rem0 < 64 ? (uint32_t)(a.steps - rem0) : 64u;
     uint32_t heads = 0, cuts = 0;
     for (; next < (uint32_t)kSeg; next += steps) heads |= 1u << next;
-    if (v0 < cnt) heads &= cnt - v0 < (uint32_t)kSeg ? (1u << (cnt - v0)) - 1 : ~0u;
-    else heads = 0;
+    heads &= v0 >= cnt ? 0u : (1u << (cnt - v0 < nw.ls ? cnt - v0 : nw.ls)) - 1;            // of the segment's own steps
     if (a.reset)
         for (int j = 0; j < ls; ++j) cuts |= (tile.reset[v0 + j] ? 1u : 0u) << j;
     const uint32_t states = a.state && own ? heads & ~cuts : 0u; // steps that begin from a given state
@@ -893,8 +892,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
     uint32_t next = t_last + 1 == a.steps ? 0u : t_last + 1 < 64 ? (uint32_t)t_last + 1 : 64u;
     uint32_t tails = 0, cuts = 0;
     for (; next < (uint32_t)kSeg; next += steps) tails |= 1u << next;
-    if (q0 < cnt) tails &= cnt - q0 < (uint32_t)kSeg ? (1u << (cnt - q0)) - 1 : ~0u;
-    else tails = 0;
+    tails &= q0 >= cnt ? 0u : (1u << (cnt - q0 < nw.ls ? cnt - q0 : nw.ls)) - 1;
     if (a.reset)                                                 // a reset of the step behind
         for (int j = 0; j < ls; ++j) cuts |= (tile.reset[v0 - j + 1] ? 1u : 0u) << j;
     cuts |= tails;

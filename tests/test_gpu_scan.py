@@ -235,6 +235,15 @@ def test_in_place_and_equal_bits(hip, shape):
             assert got == plain, over
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("form", ["linear", "sigmoid"])
+@pytest.mark.parametrize("shape", [(1100, 74, 1), (3190, 48, 1), (2048, 100, 3), (1025, 9, 31), (2100, 20, 17), (600, 300, 1), (5000, 11, 2), (10000, 37, 5)])
+def test_short_rows_that_share_a_tile(hip, shape, form, dtype):
+    test_forward(hip, shape, form, dtype)
+    test_backward(hip, shape, False, form, dtype)
+    test_backward(hip, shape, True, form, dtype)
+
+
 @pytest.mark.parametrize("shape", [(20, 9000, 1), (6, 9000, 1), (17, 5000, 2), (3, 60, 70), (3, 110, 33)])
 def test_tiles_of_other_widths(hip, shape):
     """The tests above where rows or steps give tiles of two, four, eight and sixteen waves."""
