@@ -259,8 +259,10 @@ template <class T, int W, int LN> __device__ __forceinline__ T chain_start(const
         if (q <= found) {
             // an end state may have taken the place of a nearer tile's (A, H) meanwhile
             const uint64_t ends = __ballot(s[i].kind(ch.epoch) == kEnd);
-            room.winH[q][lane & (LN - 1)] = s[i].value(0);
-            room.winA[q][lane & (LN - 1)] = s[i].value(1);
+            if (lane < LN) {                                     // the lanes that repeat these may have read it before, these after
+                room.winH[q][lane] = s[i].value(0);
+                room.winA[q][lane] = s[i].value(1);
+            }
             if (lane == 0) room.ends[q] = ends;
         }
     }
@@ -278,7 +280,7 @@ template <class T, int W, int LN> __device__ __forceinline__ T chain_start(const
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (q0 - i >= 0) c = ends[i] >> lane & 1 ? H[i] : fused(A[i], c, H[i]);
+            if (q0 - i >= 0) c = ends[i] >> (lane & (LN - 1)) & 1 ? H[i] : fused(A[i], c, H[i]);
     }
     return c;
 }

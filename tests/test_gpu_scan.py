@@ -253,6 +253,23 @@ def test_tiles_of_other_widths(hip, shape):
         test_nothing_crosses_a_reset(hip, form, shape)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(62, 3241, 11), (23, 9280, 25), (4, 60664, 21), (30, 20000, 17), (1, 20000, 96), (3, 8000, 64)])
+def test_many_equal_calls_give_equal_bits(hip, shape, dtype):
+    """Tiles that hand states on meet each other at different moments in every call."""
+    n = int(np.prod(shape))
+    rng = np.random.default_rng(11)
+    T = TYPES[dtype]
+    gate, x = (put(hip, rng.random(n).astype(T)) for _ in range(2))
+    h, dg, dx, h2, dg2, dx2 = (poison(hip, np.empty(n, T)) for _ in range(6))
+    hip.gated_scan("linear", gate, x, h, *shape)
+    hip.gated_scan_backward("linear", gate, None, h, x, dg, dx, *shape)
+    for k in range(60):
+        hip.gated_scan("linear", gate, x, h2, *shape)
+        hip.gated_scan_backward("linear", gate, None, h, x, dg2, dx2, *shape)
+        assert hip.equal(h, h2) and hip.equal(dg, dg2) and hip.equal(dx, dx2), k
+
+
 def test_no_steps_and_no_columns(hip):
     from rtensors_amd import hip as H
     st = np.arange(6, dtype=np.float32)
