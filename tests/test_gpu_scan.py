@@ -244,7 +244,7 @@ def test_short_rows_that_share_a_tile(hip, shape, form, dtype):
     test_backward(hip, shape, True, form, dtype)
 
 
-@pytest.mark.parametrize("shape", [(20, 9000, 1), (6, 9000, 1), (17, 5000, 2), (3, 60, 70), (3, 110, 33)])
+@pytest.mark.parametrize("shape", [(20, 9000, 1), (6, 9000, 1), (17, 5000, 2), (3, 60, 70), (3, 110, 33), (1100, 74, 1), (1300, 100, 3)])
 def test_tiles_of_other_widths(hip, shape):
     """The tests above where rows or steps give tiles of two, four, eight and sixteen waves."""
     test_growing_gates(hip, shape)
