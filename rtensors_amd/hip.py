@@ -92,8 +92,7 @@ class HipView:
 
 
 class HipBuf(HipView):
-    """Owns `len` elements of `dtype` in device memory; returned to the context's allocator when dropped."""
-    __slots__ = ("__weakref__",)
+    """Owns `len` elements of `dtype` in device memory; returned to the context's allocator when dropped.  Takes attributes of its users'."""
 
     def __del__(self):
         try:
