@@ -72,6 +72,7 @@ struct Product {
     void* out;                        // dst, or the splits' partial results, each as large as dst
     uint64_t b, m, k, n;
     uint32_t ti, tj, splits;          // tiles of dst, shares of the rows
+    uint64_t batch0;                  // first batch of the launch
 };
 // Tile of a block: batch-major, then the splits; within one (batch, split) the tiles in bands of eight along i, so that blocks that run
 // at the same time on one XCD (every eighth block) share columns of both operands in its L2: XCD x takes the x-th eighth of the tiles.
@@ -84,7 +85,7 @@ __device__ __forceinline__ Where where(const Product& p) {
     Where w;
     const uint32_t bs = t / tiles;
     t -= bs * tiles;
-    w.batch = bs / p.splits;
+    w.batch = p.batch0 + bs / p.splits;
     w.split = bs % p.splits;
     const uint32_t band = t / (8 * p.tj), rows = p.ti - band * 8 < 8 ? p.ti - band * 8 : 8;
     t -= band * 8 * p.tj;
@@ -428,6 +429,19 @@ template <class T> int32_t join(rt_ctx* ctx, const void* part, void* dst, uint64
     return RT_OK;
 }
 
+// `launch(part, blocks)` for all batches, by blocks of `threads`, over as many launches as that takes: the lanes of a grid are numbered in
+// 32 bits.  More than one launch comes with one split only (few tiles are split).
+constexpr uint64_t kMostLanes = 1ull << 31;
+template <class Launch> int32_t batch_launches(Product p, uint32_t threads, Launch launch) {
+    const uint64_t per = (uint64_t)p.ti * p.tj * p.splits, most = kMostLanes / threads / per;
+    if (!most) return rt_fail(RT_E_INVALID, "pack8 matmul backward: the result is too large for one launch");
+    for (; p.batch0 < p.b; p.batch0 += most) {
+        launch(p, (uint32_t)((p.b - p.batch0 < most ? p.b - p.batch0 : most) * per));
+        RT_HIP(hipGetLastError());
+    }
+    return RT_OK;
+}
+
 template <int BI, int BJ, int WI, int WJ, int DEPTH, bool EVEN> int32_t f32_launch(rt_ctx* ctx, const Product& p) {
     constexpr size_t bytes = 2 * sizeof(Stage<BI, BJ>);
     auto kernel = pack8_matmul_f32_kernel<BI, BJ, WI, WJ, DEPTH, EVEN>;
@@ -437,9 +451,9 @@ template <int BI, int BJ, int WI, int WJ, int DEPTH, bool EVEN> int32_t f32_laun
         RT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
         allowed.fetch_or(bit);
     }
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(p.b * p.splits * p.ti * p.tj)), dim3(WI * WJ * 64), bytes, ctx->stream, p);
-    RT_HIP(hipGetLastError());
-    return RT_OK;
+    return batch_launches(p, WI * WJ * 64, [&](const Product& part, uint32_t blocks) {
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(WI * WJ * 64), bytes, ctx->stream, part);
+    });
 }
 
 template <bool EVEN> int32_t f32_any(rt_ctx* ctx, const Product& p, int shape) {
@@ -472,7 +486,6 @@ int32_t run_product(rt_ctx* ctx, int dtype, Product p, void* dst) {
         s = f32[shape];
     }
     const uint64_t tiles = tiles_of(s);
-    if (tiles >= (1ull << 24)) return rt_fail(RT_E_INVALID, "pack8 matmul backward: the result is too large for one launch");
     p.ti = (uint32_t)((p.k + s.bi - 1) / s.bi);
     p.tj = (uint32_t)((p.n + s.bj - 1) / s.bj);
     const uint64_t n = p.b * p.k * p.n;
@@ -480,9 +493,10 @@ int32_t run_product(rt_ctx* ctx, int dtype, Product p, void* dst) {
     p.out = dst;
     if (p.splits > 1) RT_TRY(rt_scratch(ctx, n * p.splits * rt_elem_size(dtype), &p.out));
     if (dtype == RT_F64) {
-        if (shape == 0) hipLaunchKernelGGL((pack8_matmul_f64_kernel<128, 4, 2>), dim3((uint32_t)(tiles * p.splits)), dim3(512), 0, ctx->stream, p);
-        else hipLaunchKernelGGL((pack8_matmul_f64_kernel<64, 2, 2>), dim3((uint32_t)(tiles * p.splits)), dim3(256), 0, ctx->stream, p);
-        RT_HIP(hipGetLastError());
+        RT_TRY(batch_launches(p, shape == 0 ? 512 : 256, [&](const Product& part, uint32_t blocks) {
+            if (shape == 0) hipLaunchKernelGGL((pack8_matmul_f64_kernel<128, 4, 2>), dim3(blocks), dim3(512), 0, ctx->stream, part);
+            else hipLaunchKernelGGL((pack8_matmul_f64_kernel<64, 2, 2>), dim3(blocks), dim3(256), 0, ctx->stream, part);
+        }));
     } else {
         RT_TRY(p.k % 2 == 0 ? f32_any<true>(ctx, p, shape) : f32_any<false>(ctx, p, shape));
     }
@@ -524,5 +538,5 @@ extern "C" int32_t rt_pack8_matmul_backward(rt_ctx* ctx, int32_t dtype, const vo
         return rt_fail(RT_E_INVALID, "%s: dst overlaps an input", what);
     RT_TRY(rt_ctx_enter(ctx));
     CtxGuard g(ctx);
-    return run_product(ctx, dtype, Product{(const int8_t*)codes, (const uint8_t*)exps, upstream, nullptr, b, m, k, n, 0, 0, 1}, dst);
+    return run_product(ctx, dtype, Product{(const int8_t*)codes, (const uint8_t*)exps, upstream, nullptr, b, m, k, n, 0, 0, 1, 0}, dst);
 }
