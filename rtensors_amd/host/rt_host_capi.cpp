@@ -277,6 +277,68 @@ int rth_gated_layer_step(void* x, void* w_gate, void* w_value, void* w_out, void
     });
 }
 
+// y = op(x + bias), op: RT_U_SIGMOID, RT_U_SILU, RT_U_TANH; loss = mean_l1_loss(y, target); backward, SGD(lr) on bias (updated in place).
+// train = 0: the loss alone, no node before it (out_grad is set to null).  out_kept: the bytes the tape kept.
+int rth_activation_step(void* x, void* bias, void* target, int op, double lr, int packed, int seed_with_loss, int train, void** out_loss, void** out_grad,
+                        uint64_t* out_kept) {
+    return guarded([&] {
+        grad::GradContext ctx;
+        ctx.seed_with_loss = seed_with_loss != 0;
+        ctx.packed_activations = packed != 0;
+        grad::Var vx = ctx.input(*(Tensor*)x), vt = ctx.input(*(Tensor*)target);
+        grad::Var vb = train ? ctx.param(*(Tensor*)bias) : ctx.input(*(Tensor*)bias);
+        grad::Var loss = ctx.mean_l1_loss(ctx.unary(ctx.add(vx, vb), op), vt);
+        *out_kept = ctx.kept_bytes();
+        *out_grad = nullptr;
+        if (train) {
+            grad::SGD opt(lr);
+            opt.register_parameter(ctx, vb);
+            ctx.backwards(loss);
+            std::shared_ptr<Tensor> g = ctx.grad_of(vb);
+            if (!g) throw TensorError(ErrorKind::GradError, "no gradient reached the bias");
+            Tensor grad_out = g->contiguous();
+            opt.step();
+            *out_grad = new Tensor(grad_out);
+        }
+        *out_loss = new Tensor(loss.t);
+    });
+}
+
+// h = gated_scan(x + bias, gate) along `axis` from `state` (null: zeros), loss = mean_l1_loss(h, target); backward, SGD(lr) on bias, gate
+// and state (updated in place).  train = 0: the loss alone, no node before it.  out_grads: d(bias), d(gate), d(state) (null where
+// there is none).  reset may be null; out_kept: the bytes the tape kept.
+int rth_scan_step(void* x, void* bias, void* gate, void* state, void* reset, void* target, uint64_t axis, int form, double lr, int packed, int seed_with_loss,
+                  int train, void** out_loss, void** out_grads, uint64_t* out_kept) {
+    return guarded([&] {
+        if (form != RT_SCAN_LINEAR && form != RT_SCAN_SIGMOID) throw TensorError(ErrorKind::UnsupportedOperation, "unknown scan form");
+        grad::GradContext ctx;
+        ctx.seed_with_loss = seed_with_loss != 0;
+        ctx.packed_activations = packed != 0;
+        const int n = state ? 3 : 2;
+        void* const from[3] = {bias, gate, state};
+        grad::Var vx = ctx.input(*(Tensor*)x), vt = ctx.input(*(Tensor*)target), p[3];
+        for (int k = 0; k < n; ++k) p[k] = train ? ctx.param(*(Tensor*)from[k]) : ctx.input(*(Tensor*)from[k]);
+        grad::Var h = ctx.gated_scan(ctx.add(vx, p[0]), p[1], (size_t)axis, (ScanForm)form, state ? &p[2] : nullptr, (Tensor*)reset);
+        grad::Var loss = ctx.mean_l1_loss(h, vt);
+        *out_kept = ctx.kept_bytes();
+        for (int k = 0; k < 3; ++k) out_grads[k] = nullptr;
+        if (train) {
+            grad::SGD opt(lr);
+            for (int k = 0; k < n; ++k) opt.register_parameter(ctx, p[k]);
+            ctx.backwards(loss);
+            Tensor grads[3];
+            for (int k = 0; k < n; ++k) {
+                std::shared_ptr<Tensor> g = ctx.grad_of(p[k]);
+                if (!g) throw TensorError(ErrorKind::GradError, "no gradient reached a parameter");
+                grads[k] = g->contiguous();
+            }
+            opt.step();
+            for (int k = 0; k < n; ++k) out_grads[k] = new Tensor(grads[k]);
+        }
+        *out_loss = new Tensor(loss.t);
+    });
+}
+
 // y = x @ w; loss = mean_l1_loss(y, target); backward; SGD(lr) on w (updated in place).  Outputs: loss and d(w).
 int rth_linear_step(void* x, void* w, void* target, double lr, int seed_with_loss, void** out_loss, void** out_grad) {
     return guarded([&] {

@@ -437,3 +437,24 @@ def gated_layer_step(x: Tensor, w_gate: Tensor, w_value: Tensor, w_out: Tensor, 
     _ck(_h.rth_gated_layer_step(x._p, w_gate._p, w_value._p, w_out._p, target._p, reset._p if reset is not None else None, C.c_double(lr), 1 if packed else 0,
                                 1 if seed_with_loss else 0, C.byref(pl), grads, C.byref(kept)))
     return Tensor(pl, x.backend), [Tensor(C.c_void_p(g), x.backend) for g in grads], kept.value
+
+
+def activation_step(x: Tensor, bias: Tensor, target: Tensor, op: str, lr: float, packed: bool = False, seed_with_loss: bool = True, train: bool = True):
+    """y = op(x + bias), op sigmoid, silu or tanh; loss = mean_l1_loss(y, target); backward; SGD(lr) on bias in place.  packed: the tape
+    keeps the input of op in 8 bits.  train=False: the loss alone, no node before it.  Returns (loss, d_bias or None, bytes the tape kept)."""
+    pl, pg, kept = C.c_void_p(), C.c_void_p(), C.c_uint64(0)
+    _ck(_h.rth_activation_step(x._p, bias._p, target._p, UNARY[op], C.c_double(lr), 1 if packed else 0, 1 if seed_with_loss else 0, 1 if train else 0,
+                               C.byref(pl), C.byref(pg), C.byref(kept)))
+    return Tensor(pl, x.backend), Tensor(pg, x.backend) if train else None, kept.value
+
+
+def scan_step(x: Tensor, bias: Tensor, gate: Tensor, target: Tensor, axis: int, form: str, lr: float, state: Optional[Tensor] = None,
+              reset: Optional[Tensor] = None, packed: bool = False, seed_with_loss: bool = True, train: bool = True):
+    """h = (x + bias).gated_scan(gate, axis, form, state, reset); loss = mean_l1_loss(h, target); backward; SGD(lr) on bias, gate and state
+    in place.  packed: the tape keeps the activations of the scan in 8 bits.  train=False: the loss alone, no node before it.  Returns
+    (loss, [d_bias, d_gate, d_state], bytes the tape kept); d_state is None without a state, all three with train=False."""
+    pl, kept, grads = C.c_void_p(), C.c_uint64(0), (C.c_void_p * 3)()
+    _ck(_h.rth_scan_step(x._p, bias._p, gate._p, state._p if state is not None else None, reset._p if reset is not None else None, target._p,
+                         C.c_uint64(axis), SCAN_FORM[form], C.c_double(lr), 1 if packed else 0, 1 if seed_with_loss else 0, 1 if train else 0,
+                         C.byref(pl), grads, C.byref(kept)))
+    return Tensor(pl, x.backend), [Tensor(C.c_void_p(g), x.backend) if g else None for g in grads], kept.value
