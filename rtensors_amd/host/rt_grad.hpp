@@ -278,11 +278,10 @@ class GradContext {
 
     // f'(x) of sigmoid, silu and tanh from the ordinary operators
     static Tensor slope(int op, const Tensor& x) {
-        if (op == RT_U_TANH) {                                   // 1 - tanh^2
-            Tensor t = x.tanh();
-            t.unary_inplace(RT_U_SQUARE);
-            t *= -1.0;
-            t += 1.0;
+        if (op == RT_U_TANH) {                                   // 1 - tanh(x)^2 = 4 s(2x) s(-2x), s the sigmoid: without a difference
+            Tensor two = x * 2.0;
+            Tensor t = two.sigmoid() * (-two).sigmoid();
+            t *= 4.0;
             return t;
         }
         const Tensor s = x.sigmoid(), rest = (-x).sigmoid();     // 1 - sigmoid(x) without a difference
