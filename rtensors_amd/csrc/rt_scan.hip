@@ -314,9 +314,11 @@ template <class T, int W, int LN> __device__ __forceinline__ uint32_t take_tile(
 // first: the state before tile 0.  `run(start, serial)` goes through the stretch from its start state and returns the state it ends at;
 // so does this function.
 //
-// A product of factors above 1 can leave the range while the states stay inside it (a start of zero, say).  Where one does, the tile's
-// stretches run one after the other and only its end state is published: the plain loop's result, at the plain loop's pace.
-template <class T, int W, int LN, class Run>
+// A product of factors above 1 can leave the range while the states stay inside it (a start of zero, say), and so can the sum from a start
+// of zero (a state of -c, and x of c twice).  Where one does, the tile's stretches run one after the other and only its end state is
+// published: the plain loop's result, at the plain loop's pace.  SUMS: whether the sums are looked at.  Those of the forward sigmoid form are
+// averages of x, which leave the range only where x has.
+template <class T, int W, int LN, bool SUMS, class Run>
 __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN>& room, uint32_t item, uint32_t k, T A, T H, bool cut, bool odd, T first, Run run) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const bool last = k == ch.tiles - 1;
@@ -336,7 +338,7 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN>& room
             tcut = true;
         } else {
             th = v == 0 ? hv : fused(av, th, hv);
-            bad = bad || !finite(av);
+            bad = bad || !finite(av) || (SUMS && !finite(th));
             if (!tcut) {
                 ta = v == 0 ? av : ta * av;
                 bad = bad || !finite(ta);
@@ -450,7 +452,7 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
     T first = k == 0 && a.state ? a.state[sc] : (T)0;
     RT_PIN_LANE(first);
     T* h = a.h + base;
-    const T end = join_tile(ch, room, item, k, A, H, cuts != 0, false, first, [&](T p, bool) {
+    const T end = join_tile<T, W, 64, FORM == RT_SCAN_LINEAR>(ch, room, item, k, A, H, cuts != 0, false, first, [&](T p, bool) {
         RT_APART;
         if (in) {
 #pragma unroll
@@ -581,7 +583,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
     T first = k == 0 && a.dlast ? a.dlast[sc] : (T)0;
     RT_PIN_LANE(first);
     T *dg = a.dgate + base, *dx = a.dx + base;
-    const T end = join_tile(ch, room, item, k, A, H, cuts != 0, false, first, [&](T d, bool) {
+    const T end = join_tile<T, W, 64, true>(ch, room, item, k, A, H, cuts != 0, false, first, [&](T d, bool) {
         RT_APART;
         uint64_t rresets = resets;
         RT_PIN(rresets);
@@ -658,8 +660,8 @@ template <class T> struct Prefix {
     T A, H, wholeA, wholeH;
     bool cut, any_cut, odd;
 };
-template <class T> __device__ __forceinline__ Prefix<T> join_lanes(T A, T H, bool cut, int lane, uint32_t shift) {
-    bool odd = !finite(A);
+template <bool SUMS, class T> __device__ __forceinline__ Prefix<T> join_lanes(T A, T H, bool cut, int lane, uint32_t shift) {
+    bool odd = !finite(A) || (SUMS && !cut && !finite(H));
     for (uint32_t d = 1u << shift; d < 64; d <<= 1) {
         const T A1 = __shfl_up(A, d), H1 = __shfl_up(H, d);
         const bool c1 = __shfl_up((int)cut, d) != 0;
@@ -667,7 +669,7 @@ template <class T> __device__ __forceinline__ Prefix<T> join_lanes(T A, T H, boo
             H = cut ? H : fused(A, H1, H);
             cut = cut || c1;
             A = cut ? (T)0 : A1 * A;
-            odd = odd || !finite(A);
+            odd = odd || !finite(A) || (SUMS && !cut && !finite(H));
         }
     }
     const int top = 64 - (1 << shift) + (lane & ((1 << shift) - 1));
@@ -803,8 +805,8 @@ __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void scan_narrow_kernel(Sc
         if (cuts) A = (T)0;
         if (!own) { A = (T)1; H = (T)0; cuts = 0; }
     }
-    const Prefix<T> pre = join_lanes(A, H, cuts != 0, lane, nw.shift);
-    join_tile(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
+    const Prefix<T> pre = join_lanes<FORM == RT_SCAN_LINEAR>(A, H, cuts != 0, lane, nw.shift);
+    join_tile<T, W, 32, FORM == RT_SCAN_LINEAR>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
         return run_lanes(pre, start, serial, lane, nw.shift, [&](T p) {
             RT_APART_LANES;
             if (own) {
@@ -918,8 +920,8 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
         if (cuts) A = (T)0;
         if (!own) { A = (T)1; H = (T)0; cuts = 0; }
     }
-    const Prefix<T> pre = join_lanes(A, H, cuts != 0, lane, nw.shift);
-    join_tile(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
+    const Prefix<T> pre = join_lanes<true>(A, H, cuts != 0, lane, nw.shift);
+    join_tile<T, W, 32, true>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
         return run_lanes(pre, start, serial, lane, nw.shift, [&](T d) {
             RT_APART_LANES;
             if (own) {
