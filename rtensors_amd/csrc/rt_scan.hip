@@ -136,11 +136,18 @@ struct Chain {
     uint32_t tiles;          // along the steps
     uint32_t lines;          // sets of columns that are chained on their own
     uint32_t line0;          // the first of them in the operands: a launch takes no more than its lanes can be numbered for
-    uint32_t epoch;          // the launch's number, 30 bits
+    uint32_t epoch;          // the launch's number, below kEpochs
     uint32_t rounds;         // blocks a line gets: `tiles`, or the next multiple of 8
 };
 constexpr uint32_t kTicketPitch = 16;
 constexpr uint32_t kAgg = 1, kEnd = 2;                           // what a slot holds: (A, H), or the end state in place of H
+// A tag: 17 bits of the launch's number, 13 of A's exponent (0 in the words of H), 2 of what the slot holds.
+constexpr uint32_t kEpochs = 1u << 17;
+constexpr int kTagExponent = 4095;
+__device__ __forceinline__ uint32_t tag_of(uint32_t epoch, uint32_t kind, int e = 0) { return epoch << 15 | ((uint32_t)e & 0x1fffu) << 2 | kind; }
+__device__ __forceinline__ uint32_t tag_epoch(uint32_t tag) { return tag >> 15; }
+__device__ __forceinline__ uint32_t tag_kind(uint32_t tag) { return tag & 3u; }
+__device__ __forceinline__ int tag_exponent(uint32_t tag) { return (int)(tag << 17) >> 19; }
 
 __device__ __forceinline__ void put_word(uint64_t* p, uint32_t bits, uint32_t tag) {
     __hip_atomic_store(p, (uint64_t)tag << 32 | bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -168,15 +175,19 @@ template <class T> struct Slot {
     // 0: not there (yet); the halves of a value may come from two writes, then it is read again
     __device__ __forceinline__ uint32_t kind(uint32_t epoch) const {
         const uint32_t t = (uint32_t)(w[0] >> 32);
-        bool ok = (t >> 2) == epoch;
+        bool ok = tag_epoch(t) == epoch;
         if constexpr (kHalves == 2) ok = ok && (uint32_t)(w[1] >> 32) == t;
-        const uint32_t k = t & 3u;
+        const uint32_t k = tag_kind(t);
         if (k == kAgg) {
 #pragma unroll
-            for (int j = kHalves; j < 2 * kHalves; ++j) ok = ok && (uint32_t)(w[j] >> 32) == (epoch << 2 | kAgg);
+            for (int j = kHalves; j < 2 * kHalves; ++j) {
+                const uint32_t a = (uint32_t)(w[j] >> 32);
+                ok = ok && tag_epoch(a) == epoch && tag_kind(a) == kAgg;
+            }
         }
         return ok ? k : 0u;
     }
+    __device__ __forceinline__ int exponent() const { return tag_exponent((uint32_t)(w[kHalves] >> 32)); }
     __device__ __forceinline__ T value(int which) const {
         if constexpr (kHalves == 1) return __builtin_bit_cast(float, (uint32_t)w[which]);
         else return __builtin_bit_cast(double, (uint64_t)(uint32_t)w[which * 2 + 1] << 32 | (uint32_t)w[which * 2]);
@@ -205,31 +216,123 @@ __device__ __forceinline__ double fused(double a, double b, double c) { return _
 __device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
 __device__ __forceinline__ bool finite(double v) { return __builtin_fabs(v) < __builtin_inf(); }
 
+__device__ __forceinline__ float mantissa(float v) { return __builtin_amdgcn_frexp_mantf(v); }
+__device__ __forceinline__ double mantissa(double v) { return __builtin_amdgcn_frexp_mant(v); }
+__device__ __forceinline__ int exponent(float v) { return __builtin_amdgcn_frexp_expf(v); }
+__device__ __forceinline__ int exponent(double v) { return __builtin_amdgcn_frexp_exp(v); }
+__device__ __forceinline__ float with_sign(float v, float of) { return __builtin_copysignf(v, of); }
+__device__ __forceinline__ double with_sign(double v, double of) { return __builtin_copysign(v, of); }
+__device__ __forceinline__ float scaled(float v, int e) { return __builtin_ldexpf(v, e); }
+__device__ __forceinline__ double scaled(double v, int e) { return __builtin_ldexp(v, e); }
+
+// The product A of a stretch's factors.
+// Those of the sigmoid form are at most 1: nothing lifts a product again that falls below the range.
+template <class T> struct Falling {
+    static constexpr bool kApart = false;
+    T m;
+    static __device__ __forceinline__ Falling of(T f) { return {f}; }
+    __device__ __forceinline__ T on(T c, T h) const { return fused(m, c, h); }           // A c + h
+};
+// Those of the linear form may be above 1 behind others far below it: a state of 2^100 times 2^-200 and then 2^150 is 2^50.  A product below
+// the normal range is held as m 2^e, m at the range's lower end and e < 0; any other one as it is, with e = 0.  An infinite m says that a
+// prefix of the stretch is above the range; such a tile runs step by step.
+template <class T> struct Apart {
+    static constexpr bool kApart = true;
+    static constexpr T kNormal = sizeof(T) == 4 ? (T)0x1p-126 : (T)0x1p-1022;
+    static constexpr int kLow = sizeof(T) == 4 ? -125 : -1021, kTop = sizeof(T) == 4 ? 128 : 1024;
+    static constexpr int kDead = sizeof(T) == 4 ? -300 : -2200;  // below, A c is 0 for every number c
+    T m;
+    int e;
+    static __device__ __forceinline__ Apart of(T f) { return {f, 0}; }
+    // m 2^e of any m and e (above the range, e > 0: where a tile's product sinks below the range first, which no wave's own does)
+    static __device__ __forceinline__ Apart from(T m, int e) {
+        const int at = e + exponent(m), near = at < kLow ? kLow : at > kTop ? kTop : at;
+        return {scaled(mantissa(m), near), at - near};
+    }
+    __device__ __forceinline__ T on(T c, T h) const { return fused(m, scaled(c, e), h); }
+};
+template <class T, int FORM> using ProductOf = typename std::conditional<FORM == RT_SCAN_LINEAR, Apart<T>, Falling<T>>::type;
+
+// The product of the factors that a lane goes through, multiplied as they come; where a prefix in the wave fell below the range (or a factor
+// is 0), once more with the exponents apart.  (Exponents apart in every step: 51 -> 64 us on (2048, 4097, 1) f64.)
+__device__ __forceinline__ float least(float a, float b) { return __builtin_fminf(a, __builtin_fabsf(b)); }
+__device__ __forceinline__ double least(double a, double b) { return __builtin_fmin(a, __builtin_fabs(b)); }
+template <class T, class P> struct Running {
+    T m = (T)1, low = (T)1;
+    __device__ __forceinline__ void by(T f) {
+        m *= f;
+        if constexpr (P::kApart) low = least(low, m);
+    }
+    // factor(j) is factor j of the first n of L; odd: a prefix is above the range, or nearly (an infinite m says so itself)
+    template <int L, class F> __device__ __forceinline__ P whole(int n, F factor, bool* odd) const {
+        *odd = false;
+        if constexpr (P::kApart) {
+            if (__any(low < P::kNormal)) {
+                T p = (T)1;
+                int e = 0;
+#pragma unroll
+                for (int j = 0; j < L; ++j)
+                    if (j < n) {
+                        p *= mantissa(factor(j));
+                        e += exponent(factor(j));
+                        *odd = *odd || e > P::kTop;
+                    }
+                return P::from(p, e);
+            }
+        }
+        return P::of(m);
+    }
+};
+
 // LN: lanes that hold different columns; with 32 the upper half of a wave repeats the lower one.
-template <class T, int W, int LN> struct JoinRoom {
+template <class T, int W, int LN, class P> struct JoinRoom {
     // tiles before its own that a tile looks at (f64: as many as leave room for the blocks that the registers allow)
     static constexpr int kWindow = W <= 2 ? 1 : sizeof(T) == 4 || W == 16 ? 16 : LN == 32 && W == 8 ? 4 : 8;
-    T A[W][LN], H[W][LN], start[LN];
+    T A[W][LN], H[W][LN];
+    union {
+        T start[LN];                                             // of serial tiles, which need no products
+        int16_t E[P::kApart ? W : 1][LN];
+    };
     T winA[kWindow][LN], winH[kWindow][LN];
-    uint64_t ends[kWindow];
-    uint32_t cut[W];
+    int16_t winE[P::kApart ? kWindow : 1][LN];
+    uint64_t ends[P::kApart ? 1 : kWindow];
+    uint32_t cut[W];                                             // 1: cut, 2: odd, 4: deep
     uint32_t tile;
     int found;
+    // a wave's product and its exponent: that of m 2^e as a whole, kZero for 0, and those from -2^15 on are all the same: the other waves of
+    // a tile lift no state again that far
+    static constexpr int kZero = 1 << 14;
+    __device__ __forceinline__ void put(int w, int l, const P& a) {
+        A[w][l] = a.m;
+        if constexpr (P::kApart) {
+            const int e = a.m == (T)0 ? kZero : a.e + exponent(a.m);
+            E[w][l] = (int16_t)(e < -32768 ? -32768 : e);
+        }
+    }
+    __device__ __forceinline__ P get(int w, int l) const {
+        if constexpr (P::kApart) {
+            const int e = E[w][l] - P::kLow;
+            return P{A[w][l], e < 0 ? e : 0};
+        } else {
+            return P{A[w][l]};
+        }
+    }
 };
+constexpr int16_t kEnded = 0x7fff;                               // in place of an exponent: H is the end state
 
 // The end state of tile k - 1 for this lane's column, for all waves of the block.  Waiting is done by one wave on one word of each of the
 // tiles in the window, read by one lane each: polling whole slots takes the bandwidth that the tiles being waited for need.  Then the
 // waves read the slots between them, again where not all of their words are there yet, and go through them from the farthest.
-template <class T, int W, int LN> __device__ __forceinline__ T chain_start(const Chain& ch, JoinRoom<T, W, LN>& room, uint32_t item, uint32_t k, int w, int lane) {
-    constexpr int kWindow = JoinRoom<T, W, LN>::kWindow, kEach = (kWindow + W - 1) / W;
+template <class T, int W, int LN, class P> __device__ __forceinline__ T chain_start(const Chain& ch, JoinRoom<T, W, LN, P>& room, uint32_t item, uint32_t k, int w, int lane) {
+    constexpr int kWindow = JoinRoom<T, W, LN, P>::kWindow, kEach = (kWindow + W - 1) / W;
     if (w == 0) {
         const int n = k < (uint32_t)kWindow ? (int)k : kWindow;
         int found;                                               // nearest tile with an end state, all nearer ones having (A, H)
         for (;;) {
             uint32_t tag = 0;
             if (lane < n) tag = (uint32_t)(get_word(Slot<T>::at(ch, item - (uint32_t)(lane + 1) * ch.lines)) >> 32);
-            const bool mine = lane < n && (tag >> 2) == ch.epoch;
-            const uint64_t ends = __ballot(mine && (tag & 3u) == kEnd), aggs = __ballot(mine && (tag & 3u) == kAgg);
+            const bool mine = lane < n && tag_epoch(tag) == ch.epoch;
+            const uint64_t ends = __ballot(mine && tag_kind(tag) == kEnd), aggs = __ballot(mine && tag_kind(tag) == kAgg);
             found = ends ? (int)__builtin_ctzll(ends) : -1;
             if (found >= 0 && (~aggs & ((1ull << found) - 1)) == 0) break;
             __builtin_amdgcn_s_sleep(2);
@@ -258,29 +361,38 @@ template <class T, int W, int LN> __device__ __forceinline__ T chain_start(const
         const int q = w + i * W;
         if (q <= found) {
             // an end state may have taken the place of a nearer tile's (A, H) meanwhile
-            const uint64_t ends = __ballot(s[i].kind(ch.epoch) == kEnd);
+            const bool ended = s[i].kind(ch.epoch) == kEnd;
+            const uint64_t ends = __ballot(ended);
             if (lane < LN) {                                     // the lanes that repeat these may have read it before, these after
                 room.winH[q][lane] = s[i].value(0);
                 room.winA[q][lane] = s[i].value(1);
+                if constexpr (P::kApart) room.winE[q][lane] = ended ? kEnded : (int16_t)s[i].exponent();
             }
-            if (lane == 0) room.ends[q] = ends;
+            if constexpr (!P::kApart)
+                if (lane == 0) room.ends[q] = ends;
         }
     }
     __syncthreads();
     T c = (T)0;
+#pragma unroll 1
     for (int q0 = found; q0 >= 0; q0 -= 4) {                     // four at a time are read before the first is used
         T A[4], H[4];
         uint64_t ends[4];
+        int e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int q = q0 - i < 0 ? 0 : q0 - i;
             A[i] = room.winA[q][lane & (LN - 1)];
             H[i] = room.winH[q][lane & (LN - 1)];
-            ends[i] = room.ends[q];
+            if constexpr (P::kApart) e[i] = room.winE[q][lane & (LN - 1)];
+            else ends[i] = room.ends[q];
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (q0 - i >= 0) c = ends[i] >> (lane & (LN - 1)) & 1 ? H[i] : fused(A[i], c, H[i]);
+            if (q0 - i >= 0) {
+                if constexpr (P::kApart) c = e[i] == kEnded ? H[i] : P{A[i], e[i]}.on(c, H[i]);
+                else c = ends[i] >> (lane & (LN - 1)) & 1 ? H[i] : fused(A[i], c, H[i]);
+            }
     }
     return c;
 }
@@ -297,7 +409,7 @@ template <bool SPREAD> __device__ __forceinline__ uint32_t line_of_block(const C
 }
 // The block's tile among those of its line (one that is not there for the blocks too many); whoever takes the last one leaves the counter
 // as the next launch needs it.
-template <class T, int W, int LN> __device__ __forceinline__ uint32_t take_tile(const Chain& ch, uint32_t line, JoinRoom<T, W, LN>& room) {
+template <class T, int W, int LN, class P> __device__ __forceinline__ uint32_t take_tile(const Chain& ch, uint32_t line, JoinRoom<T, W, LN, P>& room) {
     if (ch.tiles == 1) return 0;
     if (threadIdx.x == 0) {
         uint32_t* c = ch.tickets + (uint64_t)line * kTicketPitch;
@@ -318,49 +430,97 @@ template <class T, int W, int LN> __device__ __forceinline__ uint32_t take_tile(
 // of zero (a state of -c, and x of c twice).  Where one does, the tile's stretches run one after the other and only its end state is
 // published: the plain loop's result, at the plain loop's pace.  SUMS: whether the sums are looked at.  Those of the forward sigmoid form are
 // averages of x, which leave the range only where x has.
-template <class T, int W, int LN, bool SUMS, class Run>
-__device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN>& room, uint32_t item, uint32_t k, T A, T H, bool cut, bool odd, T first, Run run) {
+template <class T, int W, int LN, bool SUMS, class P, class Run>
+__device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN, P>& room, uint32_t item, uint32_t k, const P& A, T H, bool cut, bool odd, T first, Run run) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const bool last = k == ch.tiles - 1;
-    room.A[w][lane & (LN - 1)] = A;
+    room.put(w, lane & (LN - 1), A);
     room.H[w][lane & (LN - 1)] = H;
-    if (lane == 0) room.cut[w] = (cut ? 1u : 0u) | (odd ? 2u : 0u);
+    bool deep = false;
+    if constexpr (P::kApart) deep = !cut && __any(A.e < 0);
+    if (lane == 0) room.cut[w] = (cut ? 1u : 0u) | (odd ? 2u : 0u) | (deep ? 4u : 0u);
     __syncthreads();
     const uint32_t epoch = ch.epoch;
-    T ta = (T)1, th = (T)0;
+    if constexpr (P::kApart) deep = __any((room.cut[lane & (W - 1)] & 4u) != 0);         // from here on: of the tile
+    T ta = (T)1, th = (T)0, low = (T)1;
     bool tcut = false, bad = false;
+    if (!deep) {
 #pragma unroll
-    for (int v = 0; v < W; ++v) {
-        const T av = room.A[v][lane & (LN - 1)], hv = room.H[v][lane & (LN - 1)];
-        bad = bad || (room.cut[v] & 2u);
-        if (room.cut[v] & 1u) {
-            th = hv;
-            tcut = true;
-        } else {
-            th = v == 0 ? hv : fused(av, th, hv);
-            bad = bad || !finite(av) || (SUMS && !finite(th));
-            if (!tcut) {
-                ta = v == 0 ? av : ta * av;
-                bad = bad || !finite(ta);
+        for (int v = 0; v < W; ++v) {
+            const T av = room.A[v][lane & (LN - 1)], hv = room.H[v][lane & (LN - 1)];
+            bad = bad || (room.cut[v] & 2u);
+            if (room.cut[v] & 1u) {
+                th = hv;
+                tcut = true;
+            } else {
+                th = v == 0 ? hv : fused(av, th, hv);
+                bad = bad || !finite(av) || (SUMS && !finite(th));
+                if (!tcut) {
+                    ta = v == 0 ? av : ta * av;
+                    if constexpr (P::kApart) low = least(low, ta);
+                    bad = bad || !finite(ta);
+                }
+            }
+        }
+    } else if constexpr (P::kApart) {
+#pragma unroll
+        for (int v = 0; v < W; ++v) {
+            const P av = room.get(v, lane & (LN - 1));
+            const T hv = room.H[v][lane & (LN - 1)];
+            bad = bad || (room.cut[v] & 2u);
+            if (room.cut[v] & 1u) {
+                th = hv;
+                tcut = true;
+            } else {
+                th = v == 0 ? hv : av.on(th, hv);
+                bad = bad || !finite(av.m) || (SUMS && !finite(th));
+                if (!tcut) {
+                    ta = v == 0 ? av.m : ta * av.m;
+                    if constexpr (P::kApart) low = least(low, ta);
+                    bad = bad || !finite(ta);
+                }
             }
         }
     }
     const bool serial = __any(bad);                              // the same in all waves: they look at the same numbers
     uint64_t* slot = last ? nullptr : Slot<T>::at(ch, item) + lane;
     T start = first;
+    P whole = P::of(ta);
+    if constexpr (P::kApart)
+        if (w == 0 && !last && !serial && !tcut && (deep || __any(low < P::kNormal))) {  // with the exponents apart
+            int e = 0;
+#pragma unroll
+            for (int v = 0; v < W; ++v) e += room.E[v][lane & (LN - 1)];
+            whole = {with_sign(P::kNormal, ta), e};              // nothing is left of any state
+            if (__any(e > P::kDead)) {
+                T p = (T)1;
+                e = 0;
+#pragma unroll 4
+                for (int v = 0; v < W; ++v) {
+                    const P av = room.get(v, lane & (LN - 1));
+                    p *= mantissa(av.m);
+                    e += exponent(av.m) + av.e;
+                }
+                whole = P::from(p, e);
+            }
+        }
     if (w == 0 && !last && !serial) {
-        if (tcut) Slot<T>::put(slot, 0, th, epoch << 2 | kEnd);
-        else if (k == 0) Slot<T>::put(slot, 0, fused(ta, first, th), epoch << 2 | kEnd);
+        if (tcut) Slot<T>::put(slot, 0, th, tag_of(epoch, kEnd));
+        else if (k == 0) Slot<T>::put(slot, 0, whole.on(first, th), tag_of(epoch, kEnd));
         else {
-            Slot<T>::put(slot, 1, ta, epoch << 2 | kAgg);
-            Slot<T>::put(slot, 0, th, epoch << 2 | kAgg);
+            // beyond kTagExponent, exponents are all the same to a state: nothing is left of it, or it is infinite
+            int e = 0;
+            if constexpr (P::kApart) e = whole.e < -kTagExponent ? -kTagExponent : whole.e > kTagExponent ? kTagExponent : whole.e;
+            Slot<T>::put(slot, 1, whole.m, tag_of(epoch, kAgg, e));
+            Slot<T>::put(slot, 0, th, tag_of(epoch, kAgg));
         }
     }
     if (W > 1 && k > 0) {                                        // a tile of one wave is the only one of its line
         start = chain_start(ch, room, item, k, w, lane);
-        if (w == 0 && !last && !serial && !tcut) Slot<T>::put(slot, 0, fused(ta, start, th), epoch << 2 | kEnd);
+        if (w == 0 && !last && !serial && !tcut) Slot<T>::put(slot, 0, whole.on(start, th), tag_of(epoch, kEnd));
     }
     if (serial) {
+        __syncthreads();                                         // the room of the start is that of the exponents
         if (w == 0) room.start[lane & (LN - 1)] = start;
         __syncthreads();
     }
@@ -369,14 +529,18 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN>& room
         if (!serial || turn == w) {
             if (serial) start = room.start[lane & (LN - 1)];
             else {
-                for (int v = 0; v < w; ++v) start = room.cut[v] & 1u ? room.H[v][lane & (LN - 1)] : fused(room.A[v][lane & (LN - 1)], start, room.H[v][lane & (LN - 1)]);
+                if (deep) {
+                    for (int v = 0; v < w; ++v) start = room.cut[v] & 1u ? room.H[v][lane & (LN - 1)] : room.get(v, lane & (LN - 1)).on(start, room.H[v][lane & (LN - 1)]);
+                } else {
+                    for (int v = 0; v < w; ++v) start = room.cut[v] & 1u ? room.H[v][lane & (LN - 1)] : fused(room.A[v][lane & (LN - 1)], start, room.H[v][lane & (LN - 1)]);
+                }
             }
             end = run(start, serial);
             if (serial) room.start[lane & (LN - 1)] = end;
         }
         if (serial) __syncthreads();
     }
-    if (serial && w == 0 && !last) Slot<T>::put(slot, 0, room.start[lane & (LN - 1)], epoch << 2 | kEnd);
+    if (serial && w == 0 && !last) Slot<T>::put(slot, 0, room.start[lane & (LN - 1)], tag_of(epoch, kEnd));
     return end;
 }
 
@@ -404,7 +568,8 @@ __device__ __forceinline__ uint64_t reset_bits(const uint8_t* flags, int64_t str
 // neither use nor store it.
 template <class T, int FORM, int W, int L, bool ALIGNED>
 __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain ch, uint32_t col_blocks) {
-    __shared__ JoinRoom<T, W, 64> room;
+    typedef ProductOf<T, FORM> P;
+    __shared__ JoinRoom<T, W, 64, P> room;
     const uint32_t line = line_of_block<true>(ch), k = take_tile(ch, line, room), item = k * ch.lines + line, at_line = ch.line0 + line, o = at_line / col_blocks;
     if (k >= ch.tiles) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -415,7 +580,9 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
     const int n = t0 >= a.steps ? 0 : (a.steps - t0 < (uint64_t)L ? (int)(a.steps - t0) : L);   // steps of this wave
     const uint64_t base = ((uint64_t)o * a.steps + t0) * row + col0;                            // wave-uniform
     const uint64_t sc = (uint64_t)o * row + col0 + lc;                                          // the column in (outer, inner)
-    T f[L], b[L], A = (T)1, H = (T)0;
+    T f[L], b[L], H = (T)0;
+    P A = P::of((T)1);
+    bool odd = false;
     uint64_t cuts = t0 == 0 && !a.state ? 1 : 0;
     if (n) {
         const T *gate = a.gate + base, *x = a.x + base;
@@ -436,6 +603,7 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
             }
         }
         if (a.reset) cuts |= reset_bits(a.reset + (uint64_t)o * a.steps + t0, 1, n, lane);
+        Running<T, P> run;
 #pragma unroll
         for (int j = 0; j < L; ++j) {
             if constexpr (FORM == RT_SCAN_SIGMOID) {
@@ -445,14 +613,15 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
             }
             if (j < n) {
                 H = j == 0 || (cuts >> j & 1) ? b[j] : fused(f[j], H, b[j]);
-                A = j == 0 ? f[j] : A * f[j];
+                run.by(f[j]);
             }
         }
+        A = run.template whole<L>(n, [&](int j) { return f[j]; }, &odd);
     }
     T first = k == 0 && a.state ? a.state[sc] : (T)0;
     RT_PIN_LANE(first);
     T* h = a.h + base;
-    const T end = join_tile<T, W, 64, FORM == RT_SCAN_LINEAR>(ch, room, item, k, A, H, cuts != 0, false, first, [&](T p, bool) {
+    const T end = join_tile<T, W, 64, FORM == RT_SCAN_LINEAR>(ch, room, item, k, A, H, cuts != 0, cuts == 0 && __any(odd), first, [&](T p, bool) {
         RT_APART;
         if (in) {
 #pragma unroll
@@ -512,7 +681,8 @@ struct NoRows {};
 // that one's gate.
 template <class T, int FORM, class S, int W, int L, bool ALIGNED>
 __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, S> a, Chain ch, uint32_t col_blocks) {
-    __shared__ JoinRoom<T, W, 64> room;
+    typedef ProductOf<T, FORM> P;
+    __shared__ JoinRoom<T, W, 64, P> room;
     constexpr bool kHeld = S::kHeld, kSigmoid = FORM == RT_SCAN_SIGMOID;
     typedef typename std::conditional<kHeld, HeldRows<L>, NoRows>::type Rows;
     __shared__ Rows hrows[W], xrows[kSigmoid ? W : 1];
@@ -528,7 +698,9 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
     const bool top = te == 0;
     const uint64_t base = ((uint64_t)o * a.steps + te) * row + col0;                            // of the earliest step: j is n - 1 - j rows on
     const uint64_t sc = (uint64_t)o * row + col0 + lc;
-    T g[L], up[L], hp[kHeld ? 1 : L], xv[kHeld || !kSigmoid ? 1 : L], s[L], f0 = (T)1, A = (T)1, H = (T)0;
+    T g[L], up[L], hp[kHeld ? 1 : L], xv[kHeld || !kSigmoid ? 1 : L], s[L], f0 = (T)1, H = (T)0;
+    P A = P::of((T)1);
+    bool odd = false;
     T st = (T)0;                                                 // the state before step 0
     uint64_t resets = 0, cuts = 0;                               // bit j: step j is reset; the step behind j is
     if (n) {
@@ -561,6 +733,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
         if constexpr (FORM == RT_SCAN_SIGMOID)
             if (r0 > 0) f0 = gate_of(f0).s;
         T f = f0;
+        Running<T, P> run;
 #pragma unroll
         for (int j = 0; j < L; ++j) {
             s[j] = g[j];
@@ -571,10 +744,11 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
             }
             if (j < n) {
                 H = j == 0 || (cuts >> j & 1) ? up[j] : fused(f, H, up[j]);
-                A = j == 0 ? f : A * f;
+                run.by(f);
             }
             f = s[j];
         }
+        A = run.template whole<L>(n, [&](int j) { return j == 0 ? f0 : s[j ? j - 1 : 0]; }, &odd);
         if constexpr (kHeld) {
             hrows[w].put(hv, lane);
             if constexpr (kSigmoid) xrows[w].put(xh, lane);
@@ -583,7 +757,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
     T first = k == 0 && a.dlast ? a.dlast[sc] : (T)0;
     RT_PIN_LANE(first);
     T *dg = a.dgate + base, *dx = a.dx + base;
-    const T end = join_tile<T, W, 64, true>(ch, room, item, k, A, H, cuts != 0, false, first, [&](T d, bool) {
+    const T end = join_tile<T, W, 64, true>(ch, room, item, k, A, H, cuts != 0, cuts == 0 && __any(odd), first, [&](T d, bool) {
         RT_APART;
         uint64_t rresets = resets;
         RT_PIN(rresets);
@@ -656,42 +830,82 @@ template <class TT, int W> size_t tile_bytes(const Narrow& nw, bool reset) {
 }
 template <class TT> constexpr size_t most_tile_bytes() { return offsetof(TT, reset) + TT::kMost + 1; }
 // What joins a wave's segments: the exclusive prefix of the lane's segment, and the wave's whole.
-template <class T> struct Prefix {
-    T A, H, wholeA, wholeH;
+template <class T, class P> struct Prefix {
+    P A, wholeA;
+    T H, wholeH;
     bool cut, any_cut, odd;
 };
-template <bool SUMS, class T> __device__ __forceinline__ Prefix<T> join_lanes(T A, T H, bool cut, int lane, uint32_t shift) {
-    bool odd = !finite(A) || (SUMS && !cut && !finite(H));
+template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Falling<T>> join_lanes(Falling<T> A, T H, bool cut, bool, int lane, uint32_t shift) {
+    bool odd = !finite(A.m);
+    if (cut) A.m = (T)0;
     for (uint32_t d = 1u << shift; d < 64; d <<= 1) {
-        const T A1 = __shfl_up(A, d), H1 = __shfl_up(H, d);
+        const T A1 = __shfl_up(A.m, d), H1 = __shfl_up(H, d);
         const bool c1 = __shfl_up((int)cut, d) != 0;
         if (lane >= (int)d) {
-            H = cut ? H : fused(A, H1, H);
+            H = cut ? H : fused(A.m, H1, H);
             cut = cut || c1;
-            A = cut ? (T)0 : A1 * A;
-            odd = odd || !finite(A) || (SUMS && !cut && !finite(H));
+            A.m = cut ? (T)0 : A1 * A.m;
+            odd = odd || !finite(A.m);
         }
     }
+    odd = odd || (SUMS && !finite(H));                           // a sum that was not finite on the way has stayed so
     const int top = 64 - (1 << shift) + (lane & ((1 << shift) - 1));
-    Prefix<T> p;
-    p.wholeA = __shfl(A, top);
+    Prefix<T, Falling<T>> p;
+    p.wholeA = {__shfl(A.m, top)};
     p.wholeH = __shfl(H, top);
     p.any_cut = __any(cut);
     p.odd = __any(odd);
-    const T A0 = __shfl_up(A, 1u << shift), H0 = __shfl_up(H, 1u << shift);
+    const T A0 = __shfl_up(A.m, 1u << shift), H0 = __shfl_up(H, 1u << shift);
     const bool c0 = __shfl_up((int)cut, 1u << shift) != 0;
     const bool head = lane < (1 << shift);
-    p.A = head ? (T)1 : A0;
+    p.A = {head ? (T)1 : A0};
     p.H = head ? (T)0 : H0;
     p.cut = !head && c0;
     return p;
 }
+// The same with the exponents apart: m 2^e, m at least 1, so that scaled(H1, e) leaves the range only where the product does.  Whether the
+// stretch is cut goes from lane to lane in the exponent's lowest bit.
+template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Apart<T>> join_lanes(Apart<T> A, T H, bool cut, bool odd, int lane, uint32_t shift) {
+    T m = mantissa(A.m) * (T)2;
+    int e = exponent(A.m) + A.e - 1;
+    odd = odd || (!cut && !finite(m));
+    for (uint32_t d = 1u << shift; d < 64; d <<= 1) {
+        const T m1 = __shfl_up(m, d), H1 = __shfl_up(H, d);
+        const int both = __shfl_up(e * 2 + (cut ? 1 : 0), d);
+        if (lane >= (int)d) {
+            H = cut ? H : fused(m, scaled(H1, e), H);
+            cut = cut || (both & 1);
+            m *= m1;
+            e += both >> 1;
+            if (d & 0x12) {                                      // m stays below 2^8: scaled(H1, e) loses at most 2^-142, f64 2^-1067
+                e += exponent(m) - 1;
+                m = mantissa(m) * (T)2;
+            }
+        }
+    }
+    // a sum that was not finite on the way has stayed so; each lane has the product of a prefix
+    odd = odd || (!cut && e > Apart<T>::kTop) || (SUMS && !finite(H));
+    const int top = 64 - (1 << shift) + (lane & ((1 << shift) - 1));
+    const Apart<T> a = Apart<T>::from(m, e);
+    Prefix<T, Apart<T>> p;
+    p.wholeA = {__shfl(a.m, top), __shfl(a.e, top)};
+    p.wholeH = __shfl(H, top);
+    p.any_cut = __any(cut);
+    p.odd = __any(odd);
+    const T m0 = __shfl_up(a.m, 1u << shift), H0 = __shfl_up(H, 1u << shift);
+    const int both = __shfl_up(a.e * 2 + (cut ? 1 : 0), 1u << shift);
+    const bool head = lane < (1 << shift);
+    p.A = {head ? (T)1 : m0, head ? 0 : both >> 1};
+    p.H = head ? (T)0 : H0;
+    p.cut = !head && (both & 1);
+    return p;
+}
 // Runs a wave's segments from the wave's start state: `go(start)` goes through the lane's segment and returns where it ends.
-template <class T, class Go> __device__ __forceinline__ T run_lanes(const Prefix<T>& p, T start, bool serial, int lane, uint32_t shift, Go go) {
+template <class T, class P, class Go> __device__ __forceinline__ T run_lanes(const Prefix<T, P>& p, T start, bool serial, int lane, uint32_t shift, Go go) {
     const int c = lane & ((1 << shift) - 1), seg = lane >> shift;
     T end = start;
     for (int s = 0; s < (serial ? 64 >> shift : 1); ++s) {
-        if (!serial) end = go(seg == 0 ? start : p.cut ? p.H : fused(p.A, start, p.H));
+        if (!serial) end = go(seg == 0 ? start : p.cut ? p.H : p.A.on(start, p.H));
         else {
             if (seg == s) end = go(start);
             start = __shfl(end, (s << shift) + c);
@@ -717,7 +931,8 @@ __device__ __forceinline__ int tile_segment(int tid, uint32_t shift) { return (t
 template <class T, int FORM, int W>
 __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void scan_narrow_kernel(ScanArgs<T> a, Chain ch, Narrow nw) {
     constexpr int kSeg = seg_steps<T>(), kThreads = W * 64;
-    __shared__ JoinRoom<T, W, 32> room;                          // inner is below 32
+    typedef ProductOf<T, FORM> P;
+    __shared__ JoinRoom<T, W, 32, P> room;                       // inner is below 32
     extern __shared__ __align__(16) char lds[];
     typedef ForwardTile<T, W> TT;
     TT& tile = *reinterpret_cast<TT*>(lds);
@@ -767,7 +982,8 @@ __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void scan_narrow_kernel(Sc
     const uint32_t states = a.state && own ? heads & ~cuts : 0u; // steps that begin from a given state
     cuts |= heads;
     const uint64_t place = (row0 + row_of) * inner + c;          // in (outer, inner), of the segment's first row
-    T f[kSeg], b[kSeg], A = (T)1, H = (T)0;
+    T f[kSeg], b[kSeg], H = (T)0;
+    Running<T, P> run;
     {
         uint32_t e = v0 * inner + c;
 #pragma unroll
@@ -799,13 +1015,14 @@ __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void scan_narrow_kernel(Sc
                 if (states >> j & 1)                             // rows on from the first: heads up to here, the one at 0 being the first's own
                     b[j] = fused(f[j], a.state[place + (uint64_t)__popc(heads & ((2u << j) - 1u) & ~1u) * inner], b[j]);
                 H = j == 0 || (cuts >> j & 1) ? b[j] : fused(f[j], H, b[j]);
-                A *= f[j];
+                run.by(f[j]);
             }
         }
-        if (cuts) A = (T)0;
-        if (!own) { A = (T)1; H = (T)0; cuts = 0; }
     }
-    const Prefix<T> pre = join_lanes<FORM == RT_SCAN_LINEAR>(A, H, cuts != 0, lane, nw.shift);
+    bool odd;
+    P A = run.template whole<kSeg>(ls, [&](int j) { return f[j]; }, &odd);
+    if (!own) { A = P::of((T)1); H = (T)0; cuts = 0; }
+    const Prefix<T, P> pre = join_lanes<FORM == RT_SCAN_LINEAR>(A, H, cuts != 0, own && cuts == 0 && odd, lane, nw.shift);
     join_tile<T, W, 32, FORM == RT_SCAN_LINEAR>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
         return run_lanes(pre, start, serial, lane, nw.shift, [&](T p) {
             RT_APART_LANES;
@@ -843,7 +1060,8 @@ __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void scan_narrow_kernel(Sc
 template <class T, int FORM, class S, int W>
 __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T, S> a, Chain ch, Narrow nw) {
     constexpr int kSeg = seg_steps<T>(), kThreads = W * 64;
-    __shared__ JoinRoom<T, W, 32> room;                          // inner is below 32
+    typedef ProductOf<T, FORM> P;
+    __shared__ JoinRoom<T, W, 32, P> room;                       // inner is below 32
     extern __shared__ __align__(16) char lds[];
     typedef BackwardTile<T, W> TT;
     TT& tile = *reinterpret_cast<TT*>(lds);
@@ -902,7 +1120,8 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
     cuts |= tails;
     const uint32_t lasts = a.dlast && own ? tails : 0u;
     const uint64_t place = (row0 + row_of) * inner + c;          // in (outer, inner), of the segment's last row
-    T f[kSeg], b[kSeg], A = (T)1, H = (T)0;
+    T f[kSeg], b[kSeg], H = (T)0;
+    Running<T, P> run;
     {
         uint32_t e = v0 * inner + c;
 #pragma unroll
@@ -914,13 +1133,14 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
                 if constexpr (FORM == RT_SCAN_SIGMOID) f[j] = gate_of(f[j]).s;
                 if (lasts >> j & 1) b[j] += a.dlast[place - (uint64_t)__popc(tails & ((2u << j) - 1u) & ~1u) * inner];
                 H = j == 0 || (cuts >> j & 1) ? b[j] : fused(f[j], H, b[j]);
-                A *= f[j];
+                run.by(f[j]);
             }
         }
-        if (cuts) A = (T)0;
-        if (!own) { A = (T)1; H = (T)0; cuts = 0; }
     }
-    const Prefix<T> pre = join_lanes<true>(A, H, cuts != 0, lane, nw.shift);
+    bool odd;
+    P A = run.template whole<kSeg>(ls, [&](int j) { return f[j]; }, &odd);
+    if (!own) { A = P::of((T)1); H = (T)0; cuts = 0; }
+    const Prefix<T, P> pre = join_lanes<true>(A, H, cuts != 0, own && cuts == 0 && odd, lane, nw.shift);
     join_tile<T, W, 32, true>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
         return run_lanes(pre, start, serial, lane, nw.shift, [&](T d) {
             RT_APART_LANES;
@@ -1022,7 +1242,7 @@ template <class T> int32_t make_chain(rt_ctx* ctx, uint32_t tiles, uint32_t roun
     RT_TRY(rt_chain_room(ctx, 0, (uint64_t)lines * kTicketPitch * sizeof(uint32_t), &tickets));
     RT_TRY(rt_chain_room(ctx, 1, (uint64_t)tiles * lines * Slot<T>::kWords * sizeof(uint64_t), &words));
     // the slots are cleared, and old tags with them, before numbers come round
-    if (++ctx->chain_launches == 1u << 29) {
+    if (++ctx->chain_launches == kEpochs) {
         RT_TRY(rt_chain_clear(ctx, 1));
         ctx->chain_launches = 1;
     }

@@ -1,8 +1,10 @@
-"""The linear scan where sums that a stretch forms from a start of zero leave the type's range although no state does."""
+"""The linear scan where parts of it leave the type's range although no state does: sums that a stretch forms from a start of zero, and
+products of a stretch's factors.  And the numbers of its launches, where they come round."""
 import numpy as np
 import pytest
 
-from test_gpu_scan import TYPES, hip, poison, put, run_forward  # noqa: F401
+import sequence_ref as R
+from test_gpu_scan import TYPES, hip, near, poison, put, run_forward  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +58,100 @@ def test_sums_from_zero_that_leave_the_range(hip, shape, every, dtype):
         if name == "dgate":
             g, w = g[:, 1:], w[:, 1:]                                 # the state of the first step is -c: out of the range
         assert (g == w).all(), name
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_states_that_sink_and_rise_again(hip, shape, dtype):
+    """Gates that are powers of two, no x: 40 small ones and then 40 large ones, so that a state goes far down and comes back exactly, and
+    the factors' product over a stretch (2^-200; f64 2^-1600) is far below the smallest number.  All values are exact."""
+    T, (down, top) = TYPES[dtype], {"f32": (5, 100), "f64": (40, 900)}[dtype]
+    outer, steps, inner = shape
+    k = np.arange(steps) % 80
+    e = np.where(k < 40, -down, down)
+    level = top + np.cumsum(e)
+    assert level.min() > np.log2(np.finfo(T).tiny) and level.max() <= top
+    sign = np.where(np.arange(outer * inner) % 2, -1.0, 1.0).reshape(outer, inner)
+    state = (sign * 2.0 ** top).astype(T)
+    gate = np.broadcast_to((2.0 ** e)[None, :, None], shape).astype(T)
+    d = {"gate": gate, "x": np.zeros(shape, T), "state": state, "dlast": state, "reset": None, "dh": np.zeros(shape, T)}
+    h, last = run_forward(hip, "linear", d)
+    want = (sign[:, None] * 2.0 ** level[None, :, None]).astype(T)
+    assert (h == want).all() and (last == want[:, -1]).all()
+    # backward, the gates in the opposite order; h of 2^-20 keeps dgate in the range where dx is
+    d["gate"] = np.ascontiguousarray(gate[:, ::-1])
+    small = np.full(shape, T(2) ** -20)
+    d["state"] = np.full((outer, inner), T(2) ** -20)
+    got, wish = backward(hip, d, small), plain_backward(d, small)
+    assert (wish[2] == last).all()
+    for g, w, name in zip(got, wish, ("dgate", "dx", "dstate")):
+        assert (g == w).all(), name
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_states_of_many_magnitudes(hip, shape, dtype):
+    """Gates of either sign that lead the states up and down over most of the range, slowly and fast, with x of the states' size, under the
+    bounds of the plain loop."""
+    T, most = TYPES[dtype], {"f32": 95, "f64": 900}[dtype]
+    outer, steps, inner = shape
+    rng = np.random.default_rng(steps)
+    t = np.arange(steps + 1)
+    level = most * np.sin(t / rng.uniform(5, 9)) * np.cos(t / rng.uniform(60, 90))
+    e = np.diff(level)
+    gate = (2.0 ** e)[None, :, None] * rng.choice([-0.9, 0.9, 0.5, 1.0], shape)
+    x = rng.standard_normal(shape) * (2.0 ** level[1:])[None, :, None]
+    d = {"gate": gate.astype(T), "x": x.astype(T), "state": rng.standard_normal((outer, inner)).astype(T) * T(2.0 ** level[0]), "reset": None}
+    want, M, S = R.scan("linear", d["gate"], d["x"], d["state"])
+    d["dlast"] = d["state"]
+    h, last = run_forward(hip, "linear", d)
+    near(h, want, R.scan_bound("linear", T, M, S), shape)
+    assert last.tobytes() == np.ascontiguousarray(h[:, -1]).tobytes()
+    # the same sizes from the last step back
+    d["dh"] = np.ascontiguousarray(d["x"][:, ::-1])
+    d["gate"] = np.ascontiguousarray(np.concatenate([d["gate"][:, :1], d["gate"][:, 1:][:, ::-1]], axis=1))
+    small = np.full(shape, T(2) ** -20)
+    d["state"] = np.full((outer, inner), T(2) ** -20)
+    got = backward(hip, d, small)
+    wish = R.scan_backward("linear", d["gate"], x, small, d["dh"], d["state"], None, d["dlast"])
+    for g, (w, bound), name in list(zip(got, wish, ("dgate", "dx", "dstate")))[:2]:
+        near(g, w, bound, name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("period", [48, 700, 3000])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_products_beyond_the_range_of_states_that_are_zero(hip, shape, period, dtype):
+    """Gates whose product goes far below the range and then far above it, and a state of zero that they leave at zero until a few small x
+    come near the end: whatever the products are, nothing comes of them."""
+    T, (down, up) = TYPES[dtype], {"f32": (-60, 100), "f64": (-600, 900)}[dtype]
+    outer, steps, inner = shape
+    e = np.where(np.arange(steps) % period < period // 2, down, up)
+    last = max(steps - 3, 0)
+    e[last:] = 0
+    d = {"gate": np.broadcast_to((2.0 ** e)[None, :, None], shape).astype(T), "x": np.zeros(shape, T), "state": np.zeros((outer, inner), T), "reset": None}
+    d["x"][:, last:] = 3
+    d["dlast"] = d["state"]
+    h, end = run_forward(hip, "linear", d)
+    want = np.cumsum(d["x"], axis=1)
+    assert (h == want).all() and (end == want[:, -1]).all()
+    d["dh"] = np.ascontiguousarray(d["x"][:, ::-1])
+    d["gate"] = np.ascontiguousarray(np.concatenate([d["gate"][:, :1], d["gate"][:, 1:][:, ::-1]], axis=1))
+    got, wish = backward(hip, d, h), plain_backward(d, h)
+    assert (wish[1] == want[:, ::-1]).all()
+    for g, w, name in zip(got, wish, ("dgate", "dx", "dstate")):
+        assert (g == w).all(), name
+
+
+def test_more_launches_than_there_are_numbers(hip):
+    """The words that tiles hand on carry the launch's number, one of 2^17."""
+    rng = np.random.default_rng(1)
+    shape = (1, 600, 33)
+    n = 600 * 33
+    gate, x = (put(hip, rng.random(n).astype(np.float32)) for _ in range(2))
+    h, again = poison(hip, np.empty(n, np.float32)), poison(hip, np.empty(n, np.float32))
+    hip.gated_scan("linear", gate, x, h, *shape)
+    for k in range((1 << 17) + 200):
+        hip.gated_scan("linear", gate, x, again, *shape)
+        if k % 4096 == 0 or k > 1 << 17:
+            assert hip.equal(h, again), k
