@@ -221,6 +221,8 @@ def prepare(case, seed):
     else:
         s["out"] = {k: like(s["x"]) for k in (("x",) if case["kind"] == "pack" else ("y", "dx"))}
         s["room8"] = (torch.empty(case["n"], dtype=torch.int8, device="cuda"), torch.empty(-(-case["n"] // GROUP), dtype=torch.uint8, device="cuda"))
+    if own:
+        torch.cuda.current_stream().synchronize()       # the library's context has a stream of its own: what it borrows is there before its first call
     return s
 
 
@@ -228,6 +230,8 @@ _backend = None
 
 
 def _run_own(s):
+    """The calls go to the context's own stream, one after the other.  Who reads the outputs on another stream, or gives the memory of a
+    state back, waits for the context (`_backend.sync()`) or for the device first, as `Hip.borrow` asks."""
     from rtensors_amd import hip as H
     global _backend
     if _backend is None:
