@@ -129,7 +129,7 @@ __global__ __launch_bounds__(kSBlock) void scan_backward_columns_kernel(BackArgs
 //
 // A word is 32 bits of a value and a tag, written and read as one 64-bit access at device scope: a word with the right tag is valid by
 // itself, with no order between words.  Tags hold the launch's number and are not cleared between launches.  The number comes from the
-// host, so a launch must not be replayed from a graph; the context's stream is never under capture, and make_chain refuses it.
+// host, so a launch must not be replayed from a graph; none can be: the context's stream is its own, and nothing here captures it.
 struct Chain {
     uint32_t* tickets;       // one counter a line, 64 bytes apart, 0 between launches
     uint64_t* words;
@@ -1235,9 +1235,6 @@ template <class T> int32_t make_chain(rt_ctx* ctx, uint32_t tiles, uint32_t roun
     out->epoch = 0;
     out->rounds = rounds;
     if (tiles == 1) return RT_OK;
-    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-    RT_HIP(hipStreamIsCapturing(ctx->stream, &capture));
-    if (capture != hipStreamCaptureStatusNone) return rt_fail(RT_E_INVALID, "gated scan: a launch that hands states from tile to tile cannot be captured");
     void *tickets = nullptr, *words = nullptr;
     RT_TRY(rt_chain_room(ctx, 0, (uint64_t)lines * kTicketPitch * sizeof(uint32_t), &tickets));
     RT_TRY(rt_chain_room(ctx, 1, (uint64_t)tiles * lines * Slot<T>::kWords * sizeof(uint64_t), &words));
