@@ -334,8 +334,8 @@ int32_t rt_matmul(rt_ctx* ctx, int32_t dtype,
  * single-token form of serving; last may be the state buffer itself.  h may be x itself or gate itself; any other overlap of an
  * output is RT_E_INVALID.  The state is held and summed in the tensor's own dtype (f32 / f64).  Long runs are cut into stretches that are
  * summed apart and joined by the products of their factors; how they are cut depends on the sizes (and the device), so equal calls give
- * equal bits.  A product that leaves the range upwards, or a sum from a start of zero, makes its stretches run step by step.  Products of
- * RT_SCAN_LINEAR that fall below the range keep their exponent, and what later gates lift again is there; those of RT_SCAN_SIGMOID, which
+ * equal bits.  A product that leaves the range upwards, or a sum of finite terms from a start of zero, makes its stretches run step by
+ * step.  Products of RT_SCAN_LINEAR that fall below the range keep their exponent, and what later gates lift again is there; those of RT_SCAN_SIGMOID, which
  * nothing lifts, lose what of an earlier state they carry (less than 2^-126 of that state, 2^-1022 for f64), and make an infinite one NaN.
  * A state that leaves the range inside a stretch is infinite there, as in a plain loop; behind the stretch stands the formula's value, finite
  * where later gates bring it back.  Workspace: 1 / 200 to 1 / 25 of the operands (few columns of f64) where a run is cut over several blocks, kept by the

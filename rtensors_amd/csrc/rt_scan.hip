@@ -263,24 +263,43 @@ template <class T, class P> struct Running {
         m *= f;
         if constexpr (P::kApart) low = least(low, m);
     }
-    // factor(j) is factor j of the first n of L; odd: a prefix is above the range, or nearly (an infinite m says so itself)
-    template <int L, class F> __device__ __forceinline__ P whole(int n, F factor, bool* odd) const {
+    // factor(j) and term(j), the first n of L, give the product and the sum H from a start of zero.  odd: a prefix of the product is above the
+    // range, or nearly (an infinite product says so itself); or, with SUMS, H left the range with finite terms: the plain loop's state need not
+    // have.  From a term on that is not finite it has, too; and where the stretch is cut, H is its state.
+    template <bool SUMS, int L, class F, class G> __device__ __forceinline__ P whole(T H, bool cut, int n, F factor, G term, bool* odd) const {
+        P a = P::of(m);
+        bool over = SUMS && !cut && !finite(H), fell = false;
         *odd = false;
-        if constexpr (P::kApart) {
-            if (__any(low < P::kNormal)) {
-                T p = (T)1;
-                int e = 0;
+        if constexpr (P::kApart) fell = low < P::kNormal;
+        if ((SUMS || P::kApart) && __any(over || fell)) {
+            if constexpr (P::kApart)
+                if (__any(fell)) {
+                    T p = (T)1;
+                    int e = 0;
+#pragma unroll
+                    for (int j = 0; j < L; ++j)
+                        if (j < n) {
+                            p *= mantissa(factor(j));
+                            e += exponent(factor(j));
+                            *odd = *odd || e > P::kTop;
+                        }
+                    a = P::from(p, e);
+                }
+            if (SUMS && __any(over)) {
+                T h = (T)0;
+                bool first = false;
 #pragma unroll
                 for (int j = 0; j < L; ++j)
                     if (j < n) {
-                        p *= mantissa(factor(j));
-                        e += exponent(factor(j));
-                        *odd = *odd || e > P::kTop;
+                        const T q = j == 0 ? term(j) : fused(factor(j), h, term(j));
+                        first = first || (finite(h) && finite(term(j)) && !finite(q));
+                        h = q;
                     }
-                return P::from(p, e);
+                *odd = *odd || (over && first);
             }
+            *odd = *odd && !cut;
         }
-        return P::of(m);
+        return a;
     }
 };
 
@@ -429,7 +448,7 @@ template <class T, int W, int LN, class P> __device__ __forceinline__ uint32_t t
 // A product of factors above 1 can leave the range while the states stay inside it (a start of zero, say), and so can the sum from a start
 // of zero (a state of -c, and x of c twice).  Where one does, the tile's stretches run one after the other and only its end state is
 // published: the plain loop's result, at the plain loop's pace.  SUMS: whether the sums are looked at.  Those of the forward sigmoid form are
-// averages of x, which leave the range only where x has.
+// averages of x, which leave the range only where x has.  A sum with a term that is not finite does not count: the plain loop has it too.
 template <class T, int W, int LN, bool SUMS, class P, class Run>
 __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN, P>& room, uint32_t item, uint32_t k, const P& A, T H, bool cut, bool odd, T first, Run run) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -443,7 +462,7 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN, P>& r
     const uint32_t epoch = ch.epoch;
     if constexpr (P::kApart) deep = __any((room.cut[lane & (W - 1)] & 4u) != 0);         // from here on: of the tile
     T ta = (T)1, th = (T)0, low = (T)1;
-    bool tcut = false, bad = false;
+    bool tcut = false, bad = false, wild = false;
     if (!deep) {
 #pragma unroll
         for (int v = 0; v < W; ++v) {
@@ -454,7 +473,8 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN, P>& r
                 tcut = true;
             } else {
                 th = v == 0 ? hv : fused(av, th, hv);
-                bad = bad || !finite(av) || (SUMS && !finite(th));
+                bad = bad || !finite(av);
+                wild = wild || (SUMS && !finite(th));
                 if (!tcut) {
                     ta = v == 0 ? av : ta * av;
                     if constexpr (P::kApart) low = least(low, ta);
@@ -473,7 +493,8 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN, P>& r
                 tcut = true;
             } else {
                 th = v == 0 ? hv : av.on(th, hv);
-                bad = bad || !finite(av.m) || (SUMS && !finite(th));
+                bad = bad || !finite(av.m);
+                wild = wild || (SUMS && !finite(th));
                 if (!tcut) {
                     ta = v == 0 ? av.m : ta * av.m;
                     if constexpr (P::kApart) low = least(low, ta);
@@ -482,7 +503,18 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN, P>& r
             }
         }
     }
-    const bool serial = __any(bad);                              // the same in all waves: they look at the same numbers
+    bool serial = __any(bad || wild);                            // the same in all waves: they look at the same numbers
+    if (SUMS && serial) {                                        // a sum of finite terms?  A wave's own is looked at by the wave
+        T p = (T)0;
+#pragma unroll 1
+        for (int v = 0; v < W; ++v) {
+            const T hv = room.H[v][lane & (LN - 1)];
+            const T q = v == 0 || (room.cut[v] & 1u) ? hv : deep ? room.get(v, lane & (LN - 1)).on(p, hv) : fused(room.A[v][lane & (LN - 1)], p, hv);
+            bad = bad || (!finite(q) && finite(p) && finite(hv));
+            p = q;
+        }
+        serial = __any(bad);
+    }
     uint64_t* slot = last ? nullptr : Slot<T>::at(ch, item) + lane;
     T start = first;
     P whole = P::of(ta);
@@ -616,12 +648,12 @@ __global__ __launch_bounds__(W * 64) void scan_wide_kernel(ScanArgs<T> a, Chain 
                 run.by(f[j]);
             }
         }
-        A = run.template whole<L>(n, [&](int j) { return f[j]; }, &odd);
+        A = run.template whole<FORM == RT_SCAN_LINEAR, L>(H, cuts != 0, n, [&](int j) { return f[j]; }, [&](int j) { return b[j]; }, &odd);
     }
     T first = k == 0 && a.state ? a.state[sc] : (T)0;
     RT_PIN_LANE(first);
     T* h = a.h + base;
-    const T end = join_tile<T, W, 64, FORM == RT_SCAN_LINEAR>(ch, room, item, k, A, H, cuts != 0, cuts == 0 && __any(odd), first, [&](T p, bool) {
+    const T end = join_tile<T, W, 64, FORM == RT_SCAN_LINEAR>(ch, room, item, k, A, H, cuts != 0, __any(odd), first, [&](T p, bool) {
         RT_APART;
         if (in) {
 #pragma unroll
@@ -748,7 +780,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
             }
             f = s[j];
         }
-        A = run.template whole<L>(n, [&](int j) { return j == 0 ? f0 : s[j ? j - 1 : 0]; }, &odd);
+        A = run.template whole<true, L>(H, cuts != 0, n, [&](int j) { return j == 0 ? f0 : s[j ? j - 1 : 0]; }, [&](int j) { return up[j]; }, &odd);
         if constexpr (kHeld) {
             hrows[w].put(hv, lane);
             if constexpr (kSigmoid) xrows[w].put(xh, lane);
@@ -757,7 +789,7 @@ __global__ __launch_bounds__(W * 64) void scan_backward_wide_kernel(BackArgs<T, 
     T first = k == 0 && a.dlast ? a.dlast[sc] : (T)0;
     RT_PIN_LANE(first);
     T *dg = a.dgate + base, *dx = a.dx + base;
-    const T end = join_tile<T, W, 64, true>(ch, room, item, k, A, H, cuts != 0, cuts == 0 && __any(odd), first, [&](T d, bool) {
+    const T end = join_tile<T, W, 64, true>(ch, room, item, k, A, H, cuts != 0, __any(odd), first, [&](T d, bool) {
         RT_APART;
         uint64_t rresets = resets;
         RT_PIN(rresets);
@@ -835,8 +867,24 @@ template <class T, class P> struct Prefix {
     T H, wholeH;
     bool cut, any_cut, odd;
 };
-template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Falling<T>> join_lanes(Falling<T> A, T H, bool cut, bool, int lane, uint32_t shift) {
-    bool odd = !finite(A.m);
+// Whether the wave runs its segments one after the other: `odd` of a lane, or, with SUMS, a sum over several lanes that left the range.  One
+// that was not finite on the way has stayed so; unless a lane's own that is not (`given`, and not odd) is among its terms, they are finite.
+template <bool SUMS, class T> __device__ __forceinline__ bool any_odd(bool odd, T H, bool given, bool cut, int lane, uint32_t shift) {
+    bool over = SUMS && !finite(H);
+    const bool any = __any(odd || over);
+    if (!SUMS || !any) return any;
+    for (uint32_t d = 1u << shift; d < 64; d <<= 1) {
+        const int below = __shfl_up((given ? 2 : 0) | (cut ? 1 : 0), d);
+        if (lane >= (int)d) {
+            given = given || (!cut && (below & 2));
+            cut = cut || (below & 1);
+        }
+    }
+    return __any(odd || (over && !given));
+}
+template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Falling<T>> join_lanes(Falling<T> A, T H, bool cut, bool odd, int lane, uint32_t shift) {
+    odd = odd || (!cut && !finite(A.m));
+    const bool given = !finite(H), own_cut = cut;
     if (cut) A.m = (T)0;
     for (uint32_t d = 1u << shift; d < 64; d <<= 1) {
         const T A1 = __shfl_up(A.m, d), H1 = __shfl_up(H, d);
@@ -848,13 +896,12 @@ template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Falling<T>> j
             odd = odd || !finite(A.m);
         }
     }
-    odd = odd || (SUMS && !finite(H));                           // a sum that was not finite on the way has stayed so
     const int top = 64 - (1 << shift) + (lane & ((1 << shift) - 1));
     Prefix<T, Falling<T>> p;
     p.wholeA = {__shfl(A.m, top)};
     p.wholeH = __shfl(H, top);
     p.any_cut = __any(cut);
-    p.odd = __any(odd);
+    p.odd = any_odd<SUMS>(odd, H, given, own_cut, lane, shift);
     const T A0 = __shfl_up(A.m, 1u << shift), H0 = __shfl_up(H, 1u << shift);
     const bool c0 = __shfl_up((int)cut, 1u << shift) != 0;
     const bool head = lane < (1 << shift);
@@ -869,6 +916,7 @@ template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Apart<T>> joi
     T m = mantissa(A.m) * (T)2;
     int e = exponent(A.m) + A.e - 1;
     odd = odd || (!cut && !finite(m));
+    const bool given = !finite(H), own_cut = cut;
     for (uint32_t d = 1u << shift; d < 64; d <<= 1) {
         const T m1 = __shfl_up(m, d), H1 = __shfl_up(H, d);
         const int both = __shfl_up(e * 2 + (cut ? 1 : 0), d);
@@ -883,15 +931,14 @@ template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Apart<T>> joi
             }
         }
     }
-    // a sum that was not finite on the way has stayed so; each lane has the product of a prefix
-    odd = odd || (!cut && e > Apart<T>::kTop) || (SUMS && !finite(H));
+    odd = odd || (!cut && e > Apart<T>::kTop);                   // each lane has the product of a prefix
     const int top = 64 - (1 << shift) + (lane & ((1 << shift) - 1));
     const Apart<T> a = Apart<T>::from(m, e);
     Prefix<T, Apart<T>> p;
     p.wholeA = {__shfl(a.m, top), __shfl(a.e, top)};
     p.wholeH = __shfl(H, top);
     p.any_cut = __any(cut);
-    p.odd = __any(odd);
+    p.odd = any_odd<SUMS>(odd, H, given, own_cut, lane, shift);
     const T m0 = __shfl_up(a.m, 1u << shift), H0 = __shfl_up(H, 1u << shift);
     const int both = __shfl_up(a.e * 2 + (cut ? 1 : 0), 1u << shift);
     const bool head = lane < (1 << shift);
@@ -1020,9 +1067,9 @@ __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void scan_narrow_kernel(Sc
         }
     }
     bool odd;
-    P A = run.template whole<kSeg>(ls, [&](int j) { return f[j]; }, &odd);
+    P A = run.template whole<FORM == RT_SCAN_LINEAR, kSeg>(H, cuts != 0, ls, [&](int j) { return f[j]; }, [&](int j) { return b[j]; }, &odd);
     if (!own) { A = P::of((T)1); H = (T)0; cuts = 0; }
-    const Prefix<T, P> pre = join_lanes<FORM == RT_SCAN_LINEAR>(A, H, cuts != 0, own && cuts == 0 && odd, lane, nw.shift);
+    const Prefix<T, P> pre = join_lanes<FORM == RT_SCAN_LINEAR>(A, H, cuts != 0, own && odd, lane, nw.shift);
     join_tile<T, W, 32, FORM == RT_SCAN_LINEAR>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
         return run_lanes(pre, start, serial, lane, nw.shift, [&](T p) {
             RT_APART_LANES;
@@ -1138,9 +1185,9 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
         }
     }
     bool odd;
-    P A = run.template whole<kSeg>(ls, [&](int j) { return f[j]; }, &odd);
+    P A = run.template whole<true, kSeg>(H, cuts != 0, ls, [&](int j) { return f[j]; }, [&](int j) { return b[j]; }, &odd);
     if (!own) { A = P::of((T)1); H = (T)0; cuts = 0; }
-    const Prefix<T, P> pre = join_lanes<true>(A, H, cuts != 0, own && cuts == 0 && odd, lane, nw.shift);
+    const Prefix<T, P> pre = join_lanes<true>(A, H, cuts != 0, own && odd, lane, nw.shift);
     join_tile<T, W, 32, true>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
         return run_lanes(pre, start, serial, lane, nw.shift, [&](T d) {
             RT_APART_LANES;

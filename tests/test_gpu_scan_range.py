@@ -155,3 +155,64 @@ def test_more_launches_than_there_are_numbers(hip):
         hip.gated_scan("linear", gate, x, again, *shape)
         if k % 4096 == 0 or k > 1 << 17:
             assert hip.equal(h, again), k
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("form", ["linear", "sigmoid"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_values_that_are_not_finite_next_to_sums_that_overflow(hip, shape, form, dtype):
+    """NaN and infinities in some columns' x, in others the pairs of the first test, in others neither, resets here and there: each column
+    has what it has on its own, kinds and places of the values that are not finite as in the plain loop."""
+    T = TYPES[dtype]
+    c = T(0.9) * np.finfo(T).max
+    outer, steps, inner = shape
+    rng = np.random.default_rng(inner)
+    gate, x, state = np.ones(shape, T), np.zeros(shape, T), np.zeros((outer, inner), T)
+    kind = np.arange(outer * inner).reshape(outer, inner) % 4
+    pairs = np.zeros(steps, T)
+    pairs[1:] = np.where(np.arange(steps - 1) % 4 < 2, c, -c)
+    for o in range(outer):
+        for i in range(inner):
+            if kind[o, i] == 0:
+                x[o, :, i], state[o, i] = rng.integers(-5, 6, steps), 7
+            elif kind[o, i] == 1:
+                x[o, :, i], state[o, i] = rng.integers(-5, 6, steps), 7
+                x[o, steps // 3, i] = (np.inf, -np.inf, np.nan)[i % 3]
+            elif kind[o, i] == 2:
+                x[o, :, i], state[o, i] = pairs, -c
+            else:                                     # both: the pairs before, an infinity behind
+                x[o, :, i], state[o, i] = pairs, -c
+                x[o, steps // 2 :, i] = 0
+                x[o, (steps + steps // 2) // 2, i] = np.inf
+    reset = np.zeros((outer, steps), bool)
+    if form == "sigmoid":                             # forward: averages of x, not sums
+        gate[:] = 40
+        with np.errstate(all="ignore"):
+            x = np.where(np.isfinite(x), np.sign(x), x).astype(T)
+    d = {"gate": gate, "x": x, "state": state if form == "linear" else np.sign(state), "reset": reset, "dlast": state}
+    with np.errstate(all="ignore"):
+        want = R.scan(form, gate, x, d["state"])[0].astype(T)
+    h, last = run_forward(hip, form, dict(d, reset=None))
+    for k in (np.isnan, np.isposinf, np.isneginf):
+        assert np.array_equal(k(h), k(want)), k
+    fine = np.isfinite(want)
+    assert (h[fine] == want[fine]).all() if form == "linear" else (np.abs(h[fine] - want[fine]) <= 1e-5).all()
+    # backward: gates of 1 (the sigmoid form: of 40, a factor of 1 within 2^-57), the columns' x from the last step on
+    d["dh"] = np.ascontiguousarray(d["x"][:, ::-1]) if form == "linear" else np.ascontiguousarray(x[:, ::-1])
+    small = np.full(shape, T(2) ** -100)
+    outs = [poison(hip, small), poison(hip, small), poison(hip, state)]
+    hip.gated_scan_backward(form, put(hip, gate), put(hip, small), put(hip, small), put(hip, d["dh"]), outs[0], outs[1], *shape, state=put(hip, state),
+                            dlast=put(hip, d["dlast"]), dstate=outs[2])
+    dx = hip.dump(outs[1]).reshape(shape)
+    if form == "linear":
+        plain = plain_backward(dict(d, state=state), small)[1] if np.isfinite(d["dh"]).all() else None
+        with np.errstate(all="ignore"):
+            D, carry = np.zeros(shape, T), d["dlast"]
+            for t in range(steps - 1, -1, -1):
+                D[:, t] = d["dh"][:, t] + carry
+                carry = D[:, t]
+        assert plain is None or (plain == D).all()
+        for k in (np.isnan, np.isposinf, np.isneginf):
+            assert np.array_equal(k(dx), k(D)), k
+        fine = np.isfinite(D)
+        assert (dx[fine] == D[fine]).all()
