@@ -215,6 +215,8 @@ __device__ __forceinline__ float fused(float a, float b, float c) { return __bui
 __device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
 __device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
 __device__ __forceinline__ bool finite(double v) { return __builtin_fabs(v) < __builtin_inf(); }
+__device__ __forceinline__ bool infinite(float v) { return __builtin_fabsf(v) == __builtin_inff(); }
+__device__ __forceinline__ bool infinite(double v) { return __builtin_fabs(v) == __builtin_inf(); }
 
 __device__ __forceinline__ float mantissa(float v) { return __builtin_amdgcn_frexp_mantf(v); }
 __device__ __forceinline__ double mantissa(double v) { return __builtin_amdgcn_frexp_mant(v); }
@@ -226,7 +228,7 @@ __device__ __forceinline__ float scaled(float v, int e) { return __builtin_ldexp
 __device__ __forceinline__ double scaled(double v, int e) { return __builtin_ldexp(v, e); }
 
 // The product A of a stretch's factors.
-// Those of the sigmoid form are at most 1: nothing lifts a product again that falls below the range.
+// Those of the sigmoid form are at most 1: nothing lifts a product again that falls below the range, and none goes above it.
 template <class T> struct Falling {
     static constexpr bool kApart = false;
     T m;
@@ -235,7 +237,8 @@ template <class T> struct Falling {
 };
 // Those of the linear form may be above 1 behind others far below it: a state of 2^100 times 2^-200 and then 2^150 is 2^50.  A product below
 // the normal range is held as m 2^e, m at the range's lower end and e < 0; any other one as it is, with e = 0.  An infinite m says that a
-// prefix of the stretch is above the range; such a tile runs step by step.
+// prefix of the stretch is above the range, or a factor infinite; such a tile runs step by step.  NaN says that a factor is NaN: behind it the
+// plain loop's state is NaN as well.
 template <class T> struct Apart {
     static constexpr bool kApart = true;
     static constexpr T kNormal = sizeof(T) == 4 ? (T)0x1p-126 : (T)0x1p-1022;
@@ -264,13 +267,13 @@ template <class T, class P> struct Running {
         if constexpr (P::kApart) low = least(low, m);
     }
     // factor(j) and term(j), the first n of L, give the product and the sum H from a start of zero.  odd: a prefix of the product is above the
-    // range, or nearly (an infinite product says so itself); or, with SUMS, H left the range with finite terms: the plain loop's state need not
-    // have.  From a term on that is not finite it has, too; and where the stretch is cut, H is its state.
+    // range, or nearly, or a factor is infinite; or, with SUMS, H left the range with finite terms and factors: the plain loop's state
+    // need not have.  From a term on that is not finite it has, too; and where the stretch is cut, H is its state.
     template <bool SUMS, int L, class F, class G> __device__ __forceinline__ P whole(T H, bool cut, int n, F factor, G term, bool* odd) const {
         P a = P::of(m);
         bool over = SUMS && !cut && !finite(H), fell = false;
         *odd = false;
-        if constexpr (P::kApart) fell = low < P::kNormal;
+        if constexpr (P::kApart) fell = low < P::kNormal || !finite(m);
         if ((SUMS || P::kApart) && __any(over || fell)) {
             if constexpr (P::kApart)
                 if (__any(fell)) {
@@ -281,7 +284,7 @@ template <class T, class P> struct Running {
                         if (j < n) {
                             p *= mantissa(factor(j));
                             e += exponent(factor(j));
-                            *odd = *odd || e > P::kTop;
+                            *odd = *odd || e > P::kTop || infinite(factor(j));
                         }
                     a = P::from(p, e);
                 }
@@ -292,7 +295,7 @@ template <class T, class P> struct Running {
                 for (int j = 0; j < L; ++j)
                     if (j < n) {
                         const T q = j == 0 ? term(j) : fused(factor(j), h, term(j));
-                        first = first || (finite(h) && finite(term(j)) && !finite(q));
+                        first = first || (j > 0 && finite(factor(j)) && finite(h) && finite(term(j)) && !finite(q));
                         h = q;
                     }
                 *odd = *odd || (over && first);
@@ -318,13 +321,13 @@ template <class T, int W, int LN, class P> struct JoinRoom {
     uint32_t cut[W];                                             // 1: cut, 2: odd, 4: deep
     uint32_t tile;
     int found;
-    // a wave's product and its exponent: that of m 2^e as a whole, kZero for 0, and those from -2^15 on are all the same: the other waves of
+    // a wave's product and its exponent: that of m 2^e as a whole, kZero for 0 and NaN, and those from -2^15 on are all the same: the other waves of
     // a tile lift no state again that far
     static constexpr int kZero = 1 << 14;
     __device__ __forceinline__ void put(int w, int l, const P& a) {
         A[w][l] = a.m;
         if constexpr (P::kApart) {
-            const int e = a.m == (T)0 ? kZero : a.e + exponent(a.m);
+            const int e = a.m == (T)0 || a.m != a.m ? kZero : a.e + exponent(a.m);
             E[w][l] = (int16_t)(e < -32768 ? -32768 : e);
         }
     }
@@ -473,12 +476,12 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN, P>& r
                 tcut = true;
             } else {
                 th = v == 0 ? hv : fused(av, th, hv);
-                bad = bad || !finite(av);
+                bad = bad || infinite(av);
                 wild = wild || (SUMS && !finite(th));
                 if (!tcut) {
                     ta = v == 0 ? av : ta * av;
                     if constexpr (P::kApart) low = least(low, ta);
-                    bad = bad || !finite(ta);
+                    bad = bad || infinite(ta);
                 }
             }
         }
@@ -493,12 +496,12 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN, P>& r
                 tcut = true;
             } else {
                 th = v == 0 ? hv : av.on(th, hv);
-                bad = bad || !finite(av.m);
+                bad = bad || infinite(av.m);
                 wild = wild || (SUMS && !finite(th));
                 if (!tcut) {
                     ta = v == 0 ? av.m : ta * av.m;
                     if constexpr (P::kApart) low = least(low, ta);
-                    bad = bad || !finite(ta);
+                    bad = bad || infinite(ta);
                 }
             }
         }
@@ -508,9 +511,9 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN, P>& r
         T p = (T)0;
 #pragma unroll 1
         for (int v = 0; v < W; ++v) {
-            const T hv = room.H[v][lane & (LN - 1)];
-            const T q = v == 0 || (room.cut[v] & 1u) ? hv : deep ? room.get(v, lane & (LN - 1)).on(p, hv) : fused(room.A[v][lane & (LN - 1)], p, hv);
-            bad = bad || (!finite(q) && finite(p) && finite(hv));
+            const T av = room.A[v][lane & (LN - 1)], hv = room.H[v][lane & (LN - 1)];
+            const T q = v == 0 || (room.cut[v] & 1u) ? hv : deep ? room.get(v, lane & (LN - 1)).on(p, hv) : fused(av, p, hv);
+            bad = bad || (!finite(q) && finite(p) && finite(hv) && av == av);
             p = q;
         }
         serial = __any(bad);
@@ -868,7 +871,8 @@ template <class T, class P> struct Prefix {
     bool cut, any_cut, odd;
 };
 // Whether the wave runs its segments one after the other: `odd` of a lane, or, with SUMS, a sum over several lanes that left the range.  One
-// that was not finite on the way has stayed so; unless a lane's own that is not (`given`, and not odd) is among its terms, they are finite.
+// that was not finite on the way has stayed so; unless a lane's own that is not, or NaN among the factors (`given`, and not odd), is part of
+// it, its terms are finite.
 template <bool SUMS, class T> __device__ __forceinline__ bool any_odd(bool odd, T H, bool given, bool cut, int lane, uint32_t shift) {
     bool over = SUMS && !finite(H);
     const bool any = __any(odd || over);
@@ -883,8 +887,7 @@ template <bool SUMS, class T> __device__ __forceinline__ bool any_odd(bool odd, 
     return __any(odd || (over && !given));
 }
 template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Falling<T>> join_lanes(Falling<T> A, T H, bool cut, bool odd, int lane, uint32_t shift) {
-    odd = odd || (!cut && !finite(A.m));
-    const bool given = !finite(H), own_cut = cut;
+    const bool given = !finite(H) || A.m != A.m, own_cut = cut;
     if (cut) A.m = (T)0;
     for (uint32_t d = 1u << shift; d < 64; d <<= 1) {
         const T A1 = __shfl_up(A.m, d), H1 = __shfl_up(H, d);
@@ -893,7 +896,6 @@ template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Falling<T>> j
             H = cut ? H : fused(A.m, H1, H);
             cut = cut || c1;
             A.m = cut ? (T)0 : A1 * A.m;
-            odd = odd || !finite(A.m);
         }
     }
     const int top = 64 - (1 << shift) + (lane & ((1 << shift) - 1));
@@ -915,8 +917,8 @@ template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Falling<T>> j
 template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Apart<T>> join_lanes(Apart<T> A, T H, bool cut, bool odd, int lane, uint32_t shift) {
     T m = mantissa(A.m) * (T)2;
     int e = exponent(A.m) + A.e - 1;
-    odd = odd || (!cut && !finite(m));
-    const bool given = !finite(H), own_cut = cut;
+    odd = odd || (!cut && infinite(m));
+    const bool given = !finite(H) || m != m, own_cut = cut;
     for (uint32_t d = 1u << shift; d < 64; d <<= 1) {
         const T m1 = __shfl_up(m, d), H1 = __shfl_up(H, d);
         const int both = __shfl_up(e * 2 + (cut ? 1 : 0), d);
@@ -1066,9 +1068,9 @@ __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void scan_narrow_kernel(Sc
             }
         }
     }
+    if (!own) { run = Running<T, P>(); H = (T)0; cuts = 0; }
     bool odd;
-    P A = run.template whole<FORM == RT_SCAN_LINEAR, kSeg>(H, cuts != 0, ls, [&](int j) { return f[j]; }, [&](int j) { return b[j]; }, &odd);
-    if (!own) { A = P::of((T)1); H = (T)0; cuts = 0; }
+    const P A = run.template whole<FORM == RT_SCAN_LINEAR, kSeg>(H, cuts != 0, ls, [&](int j) { return f[j]; }, [&](int j) { return b[j]; }, &odd);
     const Prefix<T, P> pre = join_lanes<FORM == RT_SCAN_LINEAR>(A, H, cuts != 0, own && odd, lane, nw.shift);
     join_tile<T, W, 32, FORM == RT_SCAN_LINEAR>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
         return run_lanes(pre, start, serial, lane, nw.shift, [&](T p) {
@@ -1184,9 +1186,9 @@ __global__ __launch_bounds__(W * 64) void scan_backward_narrow_kernel(BackArgs<T
             }
         }
     }
+    if (!own) { run = Running<T, P>(); H = (T)0; cuts = 0; }
     bool odd;
-    P A = run.template whole<true, kSeg>(H, cuts != 0, ls, [&](int j) { return f[j]; }, [&](int j) { return b[j]; }, &odd);
-    if (!own) { A = P::of((T)1); H = (T)0; cuts = 0; }
+    const P A = run.template whole<true, kSeg>(H, cuts != 0, ls, [&](int j) { return f[j]; }, [&](int j) { return b[j]; }, &odd);
     const Prefix<T, P> pre = join_lanes<true>(A, H, cuts != 0, own && odd, lane, nw.shift);
     join_tile<T, W, 32, true>(ch, room, item, k, pre.wholeA, pre.wholeH, pre.any_cut, pre.odd, (T)0, [&](T start, bool serial) {
         return run_lanes(pre, start, serial, lane, nw.shift, [&](T d) {

@@ -216,3 +216,41 @@ def test_values_that_are_not_finite_next_to_sums_that_overflow(hip, shape, form,
             assert np.array_equal(k(dx), k(D)), k
         fine = np.isfinite(D)
         assert (dx[fine] == D[fine]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("form", ["linear", "sigmoid"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_gates_that_are_not_finite(hip, shape, form, dtype):
+    """NaN, infinite and zero gates in some columns, none in others: kinds and places of the values that are not finite as in the plain loop,
+    the other values within its bounds; forward and backward."""
+    T = TYPES[dtype]
+    outer, steps, inner = shape
+    rng = np.random.default_rng(steps + inner)
+    gate, x = rng.uniform(0.5, 1, shape), rng.standard_normal(shape)
+    column = np.arange(outer * inner).reshape(outer, inner)
+    for k, v in ((1, [np.nan]), (2, [np.inf]), (3, [-np.inf, 0.0]), (4, [np.nan, np.inf, 0.0])):
+        for q, value in enumerate(v):
+            o, i = np.nonzero(column % 6 == k)
+            gate[o, rng.integers(steps // 4, steps, o.size), i] = value
+    d = {"gate": gate.astype(T), "x": x.astype(T), "state": rng.standard_normal((outer, inner)).astype(T), "reset": rng.random((outer, steps)) < 2 / (steps + 20)}
+    with np.errstate(all="ignore"):
+        want, M, S = R.scan(form, d["gate"], d["x"], d["state"], d["reset"])
+    h, last = run_forward(hip, form, dict(d, dlast=d["state"]))
+    for k in (np.isnan, np.isposinf, np.isneginf):
+        assert np.array_equal(k(h), k(want)), k
+    fine = np.isfinite(want)
+    assert (np.abs(h.astype(want.dtype) - want)[fine] <= R.scan_bound(form, T, M, S)[fine]).all()
+    assert last.tobytes() == np.ascontiguousarray(h[:, -1]).tobytes()
+    small = np.full(shape, T(0.5))
+    outs = [poison(hip, small), poison(hip, small), poison(hip, d["state"])]
+    hip.gated_scan_backward(form, put(hip, d["gate"]), put(hip, small), put(hip, small), put(hip, d["x"]), outs[0], outs[1], *shape, state=put(hip, d["state"]),
+                            reset=put(hip, d["reset"]), dlast=put(hip, d["state"]), dstate=outs[2])
+    with np.errstate(all="ignore"):
+        wish = R.scan_backward(form, d["gate"], small, small, d["x"], d["state"], d["reset"], d["state"])
+    for out, (w, bound), name in zip(outs[1:], wish[1:], ("dx", "dstate")):
+        got = hip.dump(out).reshape(w.shape)
+        for k in (np.isnan, np.isposinf, np.isneginf):
+            assert np.array_equal(k(got), k(w)), (name, k)
+        fine = np.isfinite(w)
+        assert (np.abs(got.astype(w.dtype) - w)[fine] <= bound[fine]).all(), name
