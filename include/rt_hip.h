@@ -338,8 +338,8 @@ int32_t rt_matmul(rt_ctx* ctx, int32_t dtype,
  * step.  Products of RT_SCAN_LINEAR that fall below the range keep their exponent, and what later gates lift again is there; those of RT_SCAN_SIGMOID, which
  * nothing lifts, lose what of an earlier state they carry (less than 2^-126 of that state, 2^-1022 for f64), and make an infinite one NaN.
  * A state that leaves the range inside a stretch is infinite there, as in a plain loop; behind the stretch stands the formula's value, finite
- * where later gates bring it back.  Workspace: 1 / 200 to 1 / 25 of the operands (few columns of f64) where a run is cut over several blocks, kept by the
- * context and grown on demand.
+ * where later gates bring it back.  Workspace: 1 / 200 to 1 / 25 of the operands (few columns of f64) where a run is cut over several
+ * blocks, kept by the context and grown on demand.
  *
  * rt_gated_scan_backward: from dh (gradient of h) and dlast (gradient of last, null = 0), with a[t] the factor of p[t]:
  *     D[t] = dh[t] + (reset[t + 1] ? 0 : a[t + 1] * D[t + 1]),   D[steps - 1] = dh[steps - 1] + dlast
@@ -371,8 +371,9 @@ int32_t rt_gated_scan_backward_packed8(rt_ctx* ctx, int32_t dtype, int32_t form,
  *     M = max |x| of the group;  e = the least integer >= -119 with rint(M * 2^-e) <= 127;  byte = e + 127
  *     code = rint(x * 2^-e), ties to even;     restored = code * 2^e
  * so an element is off by at most half a step, 2^(e-1) <= M / 126.  A restored value has at most 7 significant bits: it is exact in
- * f32 and f64.  Magnitudes below 2^-120 become 0.  A group that holds NaN or an infinity (f64: or a magnitude of 127.5 * 2^127 or
- * more) has byte 255 and restores as NaN throughout, so a diverged run stays visible.
+ * f64, and in f32 wherever that reaches (of what was packed from f64, up to 127 * 2^127).  Magnitudes below 2^-120 become 0.  A group
+ * that holds NaN or an infinity (f64: or a magnitude of 127.5 * 2^127 or more) has byte 255 and restores as NaN throughout, so a diverged
+ * run stays visible.
  *   rt_pack8                  codes, exps = src[start .. start + len)
  *   rt_unpack8                dst = restored
  *   rt_pack8_unary            dst = op(src[start .. start + len)) and the 8-bit form of the source, in one pass; op is RT_U_SIGMOID,
@@ -380,11 +381,11 @@ int32_t rt_gated_scan_backward_packed8(rt_ctx* ctx, int32_t dtype, int32_t form,
  *                             signs only, which rounding to 8 bits would lose near 0)
  *   rt_pack8_unary_backward   dst = upstream * op'(restored)
  *   rt_pack8_matmul_backward  the weight gradient of y = x w:  dst[b] (k x n) = restored[b]^T (m x k, transposed) * upstream[b] (m x n)
- *                             for every batch; codes and exps are those of the whole (b, m, k) run; dst is zero for m = 0;
- *                             k and n below 2^25
+ *                             for every batch (any number of them); codes and exps are those of the whole (b, m, k) run; dst
+ *                             is zero for m = 0; k and n below 2^25
  * Buffers are row-major runs from element 0.  dst of rt_pack8_unary may be src (start = 0), that of rt_pack8_unary_backward may be
  * upstream; any other overlap of an output is RT_E_INVALID.  f32 products are summed in f32, f64 ones in f64, in an order that
- * depends on the sizes alone. */
+ * depends on the sizes (and the device) alone. */
 #define RT_PACK8_GROUP 32
 int32_t rt_pack8(rt_ctx* ctx, int32_t dtype, const void* src, uint64_t src_len, uint64_t start, uint64_t len,
                  void* codes, uint64_t codes_len, void* exps, uint64_t exps_len);

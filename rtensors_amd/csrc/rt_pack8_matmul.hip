@@ -43,9 +43,9 @@ __device__ __forceinline__ Parts parts_of(const uint32_t (&v)[8]) {
     return out;
 }
 
-// Bound by the matrix instructions: 16384 x 4096 x 4096 takes 1318 us, three bf16 products at 1250 TFLOP/s (the card's bf16 matmul of 8192^3
-// runs at 1154), 417 TFLOP/s of f32; short shares by what surrounds them: 65536 x 256 x 320 takes 50 us, of which 6 are the join, about
-// 10 the first loads and the partial results, and 24 steps of 1.4 us the rest.
+// Bound by the matrix instructions: 16384 x 4096 x 4096 takes 1358 us (1340 to 1390 from run to run), three bf16 products at 1215 TFLOP/s
+// (the card's bf16 matmul of 8192^3 runs at 1154), 405 TFLOP/s of f32; short shares by what surrounds them: 65536 x 256 x 320 takes 54 us,
+// of which 6 are the join, about 10 the first loads and the partial results, and 24 steps of 1.5 us the rest.
 //
 // dst tile of BI x BJ by WI x WJ waves, kStep rows of both operands staged in LDS at a time, two buffers.  LDS holds 16-byte pieces of
 // eight rows of one column, [part][row group][column]: what a lane of the 32x32x16 matrix instruction takes is one piece, and neither
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(WI * WJ * 64) void pack8_matmul_f32_kernel(Product 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 constexpr int kStep64 = 16;
 
-// Bound by the f64 matrix instructions: 8192 x 2048 x 2048 takes 1123 us, 61 TFLOP/s (the card's f64 matmul reaches 73).
+// Bound by the f64 matrix instructions: 8192 x 2048 x 2048 takes 1127 us, 61 TFLOP/s (the card's f64 matmul reaches 73).
 // SIDE x SIDE of dst by WI x WJ waves, the 16x16x4 matrix instruction, kStep64 rows staged at a time, ahead as in the f32 kernel.  The
 // pitch of the staged rows, in words, is 32 more than a multiple of 64: the two rows that half a wave reads lie on the two halves of the
 // banks.
@@ -468,7 +468,7 @@ template <bool EVEN> int32_t f32_any(rt_ctx* ctx, const Product& p, int shape) {
 int32_t run_product(rt_ctx* ctx, int dtype, Product p, void* dst) {
     struct Shape { uint64_t bi, bj, least_rows, per_cu; double rate; };
     // The tile's shape: the larger, the fewer conversions there are for each matrix instruction.  `rate` is what a shape reaches of the
-    // first one's rate on a result it divides (16384 x 4096 x 4096: 1318, 1569 and 1765 us -- the smaller ones are better than that on
+    // first one's rate on a result it divides (16384 x 4096 x 4096, measured together: 1318, 1569 and 1765 us -- the smaller ones are better than that on
     // short shares, hence less weight); the shape with the least padded area at its rate is taken, of those that give every CU a block.
     static const Shape f32[3] = {{256, 256, 512, 1, 1.0}, {256, 128, 256, 1, 0.8}, {128, 128, 64, 2, 0.6}};
     static const Shape f64[2] = {{128, 128, 128, 2, 1.0}, {64, 64, 64, 4, 1.0}};

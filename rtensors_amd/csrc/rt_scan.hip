@@ -62,7 +62,7 @@ template <class T, class S> struct BackArgs {
 };
 
 // One lane per column, the steps one after the other: for a token and a few steps more, where a launch is most of the time ((64, 1, 2048)
-// f32 2.4 us in the kernel), and for so many columns that they fill the card ((2000, 8, 4096) f32 139 us, 5.9 TB/s).
+// f32 2.7 us in the kernel), and for so many columns that they fill the card ((2000, 8, 4096) f32 linear 149 us, 5.5 TB/s).
 template <class T, int FORM>
 __global__ __launch_bounds__(kSBlock) void scan_columns_kernel(ScanArgs<T> a) {
     const uint64_t col = a.col0 + (uint64_t)blockIdx.x * kSBlock + threadIdx.x;
@@ -115,6 +115,8 @@ __global__ __launch_bounds__(kSBlock) void scan_backward_columns_kernel(BackArgs
 }
 
 // ---- tiles along the steps ---------------------------------------------------------------------------------------------------------
+// A prefix scan in one pass with look-back to the tiles before ("Single-pass Parallel Prefix Scan with Decoupled Look-back", Merrill and
+// Garland, 2016), of pairs.
 // Two stretches of the recurrence join as (A1, H1), (A2, H2) -> (A1 A2, A2 H1 + H2): A is the product of a stretch's factors, H what
 // it ends at from a state of zero.  A block takes a tile of the steps for 64 columns, holds it in registers, and needs one thing from
 // the tiles before: the state it starts from.  So that the data are read once, the tiles of a column run in the same launch and hand
@@ -257,7 +259,7 @@ template <class T> struct Apart {
 template <class T, int FORM> using ProductOf = typename std::conditional<FORM == RT_SCAN_LINEAR, Apart<T>, Falling<T>>::type;
 
 // The product of the factors that a lane goes through, multiplied as they come; where a prefix in the wave fell below the range (or a factor
-// is 0), once more with the exponents apart.  (Exponents apart in every step: 51 -> 64 us on (2048, 4097, 1) f64.)
+// is 0), once more with the exponents apart.  (Exponents apart in every step: 64 us in place of 51 on (2048, 4097, 1) f64.)
 __device__ __forceinline__ float least(float a, float b) { return __builtin_fminf(a, __builtin_fabsf(b)); }
 __device__ __forceinline__ double least(double a, double b) { return __builtin_fmin(a, __builtin_fabs(b)); }
 template <class T, class P> struct Running {
@@ -598,7 +600,7 @@ __device__ __forceinline__ uint64_t reset_bits(const uint8_t* flags, int64_t str
 #define RT_PIN_LANE(v) asm volatile("" : "+v"(v))
 
 // W waves of 64 columns, L steps each, in registers: 2 L values a lane, all of them loaded before the first is used, so that the one pass
-// over the data is bound by HBM: (1, 65536, 4096) f32 547 us, 5.9 TB/s; (1, 8192, 1024) 22 us, of which about 7 are the launch and the
+// over the data is bound by HBM: (1, 65536, 4096) f32 linear 542 us, 5.9 TB/s; (1, 8192, 1024) sigmoid 22 us, of which about 7 are the launch and the
 // chain.  Shorter or longer tiles lose to more joins or to fewer blocks.  Lanes behind the last column load what the last column holds, and
 // neither use nor store it.
 template <class T, int FORM, int W, int L, bool ALIGNED>
@@ -710,8 +712,8 @@ template <int L> struct HeldRows {
 };
 struct NoRows {};
 
-// The same backward, five values a step in registers, so half the steps: (8, 2048, 2048) f32 146 us, 5.5 TB/s; from the 8-bit form
-// (1, 50000, 1088) 197 us, 5.0 TB/s, and (1, 50000, 1111) 279 us: there a wave's 64 columns touch three cache lines a row in place of two, two
+// The same backward, five values a step in registers, so half the steps: (8, 2048, 2048) f32 sigmoid 147 us, 5.5 TB/s; from the 8-bit form
+// (1, 50000, 1088) 196 us, 5.0 TB/s, and (1, 50000, 1111) 277 us: there a wave's 64 columns touch three cache lines a row in place of two, two
 // code lines in place of one, and neighbours share few of them (1.7 times the reads).  Position r counts from the last step.  A state's gradient D comes to a step from the one behind it (r - 1) times
 // that one's gate.
 template <class T, int FORM, class S, int W, int L, bool ALIGNED>
@@ -975,7 +977,8 @@ template <class T, class P, class Go> __device__ __forceinline__ T run_lanes(con
 // Segment of a lane: a wave's lanes hold 64 >> shift consecutive ones.
 __device__ __forceinline__ int tile_segment(int tid, uint32_t shift) { return (tid >> 6) * (64 >> shift) + ((tid & 63) >> shift); }
 
-// Bound by the arithmetic and by LDS as much as by memory: (2048, 4097, 1) f64 48 us, 4.1 TB/s, (64, 2^19, 1) f32 101 us, 4.0 TB/s.
+// Half of the waves' cycles are waits, neither memory nor LDS nor the arithmetic is full: (2048, 4097, 1) f64 linear 51 us, 3.9 TB/s,
+// (64, 2^19, 1) f32 linear 100 us, sigmoid 101 us, 4.0 TB/s.
 // Four waves a tile and six on a SIMD, so that there are blocks in every phase; longer tiles for few rows.
 template <class T, int FORM, int W>
 __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void scan_narrow_kernel(ScanArgs<T> a, Chain ch, Narrow nw) {
@@ -1103,7 +1106,7 @@ __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void scan_narrow_kernel(Sc
     }
 }
 
-// Backward: (2048, 8192, 1) f32 linear 75 us, 4.5 TB/s, (100, 50001, 5) f32 sigmoid 185 us, 3.2 TB/s; four waves a tile in place of eight
+// Backward: (2048, 8192, 1) f32 linear 82 us, 4.1 TB/s, (100, 50001, 5) f32 sigmoid 187 us, 3.2 TB/s; four waves a tile in place of eight
 // make that 216 us.  The segments go through the tile from its end.  Only D comes out of the recurrence; the gradients are formed from it element
 // by element afterwards, in memory order.
 template <class T, int FORM, class S, int W>
@@ -1319,9 +1322,9 @@ constexpr uint64_t kWideLeast = 32;             // inner: at least half of a wav
 constexpr uint64_t kWideMost = 1ull << 22;      // inner: a wave's rows are addressed with 32-bit offsets; beyond it columns alone fill the card
 constexpr uint64_t kFewSteps = 8;               // steps that one lane a column goes through without help
 
-// Rows of few columns that are too few to hide the chain's latency take longer tiles.  f32 with 16, 8 and 4 waves a tile: one row of 2^25
-// 296, 636 and 1484 us; 4 rows of 2^23 154, 181 and 395 us; 8 of 2^22 153, 117 and 211 us; 16 of 2^21 153, 107 and 122 us; 32 of 2^20
-// 154, 104 and 102 us.  f64 (16 and 4 waves): 8 rows of 2^21 152 and 222 us; 16 of 2^20 148 and 164 us; 2048 of 4097 100 and 48 us.
+// Rows of few columns that are too few to hide the chain's latency take longer tiles.  Linear, f32 with 16, 8 and 4 waves a tile: one row of
+// 2^25 285, 616 and 1386 us; 4 rows of 2^23 168, 177 and 371 us; 8 of 2^22 170, 119 and 201 us; 16 of 2^21 165, 111 and 122 us; 32 of 2^20
+// 167, 108 and 108 us.  f64 (16 and 4 waves): 8 rows of 2^21 164 and 317 us; 16 of 2^20 159 and 174 us; 2048 of 4097 104 and 52 us.
 constexpr uint64_t kFewRows = 16;
 
 template <class T> bool whole_lines(uint64_t inner) { return inner * sizeof(T) % 128 == 0; }
@@ -1408,7 +1411,7 @@ template <class T> int32_t forward_typed(rt_ctx* ctx, int form, const ScanArgs<T
 
 template <class T, int FORM, class S> int32_t backward_form(rt_ctx* ctx, const BackArgs<T, S>& a) {
     // waves of a wide tile: with the registers of the linear form two blocks of eight fit a CU, of the other one three of four; longer tiles
-    // make shorter chains (linear from the 8-bit form over (1, 50000, 1088): 195 us with four, 164 with eight; the other one 199 and 215)
+    // make shorter chains (linear from the 8-bit form over (1, 50000, 1088): 195 us with four, 169 with eight; the other one 199 and 215)
     constexpr int kWaves = FORM == RT_SCAN_LINEAR ? 8 : 4, kNarrowWaves = 8, L = backward_steps<T>();
     if (by_columns(a.steps, a.inner)) return columns_launches(ctx, a, scan_backward_columns_kernel<T, FORM, S>);
     if (a.inner < kWideLeast) {
