@@ -251,7 +251,7 @@ template <class T> struct Apart {
     static __device__ __forceinline__ Apart of(T f) { return {f, 0}; }
     // m 2^e of any m and e (above the range, e > 0: where a tile's product sinks below the range first, which no wave's own does)
     static __device__ __forceinline__ Apart from(T m, int e) {
-        const int at = e + exponent(m), near = at < kLow ? kLow : at > kTop ? kTop : at;
+        const int at = m == (T)0 ? 0 : e + exponent(m), near = at < kLow ? kLow : at > kTop ? kTop : at;   // 0 times what leaves the range is NaN
         return {scaled(mantissa(m), near), at - near};
     }
     __device__ __forceinline__ T on(T c, T h) const { return fused(m, scaled(c, e), h); }

@@ -254,3 +254,30 @@ def test_gates_that_are_not_finite(hip, shape, form, dtype):
             assert np.array_equal(k(got), k(w)), (name, k)
         fine = np.isfinite(w)
         assert (np.abs(got.astype(w.dtype) - w)[fine] <= bound[fine]).all(), name
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("every", [9, 50, 700])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_zero_gates_among_growing_ones(hip, shape, every, dtype):
+    """The product of a stretch with a zero gate in it is 0 however large its other factors are."""
+    T, up = TYPES[dtype], {"f32": 3, "f64": 20}[dtype]
+    outer, steps, inner = shape
+    gate = np.full(shape, T(2) ** up)
+    gate[:, 5::every] = 0
+    last = max(steps - 3, 0)
+    gate[:, last:] = 1
+    x = np.zeros(shape, T)
+    x[:, last:] = 3
+    d = {"gate": gate, "x": x, "state": np.ones((outer, inner), T), "reset": None}
+    d["dlast"] = d["state"]
+    h, end = run_forward(hip, "linear", d)
+    want, p = np.zeros(shape, T), d["state"]
+    for t in range(steps):
+        p = gate[:, t] * p + x[:, t]
+        want[:, t] = p
+    assert (h == want).all() and (end == want[:, -1]).all()
+    d["dh"] = np.ascontiguousarray(x[:, ::-1])
+    d["gate"] = np.ascontiguousarray(np.concatenate([gate[:, :1], gate[:, 1:][:, ::-1]], axis=1))
+    got, wish = backward(hip, d, h), plain_backward(d, h)
+    assert np.isfinite(wish[1]).all() and (got[1] == wish[1]).all() and (got[2] == wish[2]).all()
