@@ -874,22 +874,22 @@ template <class T, class P> struct Prefix {
 };
 // Whether the wave runs its segments one after the other: `odd` of a lane, or, with SUMS, a sum over several lanes that left the range.  One
 // that was not finite on the way has stayed so; unless a lane's own that is not, or NaN among the factors (`given`, and not odd), is part of
-// it, its terms are finite.
-template <bool SUMS, class T> __device__ __forceinline__ bool any_odd(bool odd, T H, bool given, bool cut, int lane, uint32_t shift) {
-    bool over = SUMS && !finite(H);
-    const bool any = __any(odd || over);
+// it, its terms are finite.  And one that is NaN without a lane's own that is (`nan`) may have met an infinity that left the range.
+template <bool SUMS, class T> __device__ __forceinline__ bool any_odd(bool odd, T H, bool given, bool nan, bool cut, int lane, uint32_t shift) {
+    const bool over = SUMS && !finite(H), any = __any(odd || over);
     if (!SUMS || !any) return any;
     for (uint32_t d = 1u << shift; d < 64; d <<= 1) {
-        const int below = __shfl_up((given ? 2 : 0) | (cut ? 1 : 0), d);
-        if (lane >= (int)d) {
-            given = given || (!cut && (below & 2));
-            cut = cut || (below & 1);
+        const int below = __shfl_up((nan ? 4 : 0) | (given ? 2 : 0) | (cut ? 1 : 0), d);
+        if (lane >= (int)d && !cut) {
+            given = given || (below & 2);
+            nan = nan || (below & 4);
+            cut = below & 1;
         }
     }
-    return __any(odd || (over && !given));
+    return __any(odd || (over && !given) || (H != H && !nan));
 }
 template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Falling<T>> join_lanes(Falling<T> A, T H, bool cut, bool odd, int lane, uint32_t shift) {
-    const bool given = !finite(H) || A.m != A.m, own_cut = cut;
+    const bool nan = H != H || A.m != A.m, given = nan || !finite(H), own_cut = cut;
     if (cut) A.m = (T)0;
     for (uint32_t d = 1u << shift; d < 64; d <<= 1) {
         const T A1 = __shfl_up(A.m, d), H1 = __shfl_up(H, d);
@@ -905,7 +905,7 @@ template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Falling<T>> j
     p.wholeA = {__shfl(A.m, top)};
     p.wholeH = __shfl(H, top);
     p.any_cut = __any(cut);
-    p.odd = any_odd<SUMS>(odd, H, given, own_cut, lane, shift);
+    p.odd = any_odd<SUMS>(odd, H, given, nan, own_cut, lane, shift);
     const T A0 = __shfl_up(A.m, 1u << shift), H0 = __shfl_up(H, 1u << shift);
     const bool c0 = __shfl_up((int)cut, 1u << shift) != 0;
     const bool head = lane < (1 << shift);
@@ -920,7 +920,7 @@ template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Apart<T>> joi
     T m = mantissa(A.m) * (T)2;
     int e = exponent(A.m) + A.e - 1;
     odd = odd || (!cut && infinite(m));
-    const bool given = !finite(H) || m != m, own_cut = cut;
+    const bool nan = H != H || m != m, given = nan || !finite(H), own_cut = cut;
     for (uint32_t d = 1u << shift; d < 64; d <<= 1) {
         const T m1 = __shfl_up(m, d), H1 = __shfl_up(H, d);
         const int both = __shfl_up(e * 2 + (cut ? 1 : 0), d);
@@ -942,7 +942,7 @@ template <bool SUMS, class T> __device__ __forceinline__ Prefix<T, Apart<T>> joi
     p.wholeA = {__shfl(a.m, top), __shfl(a.e, top)};
     p.wholeH = __shfl(H, top);
     p.any_cut = __any(cut);
-    p.odd = any_odd<SUMS>(odd, H, given, own_cut, lane, shift);
+    p.odd = any_odd<SUMS>(odd, H, given, nan, own_cut, lane, shift);
     const T m0 = __shfl_up(a.m, 1u << shift), H0 = __shfl_up(H, 1u << shift);
     const int both = __shfl_up(a.e * 2 + (cut ? 1 : 0), 1u << shift);
     const bool head = lane < (1 << shift);

@@ -281,3 +281,23 @@ def test_zero_gates_among_growing_ones(hip, shape, every, dtype):
     d["gate"] = np.ascontiguousarray(np.concatenate([gate[:, :1], gate[:, 1:][:, ::-1]], axis=1))
     got, wish = backward(hip, d, h), plain_backward(d, h)
     assert np.isfinite(wish[1]).all() and (got[1] == wish[1]).all() and (got[2] == wish[2]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("first", [np.inf, -np.inf])
+@pytest.mark.parametrize("shape", SHAPES + [(1, 9, 3), (9, 33, 2), (13, 25, 1)])
+def test_an_infinity_before_pairs_that_overflow(hip, shape, first, dtype):
+    """An infinite state stays what it is over x of -c and c in pairs, whose sums from a start of zero are infinities of either sign."""
+    T = TYPES[dtype]
+    outer, steps, inner = shape
+    c = T(0.9) * np.finfo(T).max
+    x = np.zeros(shape, T)
+    x[:, 1:] = np.where(np.arange(steps - 1) % 4 < 2, c, -c)[None, :, None]
+    x[:, 0] = first
+    d = {"gate": np.ones(shape, T), "x": x, "state": np.zeros((outer, inner), T), "reset": None, "dh": np.ascontiguousarray(x[:, ::-1])}
+    d["dlast"] = d["state"]
+    h, last = run_forward(hip, "linear", d)
+    assert (h == first).all() and (last == first).all()
+    small = np.full(shape, T(2) ** -100)
+    got = backward(hip, d, small)
+    assert (got[1] == first).all() and (got[2] == first).all()
