@@ -245,7 +245,7 @@ template <class T> struct Apart {
     static constexpr bool kApart = true;
     static constexpr T kNormal = sizeof(T) == 4 ? (T)0x1p-126 : (T)0x1p-1022;
     static constexpr int kLow = sizeof(T) == 4 ? -125 : -1021, kTop = sizeof(T) == 4 ? 128 : 1024;
-    static constexpr int kDead = sizeof(T) == 4 ? -300 : -2200;  // below, A c is 0 for every number c
+    static constexpr int kDead = sizeof(T) == 4 ? -300 : -2200;  // below, A c is 0 for every number c (an infinite one stays infinite)
     T m;
     int e;
     static __device__ __forceinline__ Apart of(T f) { return {f, 0}; }
@@ -323,13 +323,13 @@ template <class T, int W, int LN, class P> struct JoinRoom {
     uint32_t cut[W];                                             // 1: cut, 2: odd, 4: deep
     uint32_t tile;
     int found;
-    // a wave's product and its exponent: that of m 2^e as a whole, kZero for 0 and NaN, and those from -2^15 on are all the same: the other waves of
-    // a tile lift no state again that far
-    static constexpr int kZero = 1 << 14;
+    // a wave's product and its exponent: that of m 2^e as a whole, kNone for 0 and NaN, and those from -2^15 on are all the same: the other
+    // waves of a tile lift no state again that far
+    static constexpr int kNone = 32767;
     __device__ __forceinline__ void put(int w, int l, const P& a) {
         A[w][l] = a.m;
         if constexpr (P::kApart) {
-            const int e = a.m == (T)0 || a.m != a.m ? kZero : a.e + exponent(a.m);
+            const int e = a.m == (T)0 || a.m != a.m ? kNone : a.e + exponent(a.m);
             E[w][l] = (int16_t)(e < -32768 ? -32768 : e);
         }
     }
@@ -526,10 +526,15 @@ __device__ __forceinline__ T join_tile(const Chain& ch, JoinRoom<T, W, LN, P>& r
     if constexpr (P::kApart)
         if (w == 0 && !last && !serial && !tcut && (deep || __any(low < P::kNormal))) {  // with the exponents apart
             int e = 0;
+            bool none = false;                                   // 0 or NaN, of which something is left
 #pragma unroll
-            for (int v = 0; v < W; ++v) e += room.E[v][lane & (LN - 1)];
-            whole = {with_sign(P::kNormal, ta), e};              // nothing is left of any state
-            if (__any(e > P::kDead)) {
+            for (int v = 0; v < W; ++v) {
+                const int ev = room.E[v][lane & (LN - 1)];
+                e += ev;
+                none = none || ev == room.kNone;
+            }
+            whole = {with_sign(P::kNormal, ta), e};              // nothing is left of any number
+            if (__any(e > P::kDead || none)) {
                 T p = (T)1;
                 e = 0;
 #pragma unroll 4

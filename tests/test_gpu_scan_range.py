@@ -301,3 +301,27 @@ def test_an_infinity_before_pairs_that_overflow(hip, shape, first, dtype):
     small = np.full(shape, T(2) ** -100)
     got = backward(hip, d, small)
     assert (got[1] == first).all() and (got[2] == first).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what", [np.nan, 0.0])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_nan_and_zero_gates_among_very_small_ones(hip, shape, what, dtype):
+    """Nothing is left of a state behind a few gates near the smallest number, but NaN is, and an infinite state is NaN behind a gate of 0;
+    also where the gate is a tile's first one."""
+    T = TYPES[dtype]
+    outer, steps, inner = shape
+    gate = np.full(shape, np.finfo(T).tiny)
+    starts = np.array([128, 256, 512, 640, 1024, 2048, 0, 8, 16, 32, 64, 4096])
+    column = np.arange(outer * inner).reshape(outer, inner)
+    first = starts[column % starts.size] % steps
+    o, i = np.indices((outer, inner))
+    gate[o, first, i] = what
+    d = {"gate": gate, "x": np.ones(shape, T), "state": np.full((outer, inner), 1 if np.isnan(what) else np.inf, T), "reset": None}
+    d["dlast"], d["dh"] = d["state"], d["x"]
+    want = np.arange(steps)[None, :, None] >= first[:, None]
+    h, last = run_forward(hip, "linear", d)
+    assert np.array_equal(np.isnan(h), want) and np.isnan(last).all()
+    got = backward(hip, d, np.ones(shape, T))
+    before = np.arange(steps)[None, :, None] < first[:, None]       # the gate of a step is that of the state before it
+    assert np.array_equal(np.isnan(got[1]), before) and np.isnan(got[2]).all()
