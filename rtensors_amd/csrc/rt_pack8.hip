@@ -71,7 +71,7 @@ template <int OP, class T> __device__ __forceinline__ T slope_of(T x) {
 
 // Codes and exponents of a run, and op of it (OP != kNoOp): a lane has four neighbouring elements a vector, so a group is eight lanes and
 // its maximum three lane exchanges.  Bound by HBM: 2^28 f32 200 us in the kernel, 6.7 TB/s; silu of 2^26 f32 forward and backward 179 us,
-// 6.8 TB/s of which the Infinity Cache takes the codes; 2^16 elements 2.7 us in the kernel, a launch.
+// 6.8 TB/s of which the Infinity Cache takes the codes; 2^16 elements 2.6 us in the kernel, a launch.
 template <class T, int OP>
 __global__ __launch_bounds__(kPBlock) void pack8_kernel(const T* src, T* dst, int8_t* __restrict__ codes, uint8_t* __restrict__ exps, uint64_t len) {
     typedef typename std::conditional<sizeof(T) == 4, uint32_t, uint64_t>::type U;

@@ -62,7 +62,7 @@ template <class T, class S> struct BackArgs {
 };
 
 // One lane per column, the steps one after the other: for a token and a few steps more, where a launch is most of the time ((64, 1, 2048)
-// f32 2.7 us in the kernel), and for so many columns that they fill the card ((2000, 8, 4096) f32 linear 149 us, 5.5 TB/s).
+// f32 2.8 us in the kernel), and for so many columns that they fill the card ((2000, 8, 4096) f32 linear 149 us, 5.5 TB/s).
 template <class T, int FORM>
 __global__ __launch_bounds__(kSBlock) void scan_columns_kernel(ScanArgs<T> a) {
     const uint64_t col = a.col0 + (uint64_t)blockIdx.x * kSBlock + threadIdx.x;
